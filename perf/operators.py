@@ -4,7 +4,7 @@ user's program makes, and their values in 64 bits.
 
   grouped_matmul        C[rows of e] = A[rows of e] · B[e]          (f16 / bf16)
   grouped_matmul_wgrad  G[e] = A[rows of e]^T · D[rows of e]        (f16 / bf16)
-  quantize_fp8          S = max(max|block| / 448, 2^-63) in f32, Q = e4m3(X / S)
+  quantize_fp8          S = m / 448, Q = e4m3(448 X / m), m = max(max|block|, 448 · 2^-63)
   matmul_fp8            C = Σ_b SA[·, b] SB[b, ·] (A_b · B_b), b = blocks of 128 along K
   grouped_matmul_fp8    the same for the rows of each expert
 
@@ -202,14 +202,16 @@ def _blocks(case):
 
 
 def _quantize(x, br, bc):
-    """(X / S in f32, to be rounded to e4m3, and S in f32)."""
+    """(448 X / m in f32, to be rounded to e4m3, and S in f32). 448 X is taken as 1.75 X, against m / 256: exact for
+    16-bit X, so that a quotient on the border between two e4m3 values comes out on it."""
     *lead, r, c = x.shape
     rb, cb = -(-r // br), -(-c // bc)
     p = torch.nn.functional.pad(x.float(), (0, cb * bc - c, 0, rb * br - r))
     p = p.view(*lead, rb, br, cb, bc)
-    most = p.abs().amax(dim=(-3, -1))
-    s = torch.clamp(most / torch.full_like(most, _MAX), min=_LEAST)  # a tensor divisor: torch multiplies by 1 / number
-    return (p / s[..., :, None, :, None]).view(*lead, rb * br, cb * bc)[..., :r, :c], s
+    most = p.abs().amax(dim=(-3, -1)).clamp(min=_MAX * _LEAST)
+    s = most / torch.full_like(most, _MAX)  # a tensor divisor: torch multiplies by 1 / number
+    q = (p * (_MAX / 256)) / (most / 256)[..., :, None, :, None]
+    return q.view(*lead, rb * br, cb * bc)[..., :r, :c], s
 
 
 def _values(q, s):
@@ -330,10 +332,9 @@ def exact(case, seed):
         b = x.new_zeros(-(-r // br) * br, -(-c // bc) * bc)
         b[:r, :c] = x
         most = b.abs().reshape(b.shape[0] // br, br, -1, bc).permute(0, 2, 1, 3).flatten(2).max(dim=2).values
-        scale = torch.clamp(most / _MAX, min=_LEAST)
-        stored = scale.float().double()  # Q goes by the scale as it is kept
-        over = stored.repeat_interleave(br, 0)[:r].repeat_interleave(bc, 1)[:, :c]
-        return {"q": _e4m3_64(torch.clamp(x / over, -_MAX, _MAX)), "s": scale}
+        most = torch.clamp(most, min=_MAX * _LEAST)
+        over = most.repeat_interleave(br, 0)[:r].repeat_interleave(bc, 1)[:, :c]
+        return {"q": _e4m3_64(x * _MAX / over), "s": most / _MAX}
     if op == "fp8":
         gradient = case["form"] == "weight gradient"
         a = _spread64(s["a"], s["sa"], 1, 128)

@@ -202,15 +202,15 @@ def _blocks(case):
 
 
 def _quantize(x, br, bc):
-    """(448 X / m in f32, to be rounded to e4m3, and S in f32). 448 X is taken as 1.75 X, against m / 256: exact for
-    16-bit X, so that a quotient on the border between two e4m3 values comes out on it."""
+    """(448 X / m in f32, to be rounded to e4m3, and S in f32). 448 X is taken as 0.4375 X, against m / 1024: exact for
+    16-bit X and never infinite, so that a quotient on the border between two e4m3 values comes out on it."""
     *lead, r, c = x.shape
     rb, cb = -(-r // br), -(-c // bc)
     p = torch.nn.functional.pad(x.float(), (0, cb * bc - c, 0, rb * br - r))
     p = p.view(*lead, rb, br, cb, bc)
     most = p.abs().amax(dim=(-3, -1)).clamp(min=_MAX * _LEAST)
     s = most / torch.full_like(most, _MAX)  # a tensor divisor: torch multiplies by 1 / number
-    q = (p * (_MAX / 256)) / (most / 256)[..., :, None, :, None]
+    q = (p * (_MAX / 1024)) / (most / 1024)[..., :, None, :, None]
     return q.view(*lead, rb * br, cb * bc)[..., :r, :c], s
 
 

@@ -49,7 +49,7 @@ typedef enum tbStatus {
 } tbStatus;
 
 /* Element types (memref element types of A, B and C). */
-typedef enum tbDtype { TB_F16 = 0, TB_F32 = 1, TB_BF16 = 2 } tbDtype;
+typedef enum tbDtype { TB_F16 = 0, TB_F32 = 1, TB_BF16 = 2, TB_E4M3 = 3 } tbDtype;
 
 /* tb.reduction-mode (ProgramMappingPlan.h:37-41). UNSET means the attribute
  * is absent, which the reference resolves to split_k_serial
@@ -322,6 +322,110 @@ tbStatus tb_matmul_plan_for_shape(const tb_matmul_plan* plan, int64_t m, int64_t
 tbStatus tb_matmul(const tb_matmul_desc* desc, const void* A, int64_t lda,
                    const void* B, int64_t ldb, void* C, int64_t ldc,
                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- Products of rows grouped by expert, and of 8-bit operands ----
+ * No counterpart in the reference, whose one op is a dense f16 product. These
+ * calls take no plan: the desc is checked on every call, nothing is kept
+ * between calls, and the group sizes are read on the device. They run on the
+ * current device, which must be the stream's and the operands'.
+ *
+ * `rows` rows of A and C belong to `groups` groups: group e has the rows
+ * [offsets[e], offsets[e + 1]). `offsets` are groups + 1 non-decreasing
+ * entries on the device (int32_t, or int64_t with offsets_long), read when
+ * the kernel runs, so a captured graph follows their contents. Groups may be
+ * empty. Rows before offsets[0] and behind offsets[groups] are neither read
+ * into a result nor written. Entries outside [0, rows] are clamped to it, so
+ * that wrong offsets give wrong results but touch no other memory.
+ *
+ * Rows of an operand that do not begin on 16-byte boundaries (base, leading
+ * dimension or group stride) are first copied into `workspace`, 256-byte
+ * aligned; the *_workspace_bytes functions say how much that takes for the
+ * operands that they are given (0 in the ordinary case, then workspace may be
+ * NULL). Sums are in f32; the output is rounded once. Results repeat bit for
+ * bit (no atomics). beta = 0 does not read the output. */
+typedef struct tb_grouped_desc {
+  int64_t groups;                  /* 0 … 1024; 1 for tb_matmul_blockscaled */
+  int64_t rows;                    /* rows of A and C, over all groups */
+  int64_t n, k;                    /* B of a group: k × n */
+  int32_t ab_dtype;                /* TB_F16 or TB_BF16; *_blockscaled: TB_E4M3 */
+  int32_t c_dtype;                 /* TB_F32, TB_F16 or TB_BF16 */
+  int32_t beta;                    /* 1: add to the output's contents; 0: overwrite */
+  int32_t a_col_major;             /* tb_matmul_blockscaled only: A stored k × rows */
+  int32_t b_col_major;             /* 1: B stored n × k (k contiguous) */
+  int32_t offsets_long;            /* offsets are int64_t */
+} tb_grouped_desc;
+
+/* groups = 1, f16 operands, f32 output, beta = 1, the rest 0. */
+tbStatus tb_grouped_desc_init(tb_grouped_desc* desc);
+
+/* C[r, :] = beta·C[r, :] + A[r, :] · B[e] for the rows r of every group e.
+ * A: rows × k, row stride lda; B: groups matrices stride_b elements apart,
+ * k × n with row stride ldb >= n, or (b_col_major) n × k with ldb >= k; C:
+ * rows × n, row stride ldc. The gradient of A is the same call with C's
+ * gradient for A and the other storage order of the same weights. */
+tbStatus tb_grouped_matmul(const tb_grouped_desc* desc, const void* A, int64_t lda,
+                           const void* B, int64_t ldb, int64_t stride_b, void* C,
+                           int64_t ldc, const void* offsets, void* workspace,
+                           size_t workspace_bytes, void* stream);
+size_t tb_grouped_matmul_workspace_bytes(const tb_grouped_desc* desc, const void* A,
+                                         int64_t lda, const void* B, int64_t ldb,
+                                         int64_t stride_b);
+
+/* G[e] = beta·G[e] + A[rows of e]^T · D[rows of e]: the gradient of B from
+ * C's gradient D. A: rows × k, D: rows × n, G: groups matrices k × n, row
+ * stride ldg, stride_g elements apart. An empty group's G is beta·G. */
+tbStatus tb_grouped_matmul_wgrad(const tb_grouped_desc* desc, const void* A, int64_t lda,
+                                 const void* D, int64_t ldd, void* G, int64_t ldg,
+                                 int64_t stride_g, const void* offsets, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+size_t tb_grouped_matmul_wgrad_workspace_bytes(const tb_grouped_desc* desc, const void* A,
+                                               int64_t lda, const void* D, int64_t ldd);
+
+/* Scales of an 8-bit operand: one f32 for `block` (1 or 128) rows of A or
+ * columns of B and 128 elements along k. The scale of row / column i in
+ * k-block b is ptr[(i / block)·stride_mn + b·stride_k], of group e + e·stride_group
+ * (B of a grouped product). */
+typedef struct tb_scales {
+  const float* ptr;
+  int64_t stride_group, stride_mn, stride_k;
+  int32_t block;
+} tb_scales;
+
+/* C = beta·C + Σ_b SA[:, b] SB[b, :] (A_b · B_b), b = blocks of 128 along k
+ * (the last may be short). A: rows × k (or a_col_major), B: k × n (or
+ * b_col_major), e4m3; the product of two scales must be a finite f32. Any
+ * pairing of storage orders and scale extents is allowed: rows × 128 and
+ * 128 × 128 blocks for a layer and its input gradient, 128 × 1 blocks of both
+ * sides for its weight gradient. */
+tbStatus tb_matmul_blockscaled(const tb_grouped_desc* desc, const void* A, int64_t lda,
+                               const tb_scales* sa, const void* B, int64_t ldb,
+                               const tb_scales* sb, void* C, int64_t ldc, void* workspace,
+                               size_t workspace_bytes, void* stream);
+/* The same for the rows of each group: A with a scale per row, B[e] with
+ * 1 or 128 columns to a scale. Workspace of both: tb_grouped_matmul_workspace_bytes. */
+tbStatus tb_grouped_matmul_blockscaled(const tb_grouped_desc* desc, const void* A, int64_t lda,
+                                       const tb_scales* sa, const void* B, int64_t ldb,
+                                       int64_t stride_b, const tb_scales* sb, void* C,
+                                       int64_t ldc, const void* offsets, void* workspace,
+                                       size_t workspace_bytes, void* stream);
+
+/* ---- 8-bit operands ----
+ * m = max(max |block|, 448 · 2^-63), S = m / 448, Q = e4m3(448 · X / m), the
+ * quotient rounded to nearest, ties to even. X: batch matrices of rows × cols
+ * (f32, f16 or bf16), row stride ldx; Q: e4m3, row stride ldq; S: f32,
+ * ceil(rows / block_rows) × ceil(cols / block_cols) with strides s_row and
+ * s_col. Matrices of the batch lie stride_x, stride_q and stride_s elements
+ * apart. A NaN makes its whole block NaN; an infinity makes the block's scale
+ * infinite, its Q NaN at the infinities and 0 elsewhere. X may not overlap Q. */
+typedef struct tb_quantize_desc {
+  int64_t batch, rows, cols;
+  int64_t block_rows, block_cols;  /* 1 × 128, 128 × 1 or 128 × 128 */
+  int32_t x_dtype;                 /* TB_F32, TB_F16 or TB_BF16 */
+} tb_quantize_desc;
+tbStatus tb_quantize_blocks(const tb_quantize_desc* desc, const void* X, int64_t ldx,
+                            int64_t stride_x, void* Q, int64_t ldq, int64_t stride_q,
+                            float* S, int64_t stride_s, int64_t s_row, int64_t s_col,
+                            void* stream);
 
 /* Reads and clears the device status word the kernels set when a bounded
  * wait gives up (TB_ERR_DEVICE_TIMEOUT) — synchronises `stream`. The reference

@@ -45,7 +45,8 @@ class _LazyLib:
 
 _lib = _LazyLib()
 
-__all__ = ["KernelConfig", "MatmulPlan", "DynamicMatmulPlan", "TBError", "matmul", "plan_for", "version", "lib"]
+__all__ = ["KernelConfig", "MatmulPlan", "DynamicMatmulPlan", "TBError", "matmul", "plan_for", "version", "lib",
+           "grouped_matmul", "grouped_matmul_wgrad", "quantize_fp8", "matmul_fp8", "grouped_matmul_fp8"]
 
 _REDUCTION = {None: TB_REDUCTION_UNSET, "": TB_REDUCTION_UNSET,
               "split_k_serial": TB_REDUCTION_SPLIT_K_SERIAL,
@@ -406,3 +407,15 @@ def device_status(stream=None) -> int:
     code = _lib.tb_device_status(C.c_void_p(s.cuda_stream or None), C.byref(raw))
     _check(code)
     return raw.value
+
+
+_GROUPED = ("grouped_matmul", "grouped_matmul_wgrad", "quantize_fp8", "matmul_fp8", "grouped_matmul_fp8")
+
+
+def __getattr__(name):
+    # grouped.py imports torch, which this module does only inside its calls
+    if name in _GROUPED:
+        from . import grouped
+        globals().update({n: getattr(grouped, n) for n in _GROUPED})
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -20,7 +20,7 @@ TB_ERR_DEVICE_TIMEOUT = 4
 TB_ERR_WORKSPACE = 5
 TB_ERR_NCCL = 6
 
-TB_F16, TB_F32, TB_BF16 = 0, 1, 2
+TB_F16, TB_F32, TB_BF16, TB_E4M3 = 0, 1, 2, 3
 TB_REDUCTION_UNSET, TB_REDUCTION_SPLIT_K_SERIAL, TB_REDUCTION_SPLIT_K_PARALLEL = 0, 1, 2
 TB_ACT_NONE, TB_ACT_RELU, TB_ACT_SILU, TB_ACT_GELU_TANH = 0, 1, 2, 3
 ACTIVATIONS = {None: TB_ACT_NONE, "relu": TB_ACT_RELU, "silu": TB_ACT_SILU, "gelu_tanh": TB_ACT_GELU_TANH}
@@ -75,6 +75,24 @@ class tb_peer_handle(C.Structure):
     _fields_ = [("rows_ipc", C.c_ubyte * 64), ("rows_offset", C.c_int64), ("flags_ipc", C.c_ubyte * 64)]
 
 
+class tb_grouped_desc(C.Structure):
+    _fields_ = [
+        ("groups", C.c_int64), ("rows", C.c_int64), ("n", C.c_int64), ("k", C.c_int64),
+        ("ab_dtype", C.c_int32), ("c_dtype", C.c_int32), ("beta", C.c_int32),
+        ("a_col_major", C.c_int32), ("b_col_major", C.c_int32), ("offsets_long", C.c_int32),
+    ]
+
+
+class tb_scales(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("stride_group", C.c_int64), ("stride_mn", C.c_int64),
+                ("stride_k", C.c_int64), ("block", C.c_int32)]
+
+
+class tb_quantize_desc(C.Structure):
+    _fields_ = [("batch", C.c_int64), ("rows", C.c_int64), ("cols", C.c_int64),
+                ("block_rows", C.c_int64), ("block_cols", C.c_int64), ("x_dtype", C.c_int32)]
+
+
 # Every symbol include/tb_gemm.h declares, with its ctypes prototype.
 PROTOTYPES = {
     "tb_matmul_desc_init": (C.c_int, [C.POINTER(tb_matmul_desc)]),
@@ -121,6 +139,27 @@ PROTOTYPES = {
     "tb_matmul_run_kshard_nccl": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p,
                                             C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_size_t,
                                             C.c_void_p]),
+    "tb_grouped_desc_init": (C.c_int, [C.POINTER(tb_grouped_desc)]),
+    "tb_grouped_matmul": (C.c_int, [C.POINTER(tb_grouped_desc), C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                    C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_size_t,
+                                    C.c_void_p]),
+    "tb_grouped_matmul_workspace_bytes": (C.c_size_t, [C.POINTER(tb_grouped_desc), C.c_void_p, C.c_int64,
+                                                       C.c_void_p, C.c_int64, C.c_int64]),
+    "tb_grouped_matmul_wgrad": (C.c_int, [C.POINTER(tb_grouped_desc), C.c_void_p, C.c_int64, C.c_void_p,
+                                          C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p,
+                                          C.c_size_t, C.c_void_p]),
+    "tb_grouped_matmul_wgrad_workspace_bytes": (C.c_size_t, [C.POINTER(tb_grouped_desc), C.c_void_p, C.c_int64,
+                                                             C.c_void_p, C.c_int64]),
+    "tb_matmul_blockscaled": (C.c_int, [C.POINTER(tb_grouped_desc), C.c_void_p, C.c_int64, C.POINTER(tb_scales),
+                                        C.c_void_p, C.c_int64, C.POINTER(tb_scales), C.c_void_p, C.c_int64,
+                                        C.c_void_p, C.c_size_t, C.c_void_p]),
+    "tb_grouped_matmul_blockscaled": (C.c_int, [C.POINTER(tb_grouped_desc), C.c_void_p, C.c_int64,
+                                                C.POINTER(tb_scales), C.c_void_p, C.c_int64, C.c_int64,
+                                                C.POINTER(tb_scales), C.c_void_p, C.c_int64, C.c_void_p,
+                                                C.c_void_p, C.c_size_t, C.c_void_p]),
+    "tb_quantize_blocks": (C.c_int, [C.POINTER(tb_quantize_desc), C.c_void_p, C.c_int64, C.c_int64, C.c_void_p,
+                                     C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int64,
+                                     C.c_void_p]),
     "tb_selftest_bounded_wait": (C.c_int, [C.c_void_p, C.c_uint64]),
     "tb_device_status": (C.c_int, [C.c_void_p, C.POINTER(C.c_uint32)]),
     "tb_last_error": (C.c_char_p, []),

@@ -17,8 +17,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libtbgemm.so"
 
-SOURCES = ["tb_plan.cpp", "tb_dynamic.cpp", "tb_shard.cpp", "tb_launch.cu", "tb_peer.cu", "tb_nccl.cpp"]
-HEADERS = ["tb_plan.h", "tb_mapping.h", "tb_sm100.cuh"]
+SOURCES = ["tb_plan.cpp", "tb_dynamic.cpp", "tb_shard.cpp", "tb_launch.cu", "tb_grouped.cu", "tb_quantize.cu", "tb_peer.cu", "tb_nccl.cpp"]
+HEADERS = ["tb_plan.h", "tb_mapping.h", "tb_sm100.cuh", "tb_wait.cuh"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

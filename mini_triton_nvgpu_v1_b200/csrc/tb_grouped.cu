@@ -1,0 +1,1208 @@
+// tb_grouped.cu — matrix products whose rows belong to groups (experts) and
+// matrix products of 8-bit operands with a scale per block of 128.
+//
+//   rows grouped   C[r, :] = beta·C[r, :] + A[r, :] · B[e]     r in group e
+//   K grouped      G[e] = beta·G[e] + A[rows of e]^T · D[rows of e]
+//   8-bit          C = beta·C + Σ_b SA[:, b] SB[b, :] (A_b · B_b), b = blocks of 128 along K
+//
+// One kernel family, tb_grouped_sm100_kernel<KIND, BN, G>, in the manner of
+// the dense GEMM: persistent, warp-specialised, TMA into a ring of 128-byte
+// rows, tcgen05.mma into two TMEM accumulators, an epilogue that overlaps the
+// next accumulation. Group sizes are read on the device (the offsets are a
+// router's output), so no call waits for the host to learn them:
+// every CTA builds the table of tiles from the offsets when it starts.
+//
+//   warp 0      TMA producer           warp 2   row fixer (K grouped)
+//   warp 1      MMA issuer             warps 4-11  epilogue, two per lane quarter
+//
+// Rows grouped: a tile's rows begin at any row of A (a TMA coordinate other
+// than the innermost has no alignment rule); the rows past the group's end
+// are other groups' rows, whose results are not stored. A row of the result
+// depends on that row of A alone, so nothing of them can leak.
+//
+// K grouped: the K range of a tile is a range of rows, which ends anywhere
+// inside the last ring fill. Rows behind it up to the next multiple of the
+// MMA's K step would add another group's products, so the fixer warp zeroes
+// them in shared memory, in both operands (0 · NaN is NaN), between the
+// TMA's arrival and the MMA; all other fills go from TMA to MMA directly.
+//
+// 8-bit: one ring fill is one block of 128 along K, and one accumulation in
+// TMEM. The epilogue warps take each block's sums from TMEM, scale them and
+// add them to f32 registers while the MMAs of the next block run into the
+// other accumulator. The sum of 128 products of two e4m3 values is held in
+// f32 by the MMA, and the sum over blocks in f32 registers.
+//
+// Few tiles (a decoding step): the K range is split over the CTAs of a
+// cluster, which add their partial sums through distributed shared memory in
+// a fixed order — no workspace, no atomics, results repeat bit for bit.
+//
+// Every wait is bounded, as in the dense GEMM.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cstring>
+#include <string>
+
+#include "tb_plan.h"
+#include "tb_sm100.cuh"
+#include "tb_wait.cuh"
+
+using namespace tb::sm100;
+
+namespace {
+
+constexpr int kThreadsG = 384;
+constexpr int kMaxGroups = 1024;
+constexpr int kMaxStages = 10;
+constexpr size_t kSmemLimitG = 232448;  // 227 KB opt-in per CTA
+
+enum Kind : int { kHalf = 0, kByte = 1 };  // 16-bit operands (f16 / bf16), 8-bit operands (e4m3)
+
+// KIND's ring fill is 128 bytes of K: 64 or 128 elements, four MMA K steps.
+template <int KIND, int BN, int G>
+struct GCfg {
+  static constexpr int kEl = KIND == kByte ? 1 : 2;
+  static constexpr int kKB = 128 / kEl;                 // K elements per fill
+  static constexpr int kMmaK = 32 / kEl;                // K elements per MMA
+  static constexpr int kBM = 128 * G;                   // tile rows
+  static constexpr int kBnCta = BN / G;                 // B columns a CTA loads
+  static constexpr uint32_t kABytes = 128 * 128;
+  static constexpr uint32_t kBBytes = kBnCta * 128;
+  static constexpr uint32_t kStageBytes = kABytes + kBBytes;
+  static constexpr int kMnBox = 128 / kEl;              // columns of an MN-major box
+  static constexpr uint32_t kMnBoxBytes = kKB * 128;
+  static constexpr uint32_t kMnStep = kMmaK * 128;      // bytes per MMA K step, MN-major
+  static constexpr int kAccs = 2;
+  static constexpr uint32_t kTmemCols = kAccs * BN;
+  static constexpr int kHalfCols = BN / 2;              // columns per epilogue warp
+  static constexpr int kChunks = kHalfCols / 32;
+  static constexpr uint32_t kRedStride = (BN + 4) * 4;  // bytes per row of the cluster's partial sums
+  static constexpr uint32_t kRedBytes = 128 * kRedStride;
+};
+
+// Tiles of every group, built by each CTA from the offsets.
+struct GroupTable {
+  int32_t start[kMaxGroups];
+  int32_t rows[kMaxGroups];
+  int32_t cum[kMaxGroups + 1];  // rows grouped: tiles before group e
+};
+
+struct GBars {
+  uint64_t full[kMaxStages], empty[kMaxStages], fix[kMaxStages];
+  uint64_t tfull[2], tempty[2];
+  uint64_t drain, ready, consumed;
+  uint32_t tmem_holder;
+  int abort_flag;
+};
+
+constexpr size_t kTailBytes = sizeof(GroupTable) + sizeof(GBars) + 64;
+
+struct GScale {           // scale of element (mn, k-block b): p[(mn >> shift)·smn + b·sk], per group + sg
+  const float* p;
+  int64_t sg, smn, sk;
+  int32_t shift;          // 7: one scale per 128 rows / columns; 0: per row / column
+};
+
+struct GParams {
+  int32_t k_grouped;      // 1: K ranges are the groups (weight gradient)
+  int32_t groups;
+  int32_t M, N, K;        // rows grouped: A is M × K; K grouped: A is K × M, D is K × N (K = rows of both)
+  int32_t tiles_m, tiles_n;  // K grouped: tiles of one group; rows grouped: tiles_n only
+  const void* offsets;    // groups + 1 entries, or null: one group of all rows
+  int32_t offsets_64;
+  int32_t a_mn, b_kmaj;
+  uint32_t fmt;           // MMA operand format (idesc bits 7 and 10)
+  int32_t beta, c_dtype, vec;  // vec: bytes of a vector access to C (32, 16 or 0)
+  void* C;
+  int64_t ldc, group_c;
+  GScale sa, sb;
+  int32_t stages, split;  // ring depth; CTAs per cluster that share a tile's K range (G = 1)
+};
+
+__device__ __forceinline__ int32_t read_offset(const GParams& p, int32_t i) {
+  // Offsets out of [0, rows] are clamped: no access leaves the operands.
+  const int32_t rows = p.k_grouped ? p.K : p.M;
+  long long v;
+  if (!p.offsets) v = i ? rows : 0;
+  else if (p.offsets_64) v = static_cast<const long long*>(p.offsets)[i];
+  else v = static_cast<const int32_t*>(p.offsets)[i];
+  return (int32_t)(v < 0 ? 0 : v > rows ? rows : v);
+}
+
+struct GTile {
+  int32_t e;         // group
+  int32_t row0;      // first row of A and C (rows grouped) or of G[e] (K grouped)
+  int32_t rows, n0, cols;
+  int32_t k0, k_end; // K range of the tile
+  int32_t f0, f1;    // this CTA's ring fills of it
+};
+
+// Tile t. Inside a group, tiles go in bands of 8 tile rows, rows fastest:
+// the CTAs at work share few panels of A and B.
+template <int BM, int BN, int KB>
+__device__ __forceinline__ GTile tile_at(const GParams& p, const GroupTable& tab, int32_t t, int32_t part,
+                                         int32_t& cursor) {
+  GTile g;
+  int32_t u, group_rows, tiles_m;
+  if (p.k_grouped) {
+    const int32_t per = p.tiles_m * p.tiles_n;
+    g.e = t / per;
+    u = t - g.e * per;
+    tiles_m = p.tiles_m;
+    group_rows = p.M;
+    g.row0 = 0;
+    g.k0 = tab.start[g.e];
+    g.k_end = g.k0 + tab.rows[g.e];
+  } else {
+    while (tab.cum[cursor + 1] <= t) ++cursor;  // t < cum[groups], and t only grows
+    g.e = cursor;
+    u = t - tab.cum[cursor];
+    group_rows = tab.rows[cursor];
+    tiles_m = (group_rows + BM - 1) / BM;
+    g.row0 = tab.start[cursor];
+    g.k0 = 0;
+    g.k_end = p.K;
+  }
+  const int32_t band = u / (8 * p.tiles_n), v = u - band * 8 * p.tiles_n;
+  const int32_t height = min(8, tiles_m - band * 8);
+  const int32_t n = v / height, m = band * 8 + v - n * height;
+  g.row0 += m * BM;
+  g.rows = min(BM, group_rows - m * BM);
+  g.n0 = n * BN;
+  g.cols = min(BN, p.N - g.n0);
+  const int32_t fills = (g.k_end - g.k0 + KB - 1) / KB;
+  g.f0 = (int32_t)((int64_t)fills * part / p.split);
+  g.f1 = (int32_t)((int64_t)fills * (part + 1) / p.split);
+  return g;
+}
+
+__device__ __forceinline__ float load_out(const GParams& p, const char* q) {
+  if (p.c_dtype == TB_F32) return *reinterpret_cast<const float*>(q);
+  if (p.c_dtype == TB_F16) return __half2float(*reinterpret_cast<const __half*>(q));
+  return __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(q));
+}
+__device__ __forceinline__ void store_out(const GParams& p, char* q, float v) {
+  if (p.c_dtype == TB_F32) *reinterpret_cast<float*>(q) = v;
+  else if (p.c_dtype == TB_F16) *reinterpret_cast<__half*>(q) = __float2half_rn(v);
+  else *reinterpret_cast<__nv_bfloat16*>(q) = __float2bfloat16_rn(v);
+}
+__device__ __forceinline__ uint32_t pack2(const GParams& p, float a, float b) {
+  uint32_t w;
+  if (p.c_dtype == TB_F16) {
+    const __half2 h = __floats2half2_rn(a, b);
+    memcpy(&w, &h, 4);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    memcpy(&w, &h, 4);
+  }
+  return w;
+}
+__device__ __forceinline__ float2 unpack2(const GParams& p, uint32_t w) {
+  if (p.c_dtype == TB_F16) {
+    __half2 h;
+    memcpy(&h, &w, 4);
+    return __half22float2(h);
+  }
+  __nv_bfloat162 h;
+  memcpy(&h, &w, 4);
+  return __bfloat1622float2(h);
+}
+// 32 bytes in one store: a whole sector, so that a warp's rows need no merging in L2.
+__device__ __forceinline__ void st_32(void* q, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(q), "r"(w[0]), "r"(w[1]),
+               "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
+// beta·C + v of `ncol` of 32 consecutive columns at q.
+__device__ __forceinline__ void emit32(const GParams& p, char* q, float (&v)[32], int ncol) {
+  const int el = p.c_dtype == TB_F32 ? 4 : 2;
+  if (ncol < 32 || !p.vec) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < ncol) store_out(p, q + i * el, p.beta ? v[i] + load_out(p, q + i * el) : v[i]);
+    return;
+  }
+  if (p.c_dtype == TB_F32) {
+    if (p.beta) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float4 c = reinterpret_cast<const float4*>(q)[i];
+        v[4 * i] += c.x; v[4 * i + 1] += c.y; v[4 * i + 2] += c.z; v[4 * i + 3] += c.w;
+      }
+    }
+    if (p.vec == 32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(v[8 * i + j]);
+        st_32(q + 32 * i, w);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        reinterpret_cast<float4*>(q)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    }
+    return;
+  }
+  if (p.beta) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 c = reinterpret_cast<const uint4*>(q)[i];
+      const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = unpack2(p, w[j]);
+        v[8 * i + 2 * j] += f.x;
+        v[8 * i + 2 * j + 1] += f.y;
+      }
+    }
+  }
+  uint32_t w[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) w[j] = pack2(p, v[2 * j], v[2 * j + 1]);
+  if (p.vec == 32) {
+    st_32(q, w);
+    st_32(q + 32, w + 8);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      reinterpret_cast<uint4*>(q)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  }
+}
+
+template <int KIND, int BN, int G>
+__global__ void __launch_bounds__(kThreadsG, 1)
+    tb_grouped_sm100_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA32,
+                            const __grid_constant__ CUtensorMap tmB, const __grid_constant__ GParams p) {
+  using Cf = GCfg<KIND, BN, G>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  const int S = p.stages;
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + (size_t)S * Cf::kABytes;
+  uint8_t* red = smem + (size_t)S * Cf::kStageBytes;
+  uint8_t* tail = red + (p.split > 1 ? Cf::kRedBytes : 0u);
+  GBars& bars = *reinterpret_cast<GBars*>(tail);
+  GroupTable& tab = *reinterpret_cast<GroupTable*>(tail + ((sizeof(GBars) + 15) & ~size_t(15)));
+  volatile int* abort_flag = &bars.abort_flag;
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);
+  const int lane = threadIdx.x % 32;
+  const int cluster = G * p.split;
+  const uint32_t crank = cluster > 1 ? cluster_ctarank() : 0u;
+  const uint32_t rank = G == 2 ? crank : 0u;        // CTA of the pair
+  const int32_t part = G == 2 ? 0 : (int32_t)crank; // part of the K range
+  const bool leader = rank == 0;
+  const int32_t first = blockIdx.x / cluster, stride = gridDim.x / cluster;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      // K grouped pairs: both producers (or fixers) arrive for each fill
+      mbar_init(smem_addr(&bars.full[s]), p.k_grouped ? G : 1);
+      mbar_init(smem_addr(&bars.empty[s]), 1);
+      mbar_init(smem_addr(&bars.fix[s]), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(smem_addr(&bars.tfull[a]), 1);
+      mbar_init(smem_addr(&bars.tempty[a]), 8 * G);
+    }
+    mbar_init(smem_addr(&bars.drain), 1);
+    mbar_init(smem_addr(&bars.ready), 8 * p.split);
+    mbar_init(smem_addr(&bars.consumed), 8 * p.split);
+    bars.abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
+  if (warp == 1) {
+    tmem_alloc_g<G>(smem_addr(&bars.tmem_holder), Cf::kTmemCols);
+    tmem_relinquish_g<G>();
+  }
+  for (int32_t e = threadIdx.x; e < p.groups; e += kThreadsG) {
+    const int32_t s = read_offset(p, e), n = max(0, read_offset(p, e + 1) - s);
+    tab.start[e] = s;
+    tab.rows[e] = n;
+  }
+  __syncthreads();
+  if (warp == 0 && !p.k_grouped) {
+    int32_t before = 0;
+    for (int32_t e0 = 0; e0 < p.groups; e0 += 32) {
+      int32_t v = e0 + lane < p.groups ? (tab.rows[e0 + lane] + Cf::kBM - 1) / Cf::kBM * p.tiles_n : 0;
+#pragma unroll
+      for (int d = 1; d < 32; d *= 2) {
+        const int32_t o = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += o;
+      }
+      if (e0 + lane < p.groups) tab.cum[e0 + lane + 1] = before + v;
+      before += __shfl_sync(0xffffffffu, v, 31);
+    }
+    if (lane == 0) tab.cum[0] = 0;
+  }
+  tc_fence_before();
+  if (cluster > 1) cluster_sync();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = bars.tmem_holder;
+  const int32_t tiles = p.k_grouped ? p.groups * p.tiles_m * p.tiles_n : tab.cum[p.groups];
+
+  // 8-bit, 256 columns: the epilogue keeps 128 sums per thread. 256 threads ×
+  // 216 + 128 × 72 registers = the launch's 384 × 168.
+  constexpr bool kMoveRegs = KIND == kByte && BN == 256;
+  if constexpr (kMoveRegs) {
+    if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+  }
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    int stage = 0;
+    uint32_t phase = 0;
+    long long issued = 0;
+    int32_t cursor = 0;
+    bool ok = true;
+    for (int32_t t = first; t < tiles && ok; t += stride) {
+      const GTile g = tile_at<Cf::kBM, BN, Cf::kKB>(p, tab, t, part, cursor);
+      // K-major A of a short tile: only the 32-row boxes that hold its rows
+      const int boxes = G == 1 && !p.a_mn ? (min(g.rows, 128) + 31) / 32 : 4;
+      const uint32_t bytes = (boxes < 4 ? (uint32_t)boxes * 4096u : Cf::kABytes) + Cf::kBBytes;
+      const int32_t bn = g.n0 + (int32_t)rank * Cf::kBnCta;
+      const int32_t be = p.k_grouped ? 0 : g.e;
+      for (int32_t f = g.f0; f < g.f1; ++f) {
+        if (!warp_wait(smem_addr(&bars.empty[stage]), phase ^ 1u, abort_flag, kSiteProducer, lane)) {
+          ok = false;
+          break;
+        }
+        const int32_t kx = g.k0 + f * Cf::kKB;
+        const bool fix = p.k_grouped && (min(Cf::kKB, g.k_end - kx) % Cf::kMmaK) != 0;
+        const uint32_t dA = smem_addr(sA + (size_t)stage * Cf::kABytes);
+        const uint32_t dB = smem_addr(sB + (size_t)stage * Cf::kBBytes);
+        if (elect_one()) {
+          uint32_t bar;
+          if (fix) {  // this CTA's fixer takes the fill on from here
+            bar = smem_addr(&bars.fix[stage]);
+            mbar_expect_tx(bar, bytes);
+          } else {
+            bar = smem_addr(&bars.full[stage]);
+            if (leader) mbar_expect_tx(bar, G * bytes);
+            if constexpr (G == 2) {
+              bar = map_to_cta(bar, 0);
+              if (p.k_grouped && !leader) mbar_arrive_cluster(bar);
+            }
+          }
+          auto load2 = [&](uint32_t dst, const CUtensorMap* m, int32_t x, int32_t y) {
+            if constexpr (G == 2) tma_load_2d_pair(dst, m, bar, x, y);
+            else tma_load_2d(dst, m, bar, x, y);
+          };
+          auto load3 = [&](uint32_t dst, int32_t x, int32_t y) {
+            if constexpr (G == 2) tma_load_3d_pair(dst, &tmB, bar, x, y, be);
+            else tma_load_3d(dst, &tmB, bar, x, y, be);
+          };
+          const int32_t am = g.row0 + (int32_t)rank * 128;
+          if (p.a_mn) {
+#pragma unroll
+            for (int j = 0; j < 128 / Cf::kMnBox; ++j)
+              load2(dA + j * Cf::kMnBoxBytes, &tmA, am + Cf::kMnBox * j, kx);
+          } else if (boxes == 4) {
+            load2(dA, &tmA, kx, am);
+          } else {
+            for (int j = 0; j < boxes; ++j) load2(dA + j * 4096, &tmA32, kx, am + 32 * j);
+          }
+          if (p.b_kmaj) {
+            load3(dB, kx, bn);
+          } else {
+#pragma unroll
+            for (int j = 0; j < Cf::kBnCta / Cf::kMnBox; ++j)
+              load3(dB + j * Cf::kMnBoxBytes, bn + Cf::kMnBox * j, kx);
+          }
+        }
+        __syncwarp();
+        ++issued;
+        if (++stage == S) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    if (lane == 0 && leader) {
+      // The newest fill of each stage must land before the CTAs exit.
+      const long long last = issued < S ? issued : S;
+      for (long long i = 0; i < last; ++i) {
+        const long long f = issued - 1 - i;
+        const uint32_t par = (uint32_t)((f / S) & 1);
+        const long long t0 = clock64();
+        while (!mbar_try_wait(smem_addr(&bars.full[f % S]), par)) {
+          if (clock64() - t0 > kWaitBudgetCycles) {
+            record_error(TB_ERR_DEVICE_TIMEOUT, kSiteDrain);
+            break;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------- MMA issuer
+    if (leader) {
+      const uint32_t idesc = idesc_f16_f32(Cf::kBM, BN, p.a_mn ? 1 : 0, p.b_kmaj ? 0 : 1) | (p.fmt << 7) |
+                             (p.fmt << 10);
+      const uint32_t a_step = p.a_mn ? Cf::kMnStep : 32u, b_step = p.b_kmaj ? 32u : Cf::kMnStep;
+      const uint32_t a_lbo = p.a_mn ? Cf::kMnBoxBytes : 16u, b_lbo = p.b_kmaj ? 16u : Cf::kMnBoxBytes;
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      int32_t cursor = 0;
+      bool issued_any = false, ok = true;
+      for (int32_t t = first; t < tiles && ok; t += stride) {
+        const GTile g = tile_at<Cf::kBM, BN, Cf::kKB>(p, tab, t, part, cursor);
+        for (int32_t f = g.f0; f < g.f1; ++f) {
+          const bool opens = KIND == kByte || f == g.f0;       // first fill of an accumulation
+          const bool closes = KIND == kByte || f + 1 == g.f1;  // last one
+          if (opens && !warp_wait(smem_addr(&bars.tempty[acc]), acc_phase ^ 1u, abort_flag, kSiteMma, lane)) {
+            ok = false;
+            break;
+          }
+          if (!warp_wait(smem_addr(&bars.full[stage]), phase, abort_flag, kSiteMma, lane)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const int32_t valid = min(Cf::kKB, g.k_end - (g.k0 + f * Cf::kKB));
+          const int steps = (valid + Cf::kMmaK - 1) / Cf::kMmaK;
+          const uint64_t da0 = smem_desc_sw128(smem_addr(sA + (size_t)stage * Cf::kABytes), a_lbo, 1024);
+          const uint64_t db0 = smem_desc_sw128(smem_addr(sB + (size_t)stage * Cf::kBBytes), b_lbo, 1024);
+          const uint32_t d = tmem_base + (uint32_t)(acc * BN);
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+              if (kk < steps) {
+                const uint64_t da = da0 + (uint64_t)((a_step * kk) >> 4);
+                const uint64_t db = db0 + (uint64_t)((b_step * kk) >> 4);
+                const uint32_t add = (!opens || kk > 0) ? 1u : 0u;
+                if constexpr (KIND == kByte) umma_f8<G>(d, da, db, idesc, add);
+                else if constexpr (G == 2) umma_f16_pair(d, da, db, idesc, add);
+                else umma_f16(d, da, db, idesc, add);
+              }
+            }
+            if constexpr (G == 2) umma_commit_pair(smem_addr(&bars.empty[stage]), 0x3);
+            else umma_commit(smem_addr(&bars.empty[stage]));
+            if (closes) {
+              if constexpr (G == 2) umma_commit_pair(smem_addr(&bars.tfull[acc]), 0x3);
+              else umma_commit(smem_addr(&bars.tfull[acc]));
+            }
+          }
+          __syncwarp();
+          issued_any = true;
+          if (closes && ++acc == 2) {
+            acc = 0;
+            acc_phase ^= 1u;
+          }
+          if (++stage == S) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok && issued_any && lane == 0) {
+        // Given up with MMAs possibly in flight: wait for them before TMEM goes.
+        if constexpr (G == 2) umma_commit_pair(smem_addr(&bars.drain), 0x1);
+        else umma_commit(smem_addr(&bars.drain));
+        const long long t0 = clock64();
+        while (!mbar_try_wait(smem_addr(&bars.drain), 0)) {
+          if (clock64() - t0 > kWaitBudgetCycles) {
+            record_error(TB_ERR_DEVICE_TIMEOUT, kSiteDrain);
+            break;
+          }
+        }
+      }
+      __syncwarp();
+    }
+  } else if (warp == 2) {
+    // --------------------------------------------------------------- fixer
+    if (p.k_grouped) {
+      int stage = 0;
+      uint32_t fix_phase = 0;  // bit s: parity of stage s's next fix
+      int32_t cursor = 0;
+      bool ok = true;
+      for (int32_t t = first; t < tiles && ok; t += stride) {
+        const GTile g = tile_at<Cf::kBM, BN, Cf::kKB>(p, tab, t, part, cursor);
+        const int32_t n = g.f1 - g.f0;
+        if (n <= 0) continue;
+        const int32_t last = (stage + n - 1) % S;  // only a tile's last fill can be short
+        const int32_t valid = min(Cf::kKB, g.k_end - (g.k0 + (g.f1 - 1) * Cf::kKB));
+        stage = (stage + n) % S;
+        if (valid % Cf::kMmaK == 0) continue;
+        if (!warp_wait(smem_addr(&bars.fix[last]), (fix_phase >> last) & 1u, abort_flag, kSiteFixer, lane)) {
+          ok = false;
+          break;
+        }
+        fix_phase ^= 1u << last;
+        // K rows [valid, next multiple of the K step) of every box of both
+        // operands: 128 bytes per row (the swizzle stays inside a row)
+        const int32_t end = (valid + Cf::kMmaK - 1) / Cf::kMmaK * Cf::kMmaK;
+        const int32_t words = (end - valid) * 8;
+        auto zero = [&](uint8_t* stage_base, int nboxes) {
+          for (int b = 0; b < nboxes; ++b) {
+            uint4* q = reinterpret_cast<uint4*>(stage_base + (size_t)b * Cf::kMnBoxBytes + (size_t)valid * 128);
+            for (int i = lane; i < words; i += 32) q[i] = make_uint4(0, 0, 0, 0);
+          }
+        };
+        zero(sA + (size_t)last * Cf::kABytes, 128 / Cf::kMnBox);
+        zero(sB + (size_t)last * Cf::kBBytes, Cf::kBnCta / Cf::kMnBox);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (G == 2) mbar_arrive_cluster(map_to_cta(smem_addr(&bars.full[last]), 0));
+          else mbar_arrive(smem_addr(&bars.full[last]));
+        }
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ epilogue
+    const int q = warp & 3;               // TMEM lane quarter
+    const int half = (warp - 4) >> 2;     // column half
+    const int row_in_tile = (int)rank * 128 + q * 32 + lane;
+    const int c_half = half * Cf::kHalfCols;
+    const uint32_t tm = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)c_half;
+    const int el = p.c_dtype == TB_F32 ? 4 : 2;
+    const uint32_t tempty0 = G == 2 ? map_to_cta(smem_addr(&bars.tempty[0]), 0) : smem_addr(&bars.tempty[0]);
+    auto release = [&](int acc) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (G == 2) mbar_arrive_cluster(tempty0 + acc * 8);
+        else mbar_arrive(tempty0 + acc * 8);
+      }
+    };
+    int acc = 0;
+    uint32_t acc_phase = 0, red_phase = 0;
+    int32_t cursor = 0;
+    bool ok = true;
+    for (int32_t t = first; t < tiles && ok; t += stride) {
+      const GTile g = tile_at<Cf::kBM, BN, Cf::kKB>(p, tab, t, part, cursor);
+      const bool row_ok = row_in_tile < g.rows;
+      const bool warp_ok = (int)rank * 128 + q * 32 < g.rows && c_half < g.cols;
+      char* crow = static_cast<char*>(p.C) +
+                   ((p.k_grouped ? (int64_t)g.e * p.group_c : 0) + ((int64_t)g.row0 + row_in_tile) * p.ldc + g.n0) * el;
+      float v[Cf::kChunks][32];
+
+      if constexpr (KIND == kByte) {
+        const int32_t arow = min(g.row0 + row_in_tile, p.M - 1);  // masked rows read some valid scale
+        const float* sa = p.sa.p + (int64_t)(arow >> p.sa.shift) * p.sa.smn;
+        const float* sb = p.sb.p + (int64_t)g.e * p.sb.sg;
+        const int32_t col0 = min(g.n0 + c_half, p.N - 1);
+#pragma unroll
+        for (int c = 0; c < Cf::kChunks; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[c][i] = 0.f;
+        for (int32_t f = g.f0; f < g.f1; ++f) {
+          const float xa = __ldg(sa + (int64_t)f * p.sa.sk);
+          const float xb = p.sb.shift ? __ldg(sb + (int64_t)(col0 >> 7) * p.sb.smn + (int64_t)f * p.sb.sk) : 1.f;
+          const float x = xa * xb;
+          if (!warp_wait(smem_addr(&bars.tfull[acc]), acc_phase, abort_flag, kSiteEpilogue, lane)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          if (warp_ok) {
+#pragma unroll
+            for (int c = 0; c < Cf::kChunks; ++c) {
+              float w[32];
+              tmem_ld_32x32b_x32(tm + (uint32_t)(acc * BN + c * 32), w);
+              if (p.sb.shift) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[c][i] = fmaf(w[i], x, v[c][i]);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                  const int32_t col = min(g.n0 + c_half + c * 32 + i, p.N - 1);
+                  v[c][i] = fmaf(w[i], x * __ldg(sb + (int64_t)col * p.sb.smn + (int64_t)f * p.sb.sk), v[c][i]);
+                }
+              }
+            }
+          }
+          release(acc);
+          if (++acc == 2) {
+            acc = 0;
+            acc_phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+      } else {
+        if (g.f1 > g.f0) {
+          if (!warp_wait(smem_addr(&bars.tfull[acc]), acc_phase, abort_flag, kSiteEpilogue, lane)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+        }
+        if (p.split > 1) {
+#pragma unroll
+          for (int c = 0; c < Cf::kChunks; ++c) {
+            if (g.f1 > g.f0) {
+              tmem_ld_32x32b_x32(tm + (uint32_t)(acc * BN + c * 32), v[c]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[c][i] = 0.f;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < Cf::kChunks; ++c) {
+            if (!warp_ok) break;
+            if (g.f1 > g.f0) {
+              tmem_ld_32x32b_x32(tm + (uint32_t)(acc * BN + c * 32), v[0]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[0][i] = 0.f;
+            }
+            const int ncol = min(32, g.cols - c_half - c * 32);
+            if (row_ok && ncol > 0) emit32(p, crow + (c_half + c * 32) * el, v[0], ncol);
+            __syncwarp();
+          }
+        }
+        if (g.f1 > g.f0) {
+          release(acc);
+          if (++acc == 2) {
+            acc = 0;
+            acc_phase ^= 1u;
+          }
+        }
+      }
+
+      if (p.split == 1) {
+        if constexpr (KIND == kByte) {
+#pragma unroll
+          for (int c = 0; c < Cf::kChunks; ++c) {
+            const int ncol = min(32, g.cols - c_half - c * 32);
+            if (row_ok && ncol > 0) emit32(p, crow + (c_half + c * 32) * el, v[c], ncol);
+          }
+          __syncwarp();
+        }
+      } else if constexpr (G == 1) {
+        // The cluster's CTAs hold partial sums of one tile. Each leaves its
+        // own in shared memory; CTA r then adds rows r, r + split, … of all
+        // of them, in CTA order, and stores them.
+        auto cluster_wait = [&](uint64_t* bar, uint32_t par) {
+          int good = 1;
+          if (lane == 0) {
+            const uint32_t b = smem_addr(bar);
+            const long long t0 = clock64();
+            while (!mbar_try_wait_cluster(b, par)) {
+              if (*abort_flag) {
+                good = 0;
+                break;
+              }
+              if (clock64() - t0 > kWaitBudgetCycles) {
+                record_error(TB_ERR_DEVICE_TIMEOUT, kSiteCluster);
+                *abort_flag = 1;
+                good = 0;
+                break;
+              }
+            }
+          }
+          good = __shfl_sync(0xffffffffu, good, 0);
+          return good != 0;
+        };
+        auto cluster_arrive = [&](uint64_t* bar) {
+          __syncwarp();
+          if (lane < p.split) mbar_arrive_cluster(map_to_cta(smem_addr(bar), (uint32_t)lane));
+        };
+        // every CTA has read the previous tile's partial sums
+        if (!cluster_wait(&bars.consumed, red_phase ^ 1u)) {
+          ok = false;
+          break;
+        }
+        if (row_ok) {
+#pragma unroll
+          for (int c = 0; c < Cf::kChunks; ++c) {
+            float4* dst = reinterpret_cast<float4*>(red + (size_t)row_in_tile * Cf::kRedStride + (c_half + c * 32) * 4);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              dst[i] = make_float4(v[c][4 * i], v[c][4 * i + 1], v[c][4 * i + 2], v[c][4 * i + 3]);
+          }
+        }
+        cluster_arrive(&bars.ready);
+        if (!cluster_wait(&bars.ready, red_phase)) {
+          ok = false;
+          break;
+        }
+        constexpr int kLaneCols = BN / 32;
+        const int rows = min(g.rows, 128);
+        for (int r = part + p.split * (warp - 4); r < rows; r += p.split * 8) {
+          const uint32_t src = smem_addr(red) + (uint32_t)r * Cf::kRedStride + (uint32_t)lane * kLaneCols * 4;
+          float s[kLaneCols];
+#pragma unroll
+          for (int i = 0; i < kLaneCols; ++i) s[i] = 0.f;
+          for (int j = 0; j < p.split; ++j) {
+            const uint32_t a = map_to_cta(src, (uint32_t)j);
+            if constexpr (kLaneCols == 4) {
+              const float4 x = ld_cluster_f4(a);
+              s[0] += x.x; s[1] += x.y; s[2] += x.z; s[3] += x.w;
+            } else {
+              const float2 x = ld_cluster_f2(a);
+              s[0] += x.x; s[1] += x.y;
+            }
+          }
+          const int c0 = lane * kLaneCols;
+          char* dst = static_cast<char*>(p.C) +
+                      ((p.k_grouped ? (int64_t)g.e * p.group_c : 0) + ((int64_t)g.row0 + r) * p.ldc + g.n0 + c0) * el;
+#pragma unroll
+          for (int i = 0; i < kLaneCols; ++i)
+            if (c0 + i < g.cols) store_out(p, dst + i * el, p.beta ? s[i] + load_out(p, dst + i * el) : s[i]);
+        }
+        cluster_arrive(&bars.consumed);
+        red_phase ^= 1u;
+      }
+    }
+  }
+
+  __syncthreads();
+  if (cluster > 1) cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_g<G>(tmem_base, Cf::kTmemCols);
+  }
+}
+
+// Copies rows of `row_bytes` to rows of ld_dst bytes (a multiple of 16), the
+// rest of each row zero: operands whose rows TMA cannot address.
+__global__ void __launch_bounds__(256)
+    tb_grouped_pack_kernel(const uint8_t* __restrict__ src, int64_t ld_src, int64_t batch_src, uint8_t* __restrict__ dst,
+                           int64_t ld_dst, int64_t batch_dst, int64_t rows, int64_t row_bytes) {
+  src += (int64_t)blockIdx.z * batch_src;
+  dst += (int64_t)blockIdx.z * batch_dst;
+  const int64_t words = ld_dst / 16;
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    for (int64_t w = threadIdx.x; w < words; w += blockDim.x) {
+      __align__(16) uint8_t b[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) b[i] = w * 16 + i < row_bytes ? src[r * ld_src + w * 16 + i] : 0;
+      *reinterpret_cast<uint4*>(dst + r * ld_dst + w * 16) = *reinterpret_cast<const uint4*>(b);
+    }
+  }
+}
+
+// ------------------------------------------------------------------- host
+
+std::atomic<PFN_cuTensorMapEncodeTiled_v12000> g_encode_fn{nullptr};
+
+tbStatus encoder(PFN_cuTensorMapEncodeTiled_v12000* out) {
+  PFN_cuTensorMapEncodeTiled_v12000 f = g_encode_fn.load();
+  if (!f) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult qres;
+    cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &qres);
+    if (e != cudaSuccess || qres != cudaDriverEntryPointSuccess || !fn)
+      return tb_fail(TB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+    f = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    g_encode_fn.store(f);
+  }
+  *out = f;
+  return TB_OK;
+}
+
+constexpr int kMaxDev = 64;
+std::atomic<int> g_sms[kMaxDev];
+
+tbStatus current_device(int* dev, int* sms) {
+  cudaError_t e = cudaGetDevice(dev);
+  if (e != cudaSuccess) return tb_fail(TB_ERR_CUDA, std::string("cudaGetDevice: ") + cudaGetErrorString(e));
+  if (*dev < 0 || *dev >= kMaxDev) return tb_fail(TB_ERR_UNSUPPORTED, "device ordinal beyond the library's table");
+  int n = g_sms[*dev].load();
+  if (!n) {
+    e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, *dev);
+    if (e != cudaSuccess)
+      return tb_fail(TB_ERR_CUDA, std::string("cudaDeviceGetAttribute: ") + cudaGetErrorString(e));
+    g_sms[*dev].store(n);
+  }
+  *sms = n;
+  return TB_OK;
+}
+
+bool al(const void* p, int64_t n) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)n == 0; }
+
+// One operand as the kernel reads it: `rows` rows of `cols` contiguous
+// elements in each of `batch` matrices.
+struct Operand {
+  const void* p;
+  int64_t rows, cols, ld, batch, stride;  // strides in elements
+  bool pack(int el) const {
+    return !al(p, 16) || (rows > 1 && ld * el % 16) || (batch > 1 && stride * el % 16);
+  }
+  int64_t packed_ld(int el) const { return (cols * el + 15) / 16 * 16; }  // bytes
+  size_t packed_bytes(int el) const {
+    return ((size_t)packed_ld(el) * (size_t)rows * (size_t)batch + 255) / 256 * 256;
+  }
+};
+
+tbStatus pack(Operand* o, int el, void* ws, cudaStream_t stream) {
+  if (o->batch > 65535) return tb_fail(TB_ERR_UNSUPPORTED, "too many groups to repack");
+  const int64_t ld = o->packed_ld(el);
+  const unsigned gx = (unsigned)std::min<int64_t>(std::max<int64_t>(1, o->rows), 4096);
+  tb_grouped_pack_kernel<<<dim3(gx, 1, (unsigned)o->batch), 256, 0, stream>>>(
+      static_cast<const uint8_t*>(o->p), o->ld * el, o->stride * el, static_cast<uint8_t*>(ws), ld, ld * o->rows,
+      o->rows, o->cols * el);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return tb_fail(TB_ERR_CUDA, std::string("tb_grouped_pack launch: ") + cudaGetErrorString(e));
+  o->p = ws;
+  o->ld = ld / el;
+  o->stride = o->ld * o->rows;
+  return TB_OK;
+}
+
+tbStatus encode(CUtensorMap* map, int dims_n, const Operand& o, int el, int is_bf16, uint32_t box0, uint32_t box1,
+                const char* what) {
+  PFN_cuTensorMapEncodeTiled_v12000 f;
+  tbStatus st = encoder(&f);
+  if (st != TB_OK) return st;
+  cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)o.batch};
+  const cuuint64_t ld = (cuuint64_t)(o.rows > 1 ? o.ld * el : (o.cols * el + 15) / 16 * 16);
+  const cuuint64_t bs = (cuuint64_t)(o.batch > 1 ? (cuuint64_t)o.stride * el : ld * (cuuint64_t)o.rows);
+  cuuint64_t strides[2] = {ld, bs};
+  cuuint32_t box[3] = {box0, box1, 1}, es[3] = {1, 1, 1};
+  const CUtensorMapDataType dt = el == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                 : is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                           : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUresult r = f(map, dt, (cuuint32_t)dims_n, const_cast<void*>(o.p), dims, strides, box, es,
+                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return tb_fail(TB_ERR_CUDA, std::string("cuTensorMapEncodeTiled(") + what + ") failed with CUresult " +
+                                    std::to_string((int)r));
+  return TB_OK;
+}
+
+struct Launch {
+  Operand a, b;
+  int el, bf16;
+  int64_t tiles;  // an upper bound of the tiles
+  GParams p;
+};
+
+template <int KIND, int BN, int G>
+tbStatus launch(Launch& L, int sms, int dev, cudaStream_t stream) {
+  using Cf = GCfg<KIND, BN, G>;
+  GParams& p = L.p;
+  CUtensorMap ta, ta32, tb_;
+  std::memset(&ta32, 0, sizeof(ta32));
+  tbStatus st = encode(&ta, 2, L.a, L.el, L.bf16, p.a_mn ? Cf::kMnBox : Cf::kKB, p.a_mn ? Cf::kKB : 128, "A");
+  if (st == TB_OK && !p.a_mn) st = encode(&ta32, 2, L.a, L.el, L.bf16, Cf::kKB, 32, "A");
+  if (st == TB_OK)
+    st = encode(&tb_, 3, L.b, L.el, L.bf16, p.b_kmaj ? Cf::kKB : Cf::kMnBox, p.b_kmaj ? Cf::kBnCta : Cf::kKB, "B");
+  if (st != TB_OK) return st;
+  const size_t fixed = 1024 + kTailBytes + (p.split > 1 ? Cf::kRedBytes : 0);
+  p.stages = (int)std::min<size_t>(kMaxStages, (kSmemLimitG - fixed) / Cf::kStageBytes);
+  const size_t smem = fixed + (size_t)p.stages * Cf::kStageBytes;
+  auto kern = tb_grouped_sm100_kernel<KIND, BN, G>;
+  static std::atomic<bool> ready[kMaxDev];
+  if (!ready[dev].load()) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemLimitG);
+    if (e != cudaSuccess)
+      return tb_fail(TB_ERR_CUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
+    ready[dev].store(true);
+  }
+  const int cluster = G * p.split;
+  const int64_t slots = std::max(1, sms / cluster);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(std::min<int64_t>(slots, L.tiles) * cluster), 1, 1);
+  cfg.blockDim = dim3(kThreadsG, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ta, ta32, tb_, p);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return tb_fail(TB_ERR_CUDA, std::string("tb_grouped launch: ") + cudaGetErrorString(e));
+  return TB_OK;
+}
+
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Tile and K split. `rows`: mean rows of a group that has any.
+tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int dev, cudaStream_t stream) {
+  GParams& p = L.p;
+  const int64_t n = p.N;
+  const int64_t kmax = p.k_grouped ? cdiv(p.K, std::max<int64_t>(1, groups)) : p.K;
+  const int64_t m = p.k_grouped ? p.M : rows;
+  const int64_t busy = p.k_grouped ? groups : std::min<int64_t>(groups, p.M);
+  auto tiles = [&](int bm, int bn) { return busy * cdiv(m, bm) * cdiv(n, bn); };
+  auto bound = [&](int bm, int bn) {
+    return p.k_grouped ? groups * cdiv(p.M, bm) * cdiv(n, bn) : (p.M / bm + std::min<int64_t>(groups, p.M)) * cdiv(n, bn);
+  };
+  auto set = [&](int bm, int bn) {
+    p.tiles_m = (int32_t)cdiv(p.M, bm);
+    p.tiles_n = (int32_t)cdiv(n, bn);
+    L.tiles = bound(bm, bn);
+  };
+  p.split = 1;
+  if (m > 128 && 2 * tiles(256, 256) >= sms / 2) {
+    set(256, 256);
+    return L.el == 1 ? launch<kByte, 256, 2>(L, sms, dev, stream) : launch<kHalf, 256, 2>(L, sms, dev, stream);
+  }
+  // An 8-bit B stored along its columns comes in boxes of 128 columns.
+  const bool wide = (L.el == 1 && !p.b_kmaj) || tiles(128, 128) >= sms;
+  const int64_t have = tiles(128, wide ? 128 : 64);
+  const int64_t fills = cdiv(kmax, 128 / L.el);
+  while (p.split < 8 && have * p.split * 2 <= sms && fills >= 4 * p.split) p.split *= 2;
+  set(128, wide ? 128 : 64);
+  if (wide)
+    return L.el == 1 ? launch<kByte, 128, 1>(L, sms, dev, stream) : launch<kHalf, 128, 1>(L, sms, dev, stream);
+  return L.el == 1 ? launch<kByte, 64, 1>(L, sms, dev, stream) : launch<kHalf, 64, 1>(L, sms, dev, stream);
+}
+
+int c_bytes(int32_t dt) { return dt == TB_F32 ? 4 : 2; }
+
+int vector_bytes(const void* C, int64_t ldc, int64_t group, int el) {
+  for (int b : {32, 16})
+    if (al(C, b) && ldc * el % b == 0 && group * el % b == 0) return b;
+  return 0;
+}
+
+tbStatus check_desc(const tb_grouped_desc* d, bool bytes) {
+  if (!d) return tb_fail(TB_ERR_INVALID_ARGUMENT, "desc must not be NULL");
+  if (d->groups < 0 || d->rows < 0 || d->n < 0 || d->k < 0)
+    return tb_fail(TB_ERR_INVALID_ARGUMENT, "groups, rows, n and k must not be negative");
+  if (d->groups > kMaxGroups)
+    return tb_fail(TB_ERR_UNSUPPORTED, "at most " + std::to_string(kMaxGroups) + " groups");
+  if (d->rows > INT32_MAX - 512 || d->n > INT32_MAX - 512 || d->k > INT32_MAX - 512)
+    return tb_fail(TB_ERR_UNSUPPORTED, "problem dimensions must fit in 32 bits");
+  if (bytes ? d->ab_dtype != TB_E4M3 : (d->ab_dtype != TB_F16 && d->ab_dtype != TB_BF16))
+    return tb_fail(TB_ERR_INVALID_ARGUMENT, bytes ? "operands must be e4m3" : "operands must be f16 or bf16");
+  if (d->c_dtype != TB_F32 && d->c_dtype != TB_F16 && d->c_dtype != TB_BF16)
+    return tb_fail(TB_ERR_INVALID_ARGUMENT, "the output must be f32, f16 or bf16");
+  if (d->beta != 0 && d->beta != 1) return tb_fail(TB_ERR_INVALID_ARGUMENT, "beta must be 0 or 1");
+  const int64_t tiles = (d->rows / 128 + d->groups + 1) * (cdiv(d->n, 64) + 1);
+  const int64_t tiles_k = (d->groups + 1) * (cdiv(d->k, 128) + 1) * (cdiv(d->n, 64) + 1);
+  if (tiles > INT32_MAX / 2 || tiles_k > INT32_MAX / 2)
+    return tb_fail(TB_ERR_UNSUPPORTED, "the problem has too many tiles");
+  return TB_OK;
+}
+
+tbStatus check_ld(int64_t ld, int64_t row, int64_t rows, const char* name) {
+  if (rows > 1 && ld < row)
+    return tb_fail(TB_ERR_INVALID_ARGUMENT, std::string(name) + ": the leading dimension must be >= the row length");
+  return TB_OK;
+}
+
+// Packs what TMA cannot address, then launches. `rows`: mean rows of a group.
+tbStatus finish(Launch& L, int64_t groups, int64_t rows, void* ws, size_t ws_bytes, void* stream_v) {
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
+  const bool pa = L.a.pack(L.el), pb = L.b.pack(L.el);
+  const size_t need = (pa ? L.a.packed_bytes(L.el) : 0) + (pb ? L.b.packed_bytes(L.el) : 0);
+  if (need && (!ws || ws_bytes < need || !al(ws, 256)))
+    return tb_fail(TB_ERR_WORKSPACE, "these operands' rows are not 16-byte aligned: they are repacked in a 256-byte "
+                                     "aligned workspace of " + std::to_string(need) + " bytes");
+  int dev, sms;
+  tbStatus st = current_device(&dev, &sms);
+  if (st != TB_OK) return st;
+  uint8_t* w = static_cast<uint8_t*>(ws);
+  if (pa) {
+    const size_t b = L.a.packed_bytes(L.el);
+    if ((st = pack(&L.a, L.el, w, stream)) != TB_OK) return st;
+    w += b;
+  }
+  if (pb && (st = pack(&L.b, L.el, w, stream)) != TB_OK) return st;
+  return choose_and_launch(L, groups, rows, sms, dev, stream);
+}
+
+// Operands of the row-grouped product: A rows × k, B groups × (k × n or n × k).
+void row_operands(const tb_grouped_desc* d, const void* A, int64_t lda, const void* B, int64_t ldb, int64_t stride_b,
+                  Operand* a, Operand* b) {
+  *a = d->a_col_major ? Operand{A, d->k, d->rows, lda, 1, 0} : Operand{A, d->rows, d->k, lda, 1, 0};
+  *b = d->b_col_major ? Operand{B, d->n, d->k, ldb, d->groups, stride_b}
+                      : Operand{B, d->k, d->n, ldb, d->groups, stride_b};
+}
+
+size_t packing(const Operand& a, const Operand& b, int el) {
+  return (a.pack(el) ? a.packed_bytes(el) : 0) + (b.pack(el) ? b.packed_bytes(el) : 0);
+}
+
+// beta = 0 and nothing to add: the rows of every group become zero.
+// (K = 0; the kernel's tiles then have no fills and store zeros, so it runs
+// with an operand that it never reads.)
+alignas(16) const unsigned char kNothing[16] = {};
+
+tbStatus run_rows(const tb_grouped_desc* d, bool bytes, const void* A, int64_t lda, const tb_scales* sa, const void* B,
+                  int64_t ldb, int64_t stride_b, const tb_scales* sb, void* C, int64_t ldc, const void* offsets,
+                  void* ws, size_t ws_bytes, void* stream) {
+  tbStatus st = check_desc(d, bytes);
+  if (st != TB_OK) return st;
+  if (d->rows == 0 || d->n == 0 || d->groups == 0) return TB_OK;
+  if (!C || (d->k > 0 && (!A || !B))) return tb_fail(TB_ERR_INVALID_ARGUMENT, "A, B and C must not be NULL");
+  const int el = bytes ? 1 : 2;
+  Launch L;
+  row_operands(d, A, lda, B, ldb, stride_b, &L.a, &L.b);
+  if ((st = check_ld(lda, L.a.cols, L.a.rows, "A")) != TB_OK) return st;
+  if ((st = check_ld(ldb, L.b.cols, L.b.rows, "B")) != TB_OK) return st;
+  if ((st = check_ld(ldc, d->n, d->rows, "C")) != TB_OK) return st;
+  const int ce = c_bytes(d->c_dtype);
+  if (!al(C, ce)) return tb_fail(TB_ERR_INVALID_ARGUMENT, "C is not aligned to its element size");
+  if (offsets && !al(offsets, d->offsets_long ? 8 : 4))
+    return tb_fail(TB_ERR_INVALID_ARGUMENT, "offsets are not aligned to their element size");
+  GParams& p = L.p;
+  std::memset(&p, 0, sizeof(p));
+  if (bytes) {
+    if (d->k > 0 && (!sa || !sb || !sa->ptr || !sb->ptr))
+      return tb_fail(TB_ERR_INVALID_ARGUMENT, "8-bit operands need their scales");
+    if (sa && sb) {
+      if ((sa->block != 1 && sa->block != 128) || (sb->block != 1 && sb->block != 128))
+        return tb_fail(TB_ERR_INVALID_ARGUMENT, "a scale covers 1 or 128 rows of A and 1 or 128 columns of B");
+      if (offsets && sa->block != 1)
+        return tb_fail(TB_ERR_UNSUPPORTED, "grouped rows need a scale for each row of A");
+      p.sa = {sa->ptr, 0, sa->stride_mn, sa->stride_k, sa->block == 128 ? 7 : 0};
+      p.sb = {sb->ptr, sb->stride_group, sb->stride_mn, sb->stride_k, sb->block == 128 ? 7 : 0};
+    }
+  }
+  L.el = el;
+  L.bf16 = d->ab_dtype == TB_BF16;
+  p.k_grouped = 0;
+  p.groups = (int32_t)d->groups;
+  p.M = (int32_t)d->rows;
+  p.N = (int32_t)d->n;
+  p.K = (int32_t)d->k;
+  p.offsets = offsets;
+  p.offsets_64 = d->offsets_long;
+  p.a_mn = d->a_col_major ? 1 : 0;
+  p.b_kmaj = d->b_col_major ? 1 : 0;
+  p.fmt = L.bf16 ? 1u : 0u;
+  p.beta = d->beta;
+  p.c_dtype = d->c_dtype;
+  p.C = C;
+  p.ldc = ldc;
+  p.vec = vector_bytes(C, ldc, 0, ce);
+  if (d->k == 0) {
+    if (d->beta) return TB_OK;
+    L.a = Operand{kNothing, 1, 16, 16, 1, 0};
+    L.b = Operand{kNothing, 1, 16, 16, 1, 0};
+  }
+  const int64_t busy = std::min<int64_t>(d->groups, d->rows);
+  return finish(L, d->groups, cdiv(d->rows, busy), ws, ws_bytes, stream);
+}
+
+}  // namespace
+
+// The status word of this translation unit's kernels; read and cleared.
+tbStatus tb_grouped_status(uint32_t* raw) {
+  uint32_t v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, g_tb_status, sizeof(v));
+  if (e != cudaSuccess)
+    return tb_fail(TB_ERR_CUDA, std::string("cudaMemcpyFromSymbol: ") + cudaGetErrorString(e));
+  if (v) {
+    const uint32_t zero = 0;
+    cudaMemcpyToSymbol(g_tb_status, &zero, sizeof(zero));
+  }
+  *raw = v;
+  return TB_OK;
+}
+
+extern "C" tbStatus tb_grouped_desc_init(tb_grouped_desc* d) {
+  tb_clear_error();
+  if (!d) return tb_fail(TB_ERR_INVALID_ARGUMENT, "desc must not be NULL");
+  std::memset(d, 0, sizeof(*d));
+  d->groups = 1;
+  d->ab_dtype = TB_F16;
+  d->c_dtype = TB_F32;
+  d->beta = 1;
+  return TB_OK;
+}
+
+extern "C" size_t tb_grouped_matmul_workspace_bytes(const tb_grouped_desc* d, const void* A, int64_t lda,
+                                                    const void* B, int64_t ldb, int64_t stride_b) {
+  if (!d || d->rows <= 0 || d->n <= 0 || d->k <= 0 || d->groups <= 0) return 0;
+  Operand a, b;
+  row_operands(d, A, lda, B, ldb, stride_b, &a, &b);
+  return packing(a, b, d->ab_dtype == TB_E4M3 ? 1 : 2);
+}
+
+extern "C" tbStatus tb_grouped_matmul(const tb_grouped_desc* d, const void* A, int64_t lda, const void* B, int64_t ldb,
+                                      int64_t stride_b, void* C, int64_t ldc, const void* offsets, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
+  tb_clear_error();
+  if (d && d->a_col_major) return tb_fail(TB_ERR_UNSUPPORTED, "grouped rows need a row-major A");
+  if (d && d->groups > 0 && !offsets) return tb_fail(TB_ERR_INVALID_ARGUMENT, "offsets must not be NULL");
+  return run_rows(d, false, A, lda, nullptr, B, ldb, stride_b, nullptr, C, ldc, offsets, workspace, workspace_bytes,
+                  stream);
+}
+
+extern "C" size_t tb_grouped_matmul_wgrad_workspace_bytes(const tb_grouped_desc* d, const void* A, int64_t lda,
+                                                          const void* D, int64_t ldd) {
+  if (!d || d->rows <= 0 || d->n <= 0 || d->k <= 0 || d->groups <= 0) return 0;
+  return packing(Operand{A, d->rows, d->k, lda, 1, 0}, Operand{D, d->rows, d->n, ldd, 1, 0}, 2);
+}
+
+extern "C" tbStatus tb_grouped_matmul_wgrad(const tb_grouped_desc* d, const void* A, int64_t lda, const void* D,
+                                            int64_t ldd, void* Gp, int64_t ldg, int64_t stride_g, const void* offsets,
+                                            void* workspace, size_t workspace_bytes, void* stream) {
+  tb_clear_error();
+  tbStatus st = check_desc(d, false);
+  if (st != TB_OK) return st;
+  if (d->a_col_major || d->b_col_major)
+    return tb_fail(TB_ERR_UNSUPPORTED, "the weight gradient takes row-major operands");
+  if (d->k == 0 || d->n == 0 || d->groups == 0) return TB_OK;
+  if (!Gp || !offsets || (d->rows > 0 && (!A || !D)))
+    return tb_fail(TB_ERR_INVALID_ARGUMENT, "A, D, G and offsets must not be NULL");
+  if (d->rows == 0 && d->beta) return TB_OK;
+  Launch L;
+  L.a = Operand{A, d->rows, d->k, lda, 1, 0};
+  L.b = Operand{D, d->rows, d->n, ldd, 1, 0};
+  if ((st = check_ld(lda, d->k, d->rows, "A")) != TB_OK) return st;
+  if ((st = check_ld(ldd, d->n, d->rows, "D")) != TB_OK) return st;
+  if ((st = check_ld(ldg, d->n, d->k, "G")) != TB_OK) return st;
+  const int ce = c_bytes(d->c_dtype);
+  if (!al(Gp, ce)) return tb_fail(TB_ERR_INVALID_ARGUMENT, "G is not aligned to its element size");
+  if (!al(offsets, d->offsets_long ? 8 : 4))
+    return tb_fail(TB_ERR_INVALID_ARGUMENT, "offsets are not aligned to their element size");
+  if (d->rows == 0) {  // every gradient is zero: the tiles have no fills
+    L.a = Operand{kNothing, 1, 8, 8, 1, 0};
+    L.b = Operand{kNothing, 1, 8, 8, 1, 0};
+  }
+  GParams& p = L.p;
+  std::memset(&p, 0, sizeof(p));
+  L.el = 2;
+  L.bf16 = d->ab_dtype == TB_BF16;
+  p.k_grouped = 1;
+  p.groups = (int32_t)d->groups;
+  p.M = (int32_t)d->k;
+  p.N = (int32_t)d->n;
+  p.K = (int32_t)d->rows;
+  p.offsets = offsets;
+  p.offsets_64 = d->offsets_long;
+  p.a_mn = 1;
+  p.b_kmaj = 0;
+  p.fmt = L.bf16 ? 1u : 0u;
+  p.beta = d->beta;
+  p.c_dtype = d->c_dtype;
+  p.C = Gp;
+  p.ldc = ldg;
+  p.group_c = stride_g;
+  p.vec = vector_bytes(Gp, ldg, stride_g, ce);
+  return finish(L, d->groups, 0, workspace, workspace_bytes, stream);
+}
+
+extern "C" tbStatus tb_matmul_blockscaled(const tb_grouped_desc* d, const void* A, int64_t lda, const tb_scales* sa,
+                                          const void* B, int64_t ldb, const tb_scales* sb, void* C, int64_t ldc,
+                                          void* workspace, size_t workspace_bytes, void* stream) {
+  tb_clear_error();
+  if (d && d->groups != 1) return tb_fail(TB_ERR_INVALID_ARGUMENT, "groups must be 1");
+  return run_rows(d, true, A, lda, sa, B, ldb, 0, sb, C, ldc, nullptr, workspace, workspace_bytes, stream);
+}
+
+extern "C" tbStatus tb_grouped_matmul_blockscaled(const tb_grouped_desc* d, const void* A, int64_t lda,
+                                                  const tb_scales* sa, const void* B, int64_t ldb, int64_t stride_b,
+                                                  const tb_scales* sb, void* C, int64_t ldc, const void* offsets,
+                                                  void* workspace, size_t workspace_bytes, void* stream) {
+  tb_clear_error();
+  if (d && d->a_col_major) return tb_fail(TB_ERR_UNSUPPORTED, "grouped rows need a row-major A");
+  if (d && d->groups > 0 && !offsets) return tb_fail(TB_ERR_INVALID_ARGUMENT, "offsets must not be NULL");
+  return run_rows(d, true, A, lda, sa, B, ldb, stride_b, sb, C, ldc, offsets, workspace, workspace_bytes, stream);
+}

@@ -42,21 +42,15 @@
 
 #include "tb_plan.h"
 #include "tb_sm100.cuh"
+#include "tb_wait.cuh"
 
 using namespace tb::sm100;
-
-__device__ uint32_t g_tb_status = 0;
 
 namespace {
 
 constexpr int kThreads = 192;
 constexpr int kCtaM = 128;            // tcgen05 M per CTA
 constexpr size_t kSmemLimit = 232448;  // 227 KB opt-in per CTA
-constexpr long long kWaitBudgetCycles = 2000000000LL;  // ≈1 s at 1.9 GHz
-
-constexpr uint32_t kSiteProducer = 1, kSiteMma = 2, kSiteEpilogue = 3, kSiteDrain = 4,
-                   kSiteSelfTest = 5;
-
 // G = CTAs per tile: 1 (cta_group::1, 128-row tile) or 2 (cta_group::2 pair,
 // 256-row tile; each CTA holds 128 rows of A, BN/2 columns of B and 128
 // rows of the accumulator).
@@ -159,40 +153,6 @@ struct KParams {
   int64_t ldc;
   float* ws;
 };
-
-__device__ __forceinline__ void record_error(uint32_t code, uint32_t site) {
-  const uint32_t v = (code << 24) | (site << 16) | (blockIdx.x & 0xFFFFu);
-  atomicCAS(&g_tb_status, 0u, v);
-}
-
-// Bounded wait: false when the abort flag is up or the budget ran out.
-__device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity,
-                                             volatile int* abort_flag, uint32_t site) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (true) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if (*abort_flag) return false;
-    if (clock64() - t0 > kWaitBudgetCycles) {
-      record_error(TB_ERR_DEVICE_TIMEOUT, site);
-      *abort_flag = 1;
-      return false;
-    }
-  }
-}
-
-// Lane 0 waits (bounded), the result is broadcast so the warp stays converged.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
-                                          uint32_t site, int lane) {
-  // Every lane probes first with the non-blocking test_wait: in the common
-  // case (phase already complete) that is one probe, while a blocking
-  // try_wait costs hundreds of cycles even on a completed phase (measured:
-  // 142 → 118 cycles per MMA for a 128×128 tile, 154 → 132 for 128×256).
-  if (mbar_test_wait(bar, parity)) return true;
-  int ok = 0;
-  if (lane == 0) ok = wait_bounded(bar, parity, abort_flag, site);
-  return __shfl_sync(0xffffffffu, ok, 0) != 0;
-}
 
 struct Extent {
   int32_t m0, n0, rows, cols, k_begin, k_end, nkb, part;
@@ -1866,10 +1826,16 @@ extern "C" tbStatus tb_device_status(void* stream, uint32_t* raw) {
   e = cudaMemcpyFromSymbol(&v, g_tb_status, sizeof(v));
   if (e != cudaSuccess)
     return tb_fail(TB_ERR_CUDA, std::string("cudaMemcpyFromSymbol: ") + cudaGetErrorString(e));
-  if (raw) *raw = v;
   if (v != 0) {
     const uint32_t zero = 0;
     cudaMemcpyToSymbol(g_tb_status, &zero, sizeof(zero));
+  }
+  uint32_t grouped = 0;
+  const tbStatus st = tb_grouped_status(&grouped);
+  if (st != TB_OK) return st;
+  if (v == 0) v = grouped;
+  if (raw) *raw = v;
+  if (v != 0) {
     char hex[16];
     std::snprintf(hex, sizeof hex, "%08x", v);
     return tb_fail(TB_ERR_DEVICE_TIMEOUT, std::string("a device-side wait timed out (status 0x") + hex +

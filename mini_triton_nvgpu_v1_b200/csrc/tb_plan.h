@@ -113,6 +113,9 @@ std::string tb_describe_dynamic(const tb_matmul_plan* plan);
 void tb_choose_tail_split(int64_t items, int64_t slots, int64_t fills, int64_t* dp_items,
                           int64_t* tail_items, int64_t* tail_segs);
 
+// Reads and clears the status word of the grouped kernels (tb_grouped.cu).
+tbStatus tb_grouped_status(uint32_t* raw);
+
 // Thread-local error message helpers (tb_plan.cpp).
 tbStatus tb_fail(tbStatus code, const std::string& msg);
 void tb_clear_error();

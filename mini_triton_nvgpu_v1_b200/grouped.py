@@ -1,0 +1,364 @@
+"""Matrix products beside ``tb.matmul``: rows grouped by expert, and 8-bit
+operands with a scale per block of 128.
+
+    grouped_matmul        C[r] = beta·C[r] + A[r] · B[e]       r in [offsets[e], offsets[e + 1])
+    grouped_matmul_wgrad  G[e] = beta·G[e] + A[rows of e]^T · D[rows of e]
+    quantize_fp8          S = max|block| / 448, Q = e4m3(X / S)
+    matmul_fp8            C = beta·C + Σ_b SA[:, b] SB[b, :] (A_b · B_b), b = blocks of 128 along k
+    grouped_matmul_fp8    the same for the rows of each expert
+
+As ``tb.matmul``, they update their output in place (``beta=1``, the default,
+adds to it; ``beta=0`` overwrites) on the current stream of its device, and
+return it. Offsets stay on the device: no call waits for the GPU, and a captured
+CUDA graph follows their contents. Operands are strided views; rows that
+do not begin on 16-byte boundaries are copied first (into ``workspace``, or a
+buffer from torch's allocator).
+
+The gradients of ``C = grouped_matmul(A, B)`` for a gradient D of C are
+``grouped_matmul(D, B.transpose(1, 2), dA, offsets)`` and
+``grouped_matmul_wgrad(A, D, dB, offsets)``; those of ``matmul_fp8`` are
+``matmul_fp8`` of D quantised along n with B.t(), and of A^T with D, both
+quantised in blocks of 128 rows (``block=(128, 1)``).
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import TBError, _check, _lib
+from . import _capi
+from ._capi import TB_BF16, TB_E4M3, TB_ERR_INVALID_ARGUMENT, TB_ERR_UNSUPPORTED, TB_F16, TB_F32
+
+__all__ = ["grouped_matmul", "grouped_matmul_wgrad", "quantize_fp8", "matmul_fp8", "grouped_matmul_fp8"]
+
+_HALF = {torch.float16: TB_F16, torch.bfloat16: TB_BF16}
+_OUT = {torch.float32: TB_F32, torch.float16: TB_F16, torch.bfloat16: TB_BF16}
+_FP8 = torch.float8_e4m3fn
+
+# What a call's shapes, strides and types decide, by those (never by address).
+_SETUP: dict = {}
+
+
+def _bad(message: str, code: int = TB_ERR_INVALID_ARGUMENT):
+    return TBError(code, message)
+
+
+def _keep(key, made):
+    if len(_SETUP) > 1024:
+        _SETUP.clear()
+    _SETUP[key] = made
+    return made
+
+
+def _same_device(**tensors) -> int:
+    device = None
+    for name, t in tensors.items():
+        if not t.is_cuda:
+            raise _bad(f"{name} must be a CUDA tensor")
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise _bad(f"{name} is on {t.device}, the others on {device}")
+    return device.index
+
+
+def _rows(t, name: str) -> int:
+    """Leading dimension of the row-major matrices t (…, rows, cols)."""
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise _bad(f"{name} must have a unit stride along its columns", TB_ERR_UNSUPPORTED)
+    return t.stride(-2) if t.shape[-2] > 1 else max(1, t.shape[-1])
+
+
+def _either(t, name: str) -> tuple[bool, int]:
+    """(column-major?, leading dimension) of the matrices t (…, rows, cols)."""
+    r, c = t.shape[-2:]
+    by_row = c <= 1 or t.stride(-1) == 1
+    by_col = r <= 1 or t.stride(-2) == 1
+    if by_col and (c <= 1 or not by_row):
+        return True, t.stride(-1) if c > 1 else max(1, r)
+    if not by_row:
+        raise _bad(f"{name} must have a unit stride along its rows or its columns", TB_ERR_UNSUPPORTED)
+    return False, t.stride(-2) if r > 1 else max(1, c)
+
+
+def _batch(t, name: str) -> int:
+    """Stride between the matrices of t (groups, rows, cols), which may not overlap."""
+    e, r, c = t.shape
+    if e <= 1 or t.numel() == 0:
+        return max(1, r * c)
+    spans = sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1)
+    reach = 1
+    for st, sz in spans:
+        if st < reach:
+            raise _bad(f"the matrices of {name} overlap", TB_ERR_UNSUPPORTED)
+        reach = st * (sz - 1) + reach
+    return t.stride(0)
+
+
+def _check_offsets(offsets, groups: int) -> int:
+    if offsets.dim() != 1 or offsets.shape[0] != groups + 1:
+        raise _bad(f"offsets must hold {groups + 1} entries, one more than there are groups")
+    if offsets.dtype not in (torch.int32, torch.int64):
+        raise _bad("offsets must be int32 or int64")
+    if not offsets.is_contiguous():
+        raise _bad("offsets must be contiguous")
+    return 1 if offsets.dtype == torch.int64 else 0
+
+
+def _desc(groups, rows, n, k, ab, c, beta, a_col, b_col, long_) -> _capi.tb_grouped_desc:
+    if beta not in (0, 1):
+        raise _bad("beta must be 0 or 1")
+    d = _capi.tb_grouped_desc()
+    d.groups, d.rows, d.n, d.k = groups, rows, n, k
+    d.ab_dtype, d.c_dtype, d.beta = ab, c, int(beta)
+    d.a_col_major, d.b_col_major, d.offsets_long = int(a_col), int(b_col), long_
+    return d
+
+
+def _scratch(need: int, workspace, device, stream):
+    """(address, bytes, tensor to keep) of a call's workspace."""
+    if not need:
+        return None, 0, None
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        if stream is not None:
+            workspace.record_stream(stream)
+    elif not workspace.is_cuda or workspace.device != device or not workspace.is_contiguous():
+        raise _bad("workspace must be a contiguous CUDA tensor on the operands' device")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
+
+
+def _call(dev: int, stream, fn, *args) -> None:
+    """fn(*args, stream) with `dev` current."""
+    sp = stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(dev)
+    if torch._C._cuda_getDevice() == dev:
+        code = fn(*args, sp or None)
+    else:
+        with torch.cuda.device(dev):
+            code = fn(*args, sp or None)
+    if code:
+        _check(code)
+
+
+def _setup_grouped(key, A, B, Cm, offsets, beta, fp8_scales):
+    if A.dim() != 2 or B.dim() != 3 or Cm.dim() != 2:
+        raise _bad("grouped products take A [rows, k], B [groups, k, n] and C [rows, n]")
+    rows, k = A.shape
+    groups, kb, n = B.shape
+    if kb != k or tuple(Cm.shape) != (rows, n):
+        raise _bad("operand shapes disagree: A [rows, k], B [groups, k, n], C [rows, n]")
+    if fp8_scales is None:
+        if A.dtype not in _HALF or B.dtype != A.dtype:
+            raise _bad("A and B must both be f16 or both be bf16")
+        ab = _HALF[A.dtype]
+    else:
+        if A.dtype != _FP8 or B.dtype != _FP8:
+            raise _bad("A and B must be float8_e4m3fn")
+        ab = TB_E4M3
+    if Cm.dtype not in _OUT:
+        raise _bad("C must be f32, f16 or bf16")
+    long_ = _check_offsets(offsets, groups)
+    b_col, ldb = _either(B, "B")
+    lda, ldc = _rows(A, "A"), _rows(Cm, "C")
+    d = _desc(groups, rows, n, k, ab, _OUT[Cm.dtype], beta, False, b_col, long_)
+    stride_b = _batch(B, "B")
+    el = 1 if fp8_scales is not None else 2
+    even = not (lda * el % 16 or ldb * el % 16 or stride_b * el % 16)
+    return d, lda, ldb, stride_b, ldc, even
+
+
+def _need(even, d, A, lda, B, ldb, stride_b) -> int:
+    if even and not (A.data_ptr() | B.data_ptr()) & 15:
+        return 0
+    return _lib.tb_grouped_matmul_workspace_bytes(C.byref(d), A.data_ptr(), lda, B.data_ptr(), ldb, stride_b)
+
+
+def grouped_matmul(A, B, Cm, offsets, *, beta: int = 1, workspace=None, stream=None):
+    """C[r] ← beta·C[r] + A[r] · B[e] for the rows r in [offsets[e],
+    offsets[e + 1]) of every group e. A [rows, k] and B [groups, k, n] f16 or
+    bf16 (B row-major, or a transposed view of weights kept as n × k), C
+    [rows, n] f32, f16 or bf16, offsets groups + 1 int32 or int64 on the
+    device. Rows outside every group keep what C held. Returns C."""
+    key = ("g", A.shape, B.shape, Cm.shape, A.stride(), B.stride(), Cm.stride(), A.dtype, B.dtype, Cm.dtype,
+           A.device, B.device, Cm.device, offsets.shape, offsets.stride(), offsets.dtype, offsets.device, beta)
+    hit = _SETUP.get(key)
+    if hit is None:
+        dev = _same_device(A=A, B=B, C=Cm, offsets=offsets)
+        hit = _keep(key, (dev, *_setup_grouped(key, A, B, Cm, offsets, beta, None)))
+    dev, d, lda, ldb, stride_b, ldc, even = hit
+    ws, nbytes, _kept = _scratch(_need(even, d, A, lda, B, ldb, stride_b), workspace, Cm.device, stream)
+    _call(dev, stream, _lib.tb_grouped_matmul, d, A.data_ptr(), lda, B.data_ptr(), ldb, stride_b, Cm.data_ptr(), ldc,
+          offsets.data_ptr(), ws, nbytes)
+    return Cm
+
+
+def grouped_matmul_wgrad(A, D, G, offsets, *, beta: int = 1, workspace=None, stream=None):
+    """G[e] ← beta·G[e] + A[rows of e]^T · D[rows of e]: the gradient of the
+    weights of :func:`grouped_matmul` from the gradient D of its output.
+    A [rows, k] and D [rows, n] f16 or bf16, G [groups, k, n] f32, f16 or
+    bf16. A group without rows gets beta·G[e]. Returns G."""
+    key = ("w", A.shape, D.shape, G.shape, A.stride(), D.stride(), G.stride(), A.dtype, D.dtype, G.dtype,
+           A.device, D.device, G.device, offsets.shape, offsets.stride(), offsets.dtype, offsets.device, beta)
+    hit = _SETUP.get(key)
+    if hit is None:
+        dev = _same_device(A=A, D=D, G=G, offsets=offsets)
+        if A.dim() != 2 or D.dim() != 2 or G.dim() != 3:
+            raise _bad("the weight gradient takes A [rows, k], D [rows, n] and G [groups, k, n]")
+        rows, k = A.shape
+        groups, n = G.shape[0], D.shape[1]
+        if D.shape[0] != rows or tuple(G.shape) != (groups, k, n):
+            raise _bad("operand shapes disagree: A [rows, k], D [rows, n], G [groups, k, n]")
+        if A.dtype not in _HALF or D.dtype != A.dtype:
+            raise _bad("A and D must both be f16 or both be bf16")
+        if G.dtype not in _OUT:
+            raise _bad("G must be f32, f16 or bf16")
+        long_ = _check_offsets(offsets, groups)
+        lda, ldd, ldg = _rows(A, "A"), _rows(D, "D"), _rows(G, "G")
+        d = _desc(groups, rows, n, k, _HALF[A.dtype], _OUT[G.dtype], beta, False, False, long_)
+        hit = _keep(key, (dev, d, lda, ldd, ldg, _batch(G, "G"), not (lda * 2 % 16 or ldd * 2 % 16)))
+    dev, d, lda, ldd, ldg, stride_g, even = hit
+    need = 0
+    if not even or (A.data_ptr() | D.data_ptr()) & 15:
+        need = _lib.tb_grouped_matmul_wgrad_workspace_bytes(C.byref(d), A.data_ptr(), lda, D.data_ptr(), ldd)
+    ws, nbytes, _kept = _scratch(need, workspace, G.device, stream)
+    _call(dev, stream, _lib.tb_grouped_matmul_wgrad, d, A.data_ptr(), lda, D.data_ptr(), ldd, G.data_ptr(), ldg,
+          stride_g, offsets.data_ptr(), ws, nbytes)
+    return G
+
+
+def _blocks(n: int) -> int:
+    return (n + 127) // 128
+
+
+def quantize_fp8(X, Q=None, S=None, *, block=(1, 128), stream=None):
+    """Q ← e4m3(448 · X / m), S ← m / 448 with m = max(max|block|, 448 · 2^-63)
+    for every block (1, 128), (128, 1) or (128, 128) of X [rows, cols] or
+    [batch, rows, cols] (f32, f16 or bf16). Q: float8_e4m3fn of X's shape; S:
+    f32 [(batch,) ceil(rows / block[0]), ceil(cols / block[1])]. A Q that is
+    not given is made with rows that begin on 16-byte boundaries, as the
+    8-bit products read them without a copy. Returns (Q, S)."""
+    br, bc = block
+    if (br, bc) not in ((1, 128), (128, 1), (128, 128)):
+        raise _bad("blocks are (1, 128), (128, 1) or (128, 128)")
+    if X.dim() not in (2, 3):
+        raise _bad("X must be [rows, cols] or [batch, rows, cols]")
+    if not X.is_cuda:
+        raise _bad("X must be a CUDA tensor")
+    if Q is None:
+        rows, cols = X.shape[-2:]
+        Q = torch.empty(*X.shape[:-1], (cols + 15) // 16 * 16, dtype=torch.uint8, device=X.device).view(_FP8)
+        Q = Q[..., :cols]
+        if stream is not None:
+            Q.record_stream(stream)
+    if S is None:
+        S = torch.empty(*X.shape[:-2], -(-X.shape[-2] // br), -(-X.shape[-1] // bc), device=X.device,
+                        dtype=torch.float32)
+        if stream is not None:
+            S.record_stream(stream)
+    key = ("q", X.shape, Q.shape, S.shape, X.stride(), Q.stride(), S.stride(), X.dtype, Q.dtype, S.dtype,
+           X.device, Q.device, S.device, br, bc)
+    hit = _SETUP.get(key)
+    if hit is None:
+        dev = _same_device(X=X, Q=Q, S=S)
+        if X.dtype not in _OUT:
+            raise _bad("X must be f32, f16 or bf16")
+        if Q.dtype != _FP8 or Q.shape != X.shape:
+            raise _bad("Q must be float8_e4m3fn of X's shape")
+        rows, cols = X.shape[-2:]
+        if S.dtype != torch.float32 or tuple(S.shape) != (*X.shape[:-2], -(-rows // br), -(-cols // bc)):
+            raise _bad("S must be f32 with one entry for each block")
+        d = _capi.tb_quantize_desc()
+        d.batch, d.rows, d.cols = (X.shape[0] if X.dim() == 3 else 1), rows, cols
+        d.block_rows, d.block_cols, d.x_dtype = br, bc, _OUT[X.dtype]
+        batched = X.dim() == 3
+        if batched:
+            _batch(Q, "Q")
+            _batch(S, "S")
+        hit = _keep(key, (dev, d, _rows(X, "X"), X.stride(0) if batched else 0, _rows(Q, "Q"),
+                          Q.stride(0) if batched else 0, S.stride(0) if batched else 0, S.stride(-2), S.stride(-1)))
+    dev, d, ldx, bx, ldq, bq, bs, s_row, s_col = hit
+    _call(dev, stream, _lib.tb_quantize_blocks, d, X.data_ptr(), ldx, bx, Q.data_ptr(), ldq, bq, S.data_ptr(), bs,
+          s_row, s_col)
+    return Q, S
+
+
+def _scales(s, name: str, mn: int, k: int, mn_axis: int, k_axis: int, lead: tuple) -> _capi.tb_scales:
+    if s.dtype != torch.float32 or s.dim() != len(lead) + 2 or tuple(s.shape[:-2]) != lead:
+        raise _bad(f"{name} must be f32 with one entry for each block")
+    per = s.shape[mn_axis]
+    if s.shape[k_axis] != _blocks(k) or per not in (mn, _blocks(mn)):
+        raise _bad(f"{name} must hold one scale for 1 or 128 rows or columns and 128 elements along k")
+    sc = _capi.tb_scales()
+    sc.stride_group = s.stride(0) if lead else 0
+    sc.stride_mn, sc.stride_k = s.stride(mn_axis), s.stride(k_axis)
+    sc.block = 1 if per == mn else 128
+    return sc
+
+
+def matmul_fp8(A, SA, B, SB, Cm, *, beta: int = 1, workspace=None, stream=None):
+    """C ← beta·C + Σ_b SA[:, b] SB[b, :] (A_b · B_b), b = blocks of 128 along
+    k. A [m, k] and B [k, n] float8_e4m3fn, each row-major or a transposed
+    view; SA f32 [m or ceil(m / 128), ceil(k / 128)]; SB f32 [ceil(k / 128),
+    n or ceil(n / 128)]; C [m, n] f32, f16 or bf16. The sum over a block and
+    over the blocks is in f32. Returns C."""
+    key = ("f", A.shape, B.shape, Cm.shape, SA.shape, SB.shape, A.stride(), B.stride(), Cm.stride(), SA.stride(),
+           SB.stride(), A.dtype, B.dtype, Cm.dtype, SA.dtype, SB.dtype, A.device, B.device, Cm.device, SA.device,
+           SB.device, beta)
+    hit = _SETUP.get(key)
+    if hit is None:
+        dev = _same_device(A=A, SA=SA, B=B, SB=SB, C=Cm)
+        if A.dim() != 2 or B.dim() != 2 or Cm.dim() != 2:
+            raise _bad("matmul_fp8 takes A [m, k], B [k, n] and C [m, n]")
+        m, k = A.shape
+        n = B.shape[1]
+        if B.shape[0] != k or tuple(Cm.shape) != (m, n):
+            raise _bad("operand shapes disagree: A [m, k], B [k, n], C [m, n]")
+        if A.dtype != _FP8 or B.dtype != _FP8:
+            raise _bad("A and B must be float8_e4m3fn")
+        if Cm.dtype not in _OUT:
+            raise _bad("C must be f32, f16 or bf16")
+        a_col, lda = _either(A, "A")
+        b_col, ldb = _either(B, "B")
+        d = _desc(1, m, n, k, TB_E4M3, _OUT[Cm.dtype], beta, a_col, b_col, 0)
+        hit = _keep(key, (dev, d, lda, ldb, _rows(Cm, "C"), _scales(SA, "SA", m, k, 0, 1, ()),
+                          _scales(SB, "SB", n, k, 1, 0, ()), not (lda % 16 or ldb % 16)))
+    dev, d, lda, ldb, ldc, sa, sb, even = hit
+    ws, nbytes, _kept = _scratch(_need(even, d, A, lda, B, ldb, 0), workspace, Cm.device, stream)
+    sa, sb = _at(sa, SA), _at(sb, SB)
+    _call(dev, stream, _lib.tb_matmul_blockscaled, d, A.data_ptr(), lda, sa, B.data_ptr(), ldb, sb, Cm.data_ptr(), ldc,
+          ws, nbytes)
+    return Cm
+
+
+def _at(scales, tensor) -> _capi.tb_scales:
+    """The layout `scales` at a tensor's address (a copy: threads share the layout)."""
+    s = _capi.tb_scales.from_buffer_copy(scales)
+    s.ptr = tensor.data_ptr()
+    return s
+
+
+def grouped_matmul_fp8(A, SA, B, SB, Cm, offsets, *, beta: int = 1, workspace=None, stream=None):
+    """:func:`matmul_fp8` for the rows of each group (:func:`grouped_matmul`):
+    A [rows, k] with SA [rows, ceil(k / 128)], B [groups, k, n] (row-major, or a
+    transposed view) with SB [groups, ceil(k / 128), n or ceil(n / 128)].
+    Returns C."""
+    key = ("h", A.shape, B.shape, Cm.shape, SA.shape, SB.shape, A.stride(), B.stride(), Cm.stride(), SA.stride(),
+           SB.stride(), A.dtype, B.dtype, Cm.dtype, SA.dtype, SB.dtype, A.device, B.device, Cm.device, SA.device,
+           SB.device, offsets.shape, offsets.stride(), offsets.dtype, offsets.device, beta)
+    hit = _SETUP.get(key)
+    if hit is None:
+        dev = _same_device(A=A, SA=SA, B=B, SB=SB, C=Cm, offsets=offsets)
+        made = _setup_grouped(key, A, B, Cm, offsets, beta, (SA, SB))
+        rows, k = A.shape
+        groups, _, n = B.shape
+        if SA.dim() != 2 or SA.shape[0] != rows:
+            raise _bad("SA must hold a scale for each row of A and 128 elements along k")
+        hit = _keep(key, (dev, *made, _scales(SA, "SA", rows, k, 0, 1, ()),
+                          _scales(SB, "SB", n, k, 2, 1, (groups,))))
+    dev, d, lda, ldb, stride_b, ldc, even, sa, sb = hit
+    ws, nbytes, _kept = _scratch(_need(even, d, A, lda, B, ldb, stride_b), workspace, Cm.device, stream)
+    sa, sb = _at(sa, SA), _at(sb, SB)
+    _call(dev, stream, _lib.tb_grouped_matmul_blockscaled, d, A.data_ptr(), lda, sa, B.data_ptr(), ldb, stride_b, sb,
+          Cm.data_ptr(), ldc, offsets.data_ptr(), ws, nbytes)
+    return Cm

@@ -1,0 +1,342 @@
+"""GPU: products of rows grouped by expert and their weight gradients,
+against the formula in 64 bits.
+
+Most inputs are small whole numbers: every product and every partial sum is
+then exact in f32 (|sum| < 2^24), so the f32 output has to be equal, and a
+16-bit output has to be the exact value rounded once."""
+from __future__ import annotations
+
+import itertools
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+OUT = {"f32": "float32", "f16": "float16", "bf16": "bfloat16"}
+
+
+def _types(name):
+    import torch
+    return getattr(torch, OUT[name])
+
+
+def _ints(shape, g, dtype, most=3):
+    import torch
+    return torch.randint(-most, most + 1, shape, generator=g, device="cuda").to(dtype)
+
+
+def _offsets(sizes, before=0, dtype=None):
+    import torch
+    ends = [before]
+    for s in sizes:
+        ends.append(ends[-1] + s)
+    return torch.tensor(ends, dtype=dtype or torch.int32, device="cuda"), ends
+
+
+def _reference(A, B, C, ends, beta):
+    out = C.double().clone()
+    for e, (lo, hi) in enumerate(zip(ends, ends[1:])):
+        out[lo:hi] = A[lo:hi].double() @ B[e].double() + (out[lo:hi] if beta else 0)
+    return out
+
+
+# One shape for each kernel and the edges of each: (sizes of the groups, k, n)
+SHAPES = {
+    "one row": ([1], 8, 8),
+    "one of everything": ([1], 1, 1),
+    "empty groups": ([0, 3, 0, 0, 5, 0], 64, 64),
+    "only empty": ([0, 0, 0], 64, 64),
+    "decode": ([1, 0, 2, 1, 1, 0, 3, 1], 1024, 512),
+    "decode, k ends inside a fill": ([2, 7, 1], 1000, 200),
+    "33 rows": ([33, 31, 32], 256, 96),
+    "odd widths": ([5, 130, 0, 127], 37, 51),
+    "rows 96 and 97": ([96, 97, 128, 129], 136, 264),
+    "128-wide tiles": ([100, 128, 60, 90, 128, 1, 77, 128], 192, 2432),
+    "pair tiles": ([300, 0, 257, 700, 256, 487], 200, 2568),
+    "pair tiles, many fills": ([512, 513, 511, 512], 1032, 2560),
+    "many groups": ([i % 5 for i in range(300)], 72, 136),
+}
+
+
+@pytest.mark.parametrize("name", list(SHAPES))
+@pytest.mark.parametrize("dtype,out,layout,beta", [("bf16", "f32", "kn", 1), ("f16", "f32", "nk", 0),
+                                                   ("bf16", "bf16", "nk", 1), ("f16", "f16", "kn", 0)])
+def test_grouped_matmul(cuda, name, dtype, out, layout, beta):
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    sizes, k, n = SHAPES[name]
+    g = torch.Generator(device="cuda")
+    g.manual_seed(len(name) + k)
+    dt = _types(dtype)
+    before, behind = (3, 5) if len(sizes) > 1 else (0, 0)
+    off, ends = _offsets(sizes, before, torch.int64 if beta else torch.int32)
+    rows = ends[-1] + behind
+    A = _ints((rows, k), g, dt)
+    A[:before] = float("nan")            # rows of no group: never part of a result
+    A[ends[-1]:] = float("inf")
+    E = len(sizes)
+    B = _ints((E, k, n), g, dt) if layout == "kn" else _ints((E, n, k), g, dt).transpose(1, 2)
+    C = _ints((rows, n), g, _types(out), 7)
+    ref = _reference(A, B, C, ends, beta)
+    got = tb.grouped_matmul(A, B, C, off, beta=beta)
+    tb.device_status()
+    assert got is C
+    assert torch.equal(C, ref.to(C.dtype))
+
+
+@pytest.mark.parametrize("name", list(SHAPES))
+@pytest.mark.parametrize("dtype,out,beta", [("bf16", "f32", 1), ("f16", "f16", 0), ("bf16", "bf16", 0)])
+def test_grouped_matmul_wgrad(cuda, name, dtype, out, beta):
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    sizes, k, n = SHAPES[name]
+    if len(sizes) > 100:
+        k, n = 24, 40
+    g = torch.Generator(device="cuda")
+    g.manual_seed(len(name) + n)
+    dt = _types(dtype)
+    before, behind = (3, 5) if len(sizes) > 1 else (0, 0)
+    off, ends = _offsets(sizes, before)
+    rows = ends[-1] + behind
+    A, D = _ints((rows, k), g, dt, 2), _ints((rows, n), g, dt, 2)
+    for t in (A, D):
+        t[:before] = float("nan")
+        t[ends[-1]:] = float("inf")
+    G = _ints((len(sizes), k, n), g, _types(out), 7)
+    ref = torch.stack([A[lo:hi].double().t() @ D[lo:hi].double() for lo, hi in zip(ends, ends[1:])])
+    if beta:
+        ref += G.double()
+    tb.grouped_matmul_wgrad(A, D, G, off, beta=beta)
+    tb.device_status()
+    assert torch.equal(G, ref.to(G.dtype))
+
+
+@pytest.mark.parametrize("k,n", [(2304, 2560), (136, 264)])   # pair tiles, one-CTA tiles
+def test_wgrad_every_length_inside_a_fill(cuda, k, n):
+    """Groups of 64·j + r rows for every r, their neighbours' rows NaN and infinite."""
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(5)
+    for r in range(0, 64, 7 if k > 1000 else 1):
+        sizes = [64 + r, 3, r, 129]
+        off, ends = _offsets(sizes, 1)
+        A, D = _ints((ends[-1] + 2, k), g, torch.bfloat16, 2), _ints((ends[-1] + 2, n), g, torch.bfloat16, 2)
+        A[ends[1]:ends[2]] = float("nan")  # group 1's gradient is NaN, its neighbours' are not
+        D[ends[1]:ends[2]] = float("inf")
+        G = torch.zeros(4, k, n, device="cuda")
+        tb.grouped_matmul_wgrad(A, D, G, off, beta=0)
+        for e in (0, 2, 3):
+            ref = A[ends[e]:ends[e + 1]].double().t() @ D[ends[e]:ends[e + 1]].double()
+            assert torch.equal(G[e], ref.float()), (r, e)
+        assert torch.isnan(G[1]).all()
+    tb.device_status()
+
+
+@pytest.mark.parametrize("dtype,out,layout", list(itertools.product(["f16", "bf16"], ["f32", "f16", "bf16"], ["kn", "nk"])))
+def test_real_values_round_once(cuda, dtype, out, layout):
+    """|error| <= (k + 2)·2^-23·Σ|a||b| for k additions in f32, each off by at most one unit in the last place,
+    and half a step of the output type for its rounding (f16 below 2^-14: half its least step, 2^-25)."""
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(11)
+    dt, od = _types(dtype), _types(out)
+    off, ends = _offsets([70, 0, 200, 41], 0)
+    k, n = 520, 328
+    A = torch.randn(ends[-1], k, generator=g, device="cuda").to(dt)
+    B = torch.randn(4, k, n, generator=g, device="cuda").to(dt)
+    if layout == "nk":
+        B = B.transpose(1, 2).contiguous().transpose(1, 2)
+    C = torch.randn(ends[-1], n, generator=g, device="cuda").to(od)
+    ref = _reference(A, B, C, ends, 1)
+    scale = _reference(A.abs(), B.abs(), C.abs(), ends, 1)
+    tb.grouped_matmul(A, B, C, off)
+    sums = (k + 2) * 2.0 ** -23 * scale
+    tol = sums + torch.finfo(od).eps / 2 * (ref.abs() + sums) + 2.0 ** -25
+    assert ((C.double() - ref).abs() <= tol).all()
+
+
+def test_strided_and_unaligned_operands(cuda):
+    """Views with a leading dimension, an odd base and transposed outputs' neighbours left alone."""
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    off, ends = _offsets([9, 0, 140, 3])
+    rows, k, n = ends[-1], 72, 88
+    for a_pad, a_skip, b_pad, c_skip in itertools.product([0, 8, 3], [0, 1, 8], [0, 5, 8], [0, 1, 4]):
+        A = _ints((rows, k + a_pad + a_skip), g, torch.float16)[:, a_skip:a_skip + k]
+        B = _ints((4, k + 1, n + b_pad), g, torch.float16)[:, :k, b_pad:]
+        whole = _ints((rows, n + 2 * c_skip), g, torch.float32, 7)
+        C = whole[:, c_skip:c_skip + n]
+        want = whole.double().clone()
+        want[:, c_skip:c_skip + n] = _reference(A, B, C, ends, 1)
+        tb.grouped_matmul(A, B, C, off)
+        assert torch.equal(whole.double(), want)
+        G = torch.zeros(4, k, n + c_skip, device="cuda", dtype=torch.float32)
+        D = _ints((rows, n + b_pad), g, torch.float16)[:, b_pad:]
+        tb.grouped_matmul_wgrad(A, D, G[:, :, c_skip:], off)
+        ref = torch.stack([A[lo:hi].double().t() @ D[lo:hi].double() for lo, hi in zip(ends, ends[1:])])
+        assert torch.equal(G[:, :, c_skip:].double(), ref)
+        assert not G[:, :, :c_skip].any()
+    tb.device_status()
+
+
+def test_weights_in_interleaved_layouts(cuda):
+    """B [groups, k, n] as a view of (k, groups, n) and of (n, groups, k) storage; G as a view of (k, groups, n)."""
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(4)
+    off, ends = _offsets([40, 7, 0, 90])
+    k, n = 80, 104
+    A = _ints((ends[-1], k), g, torch.bfloat16)
+    for B in (_ints((k, 4, n), g, torch.bfloat16).permute(1, 0, 2), _ints((n, 4, k), g, torch.bfloat16).permute(1, 2, 0)):
+        C = torch.zeros(ends[-1], n, device="cuda")
+        tb.grouped_matmul(A, B, C, off, beta=0)
+        assert torch.equal(C.double(), _reference(A, B, C, ends, 0))
+    D = _ints((ends[-1], n), g, torch.bfloat16)
+    G = torch.zeros(k, 4, n, device="cuda").permute(1, 0, 2)
+    tb.grouped_matmul_wgrad(A, D, G, off)
+    ref = torch.stack([A[lo:hi].double().t() @ D[lo:hi].double() for lo, hi in zip(ends, ends[1:])])
+    assert torch.equal(G.double(), ref)
+
+
+def test_no_rows_and_no_columns(cuda):
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    h = dict(device="cuda", dtype=torch.float16)
+    zero = torch.zeros(3, dtype=torch.int32, device="cuda")
+    C = torch.ones(4, 16, device="cuda")
+    # k = 0: the rows of a group become beta·C, others stay
+    tb.grouped_matmul(torch.empty(4, 0, **h), torch.empty(2, 0, 16, **h), C,
+                      torch.tensor([0, 1, 3], dtype=torch.int32, device="cuda"), beta=0)
+    assert torch.equal(C, torch.tensor([0., 0, 0, 1], device="cuda")[:, None].expand(4, 16))
+    tb.grouped_matmul(torch.empty(0, 8, **h), torch.ones(2, 8, 16, **h), torch.empty(0, 16, device="cuda"), zero)
+    tb.grouped_matmul(torch.ones(4, 8, **h), torch.ones(2, 8, 0, **h), torch.empty(4, 0, device="cuda"), zero)
+    tb.grouped_matmul(torch.ones(4, 8, **h), torch.ones(0, 8, 16, **h), C, zero[:1])
+    G = torch.ones(2, 8, 16, device="cuda")
+    tb.grouped_matmul_wgrad(torch.empty(0, 8, **h), torch.empty(0, 16, **h), G, zero)
+    assert (G == 1).all()
+    tb.grouped_matmul_wgrad(torch.empty(0, 8, **h), torch.empty(0, 16, **h), G, zero, beta=0)
+    assert not G.any()
+    tb.device_status()
+
+
+def test_offsets_outside_the_rows_are_clamped(cuda):
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(8)
+    A, B = _ints((50, 64), g, torch.float16), _ints((3, 64, 64), g, torch.float16)
+    for bad in ([-9, 20, 30, 1 << 30], [-(1 << 31), 20, 30, 50]):
+        C = torch.zeros(50, 64, device="cuda")
+        tb.grouped_matmul(A, B, C, torch.tensor(bad, dtype=torch.int32, device="cuda"))
+        assert torch.equal(C.double(), _reference(A, B, C * 0, [0, 20, 30, 50], 0))
+    C = torch.zeros(50, 64, device="cuda")   # a falling pair is an empty group
+    tb.grouped_matmul(A, B, C, torch.tensor([10, 40, 5, 5], dtype=torch.int64, device="cuda"))
+    assert torch.equal(C.double(), _reference(A, B, C * 0, [10, 40, 40, 40], 0))
+    G = torch.zeros(3, 64, 64, device="cuda")
+    tb.grouped_matmul_wgrad(A, A, G, torch.tensor([-5, 20, 30, 99], dtype=torch.int64, device="cuda"))
+    ref = torch.stack([A[a:b].double().t() @ A[a:b].double() for a, b in ((0, 20), (20, 30), (30, 50))])
+    assert torch.equal(G.double(), ref)
+    tb.device_status()
+
+
+def test_results_repeat_bit_for_bit(cuda):
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(9)
+    off, ends = _offsets([3, 1, 0, 4])
+    A = torch.randn(8, 4096, generator=g, device="cuda").bfloat16()
+    B = torch.randn(4, 4096, 512, generator=g, device="cuda").bfloat16()
+    runs = [tb.grouped_matmul(A, B, torch.zeros(8, 512, device="cuda"), off).clone() for _ in range(5)]
+    assert all(torch.equal(r, runs[0]) for r in runs)
+
+
+def test_a_captured_graph_follows_the_offsets(cuda):
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(10)
+    rows, k, n = 400, 136, 200
+    A, B = _ints((rows, k), g, torch.bfloat16), _ints((4, k, n), g, torch.bfloat16)
+    D = _ints((rows, n), g, torch.bfloat16, 2)
+    C, G = torch.zeros(rows, n, device="cuda"), torch.zeros(4, k, n, device="cuda")
+    off, _ = _offsets([100, 100, 100, 100])
+    tb.grouped_matmul(A, B, C, off, beta=0)
+    tb.grouped_matmul_wgrad(A, D, G, off, beta=0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tb.grouped_matmul(A, B, C, off, beta=0)
+        tb.grouped_matmul_wgrad(A, D, G, off, beta=0)
+    for sizes in ([1, 0, 399, 0], [0, 0, 0, 400], [130, 5, 65, 200]):
+        new, ends = _offsets(sizes)
+        off.copy_(new)
+        C.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(C.double(), _reference(A, B, torch.zeros_like(C), ends, 0))
+        ref = torch.stack([A[lo:hi].double().t() @ D[lo:hi].double() for lo, hi in zip(ends, ends[1:])])
+        assert torch.equal(G.double(), ref)
+
+
+def test_streams(cuda):
+    """Two calls at once on two streams, one of them with repacked operands."""
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(12)
+    off, ends = _offsets([200, 33, 0, 90])
+    sets = []
+    for k in (136, 137):
+        A, B = _ints((ends[-1], k), g, torch.float16), _ints((4, k, 264), g, torch.float16)
+        sets.append((A, B, torch.zeros(ends[-1], 264, device="cuda")))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):
+        for (A, B, C), s in zip(sets, streams):
+            tb.grouped_matmul(A, B, C, off, beta=0, stream=s)
+    torch.cuda.synchronize()
+    for A, B, C in sets:
+        assert torch.equal(C.double(), _reference(A, B, C, ends, 0))
+
+
+def test_gradients_against_the_formula_and_differences(cuda):
+    """L = Σ W·C for C = grouped(A, B): dA and dB from the operators against the formula in 64 bits and against
+    differences of L, which is linear in A and in B, so that a difference quotient has no error but rounding.
+    Whole numbers: everything is exact."""
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(13)
+    off, ends = _offsets([20, 0, 150, 7])
+    k, n = 96, 80
+    A, B = _ints((ends[-1], k), g, torch.bfloat16, 2), _ints((4, k, n), g, torch.bfloat16, 2)
+    W = _ints((ends[-1], n), g, torch.bfloat16, 2)
+    dA = torch.zeros(ends[-1], k, device="cuda")
+    dB = torch.zeros(4, k, n, device="cuda")
+    tb.grouped_matmul(W, B.transpose(1, 2), dA, off, beta=0)
+    tb.grouped_matmul_wgrad(A, W, dB, off, beta=0)
+    a, b = A.double().requires_grad_(), B.double().requires_grad_()
+    loss = sum(((a[lo:hi] @ b[e]) * W[lo:hi].double()).sum() for e, (lo, hi) in enumerate(zip(ends, ends[1:])))
+    loss.backward()
+    assert torch.equal(dA.double(), a.grad) and torch.equal(dB.double(), b.grad)
+
+    def value(A, B):
+        C = torch.zeros(ends[-1], n, device="cuda")
+        tb.grouped_matmul(A, B, C, off, beta=0)
+        return (C.double() * W.double()).sum()
+
+    base = value(A, B)
+    for r, c in ((0, 0), (19, 95), (20, 3), (176, 50)):
+        moved = A.clone()
+        moved[r, c] += 1
+        assert value(moved, B) - base == dA[r, c].double()
+    for e, i, j in ((0, 0, 0), (1, 4, 4), (2, 95, 79), (3, 50, 1)):
+        moved = B.clone()
+        moved[e, i, j] += 1
+        assert value(A, moved) - base == dB[e, i, j].double()

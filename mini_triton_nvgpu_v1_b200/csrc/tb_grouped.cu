@@ -61,12 +61,24 @@ constexpr int kMaxGroups = 1024;
 constexpr int kMaxStages = 10;
 constexpr size_t kSmemLimitG = 232448;  // 227 KB opt-in per CTA
 
-enum Kind : int { kHalf = 0, kByte = 1 };  // 16-bit operands (f16 / bf16), 8-bit operands (e4m3)
+// kHalf      16-bit operands (f16 / bf16), the whole K range summed in TMEM
+// kHalfSum   16-bit operands, segments of kSumFills fills summed in f32 registers
+// kByte      8-bit operands (e4m3), a scale of B per 128 columns
+// kByteCol   8-bit operands, a scale of B per column
+enum Kind : int { kHalf = 0, kHalfSum = 1, kByte = 2, kByteCol = 3 };
+// The MMA truncates when it adds to its accumulator: the error of a sum grows
+// with the number of additions and leans one way. An f32 output takes it out
+// of TMEM every 4 fills (256 elements of K, 16 additions) and adds the
+// segments in registers, rounded to nearest.
+constexpr int kSumFills = 4;
 
 // KIND's ring fill is 128 bytes of K: 64 or 128 elements, four MMA K steps.
 template <int KIND, int BN, int G>
 struct GCfg {
-  static constexpr int kEl = KIND == kByte ? 1 : 2;
+  static constexpr bool kBytes = KIND == kByte || KIND == kByteCol;
+  static constexpr bool kSums = KIND != kHalf;          // sums held in registers
+  static constexpr int kSegFills = kBytes ? 1 : kSumFills;  // fills per accumulation in TMEM (kSums)
+  static constexpr int kEl = kBytes ? 1 : 2;
   static constexpr int kKB = 128 / kEl;                 // K elements per fill
   static constexpr int kMmaK = 32 / kEl;                // K elements per MMA
   static constexpr int kBM = 128 * G;                   // tile rows
@@ -96,6 +108,7 @@ struct GBars {
   uint64_t full[kMaxStages], empty[kMaxStages], fix[kMaxStages];
   uint64_t tfull[2], tempty[2];
   uint64_t drain, ready, consumed;
+  alignas(16) float col_scale[8][128];  // per epilogue warp: SB of its columns in the block at hand
   uint32_t tmem_holder;
   int abort_flag;
 };
@@ -277,6 +290,37 @@ __device__ __forceinline__ void emit32(const GParams& p, char* q, float (&v)[32]
   }
 }
 
+// Two f32 in one register pair.
+__device__ __forceinline__ uint64_t pack_u32x2(uint32_t a, uint32_t b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
+  return pack_u32x2(__float_as_uint(a), __float_as_uint(b));
+}
+__device__ __forceinline__ void unpack_f32x2(uint64_t v, float& a, float& b) {
+  uint32_t x, y;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(x), "=r"(y) : "l"(v));
+  a = __uint_as_float(x);
+  b = __uint_as_float(y);
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 template <int KIND, int BN, int G>
 __global__ void __launch_bounds__(kThreadsG, 1)
     tb_grouped_sm100_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA32,
@@ -353,14 +397,11 @@ __global__ void __launch_bounds__(kThreadsG, 1)
   const uint32_t tmem_base = bars.tmem_holder;
   const int32_t tiles = p.k_grouped ? p.groups * p.tiles_m * p.tiles_n : tab.cum[p.groups];
 
-  // 8-bit, 256 columns: the epilogue keeps 128 sums per thread. 256 threads ×
+  // Sums in registers, 256 columns: 128 per epilogue thread. 256 threads ×
   // 216 + 128 × 72 registers = the launch's 384 × 168.
-  constexpr bool kMoveRegs = KIND == kByte && BN == 256;
-  if constexpr (kMoveRegs) {
-    if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-  }
-
+  constexpr bool kMoveRegs = Cf::kSums && BN == 256;
+  if (warp < 4) {
+  if constexpr (kMoveRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     int stage = 0;
@@ -460,8 +501,9 @@ __global__ void __launch_bounds__(kThreadsG, 1)
       for (int32_t t = first; t < tiles && ok; t += stride) {
         const GTile g = tile_at<Cf::kBM, BN, Cf::kKB>(p, tab, t, part, cursor);
         for (int32_t f = g.f0; f < g.f1; ++f) {
-          const bool opens = KIND == kByte || f == g.f0;       // first fill of an accumulation
-          const bool closes = KIND == kByte || f + 1 == g.f1;  // last one
+          // first and last fill of an accumulation
+          const bool opens = Cf::kSums ? (f - g.f0) % Cf::kSegFills == 0 : f == g.f0;
+          const bool closes = f + 1 == g.f1 || (Cf::kSums && (f + 1 - g.f0) % Cf::kSegFills == 0);
           if (opens && !warp_wait(smem_addr(&bars.tempty[acc]), acc_phase ^ 1u, abort_flag, kSiteMma, lane)) {
             ok = false;
             break;
@@ -483,7 +525,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
                 const uint64_t da = da0 + (uint64_t)((a_step * kk) >> 4);
                 const uint64_t db = db0 + (uint64_t)((b_step * kk) >> 4);
                 const uint32_t add = (!opens || kk > 0) ? 1u : 0u;
-                if constexpr (KIND == kByte) umma_f8<G>(d, da, db, idesc, add);
+                if constexpr (Cf::kBytes) umma_f8<G>(d, da, db, idesc, add);
                 else if constexpr (G == 2) umma_f16_pair(d, da, db, idesc, add);
                 else umma_f16(d, da, db, idesc, add);
               }
@@ -561,7 +603,9 @@ __global__ void __launch_bounds__(kThreadsG, 1)
         }
       }
     }
-  } else if (warp >= 4) {
+  }
+  } else {
+    if constexpr (kMoveRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ------------------------------------------------------------ epilogue
     const int q = warp & 3;               // TMEM lane quarter
     const int half = (warp - 4) >> 2;     // column half
@@ -578,6 +622,37 @@ __global__ void __launch_bounds__(kThreadsG, 1)
         else mbar_arrive(tempty0 + acc * 8);
       }
     };
+    auto cluster_wait = [&](uint64_t* bar, uint32_t par) {
+      int good = 1;
+      if (lane == 0) {
+        const uint32_t b = smem_addr(bar);
+        const long long t0 = clock64();
+        while (!mbar_try_wait_cluster(b, par)) {
+          if (*abort_flag) {
+            good = 0;
+            break;
+          }
+          if (clock64() - t0 > kWaitBudgetCycles) {
+            record_error(TB_ERR_DEVICE_TIMEOUT, kSiteCluster);
+            *abort_flag = 1;
+            good = 0;
+            break;
+          }
+        }
+      }
+      good = __shfl_sync(0xffffffffu, good, 0);
+      return good != 0;
+    };
+    auto cluster_arrive = [&](uint64_t* bar) {
+      __syncwarp();
+      if (lane < p.split) mbar_arrive_cluster(map_to_cta(smem_addr(bar), (uint32_t)lane));
+    };
+    // this row's partial sums of chunk c, for the cluster
+    auto leave = [&](int c, const float (&s)[32]) {
+      float4* dst = reinterpret_cast<float4*>(red + (size_t)row_in_tile * Cf::kRedStride + (c_half + c * 32) * 4);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dst[i] = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+    };
     int acc = 0;
     uint32_t acc_phase = 0, red_phase = 0;
     int32_t cursor = 0;
@@ -588,50 +663,95 @@ __global__ void __launch_bounds__(kThreadsG, 1)
       const bool warp_ok = (int)rank * 128 + q * 32 < g.rows && c_half < g.cols;
       char* crow = static_cast<char*>(p.C) +
                    ((p.k_grouped ? (int64_t)g.e * p.group_c : 0) + ((int64_t)g.row0 + row_in_tile) * p.ldc + g.n0) * el;
-      float v[Cf::kChunks][32];
+      float v[Cf::kSums ? Cf::kChunks : 1][32];
 
-      if constexpr (KIND == kByte) {
-        const int32_t arow = min(g.row0 + row_in_tile, p.M - 1);  // masked rows read some valid scale
-        const float* sa = p.sa.p + (int64_t)(arow >> p.sa.shift) * p.sa.smn;
-        const float* sb = p.sb.p + (int64_t)g.e * p.sb.sg;
-        const int32_t col0 = min(g.n0 + c_half, p.N - 1);
+      if constexpr (Cf::kSums) {
+        // Each accumulation is taken from TMEM, scaled, and added to this
+        // thread's sums two at a time. A chunk's load runs while the one
+        // before it is added.
+        uint64_t sum[Cf::kChunks][16];
 #pragma unroll
         for (int c = 0; c < Cf::kChunks; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[c][i] = 0.f;
-        for (int32_t f = g.f0; f < g.f1; ++f) {
-          const float xa = __ldg(sa + (int64_t)f * p.sa.sk);
-          const float xb = p.sb.shift ? __ldg(sb + (int64_t)(col0 >> 7) * p.sb.smn + (int64_t)f * p.sb.sk) : 1.f;
+          for (int i = 0; i < 16; ++i) sum[c][i] = 0;
+        const float *sa = nullptr, *sb = nullptr;
+        int64_t sb_col[4] = {0, 0, 0, 0};
+        float xa = 1.f, xb = 1.f, xc[4] = {0.f, 0.f, 0.f, 0.f};
+        // scales of block f: this row's, and the columns' (one, or this
+        // lane's of the warp's columns); fetched a block ahead
+        auto fetch = [&](int32_t f) {
+          if (f >= g.f1) return;
+          xa = __ldg(sa + (int64_t)f * p.sa.sk);
+          if constexpr (KIND == kByte) xb = __ldg(sb + (int64_t)f * p.sb.sk);
+          if constexpr (KIND == kByteCol) {
+#pragma unroll
+            for (int j = 0; j < Cf::kHalfCols / 32; ++j) xc[j] = __ldg(sb + sb_col[j] + (int64_t)f * p.sb.sk);
+          }
+        };
+        if constexpr (Cf::kBytes) {
+          const int32_t arow = min(g.row0 + row_in_tile, p.M - 1);  // masked rows read some valid scale
+          sa = p.sa.p + (int64_t)(arow >> p.sa.shift) * p.sa.smn;
+          sb = p.sb.p + (int64_t)g.e * p.sb.sg;
+          if constexpr (KIND == kByte) {
+            sb += (int64_t)(min(g.n0 + c_half, p.N - 1) >> 7) * p.sb.smn;
+          } else {
+#pragma unroll
+            for (int j = 0; j < Cf::kHalfCols / 32; ++j)
+              sb_col[j] = (int64_t)min(g.n0 + c_half + 32 * j + lane, p.N - 1) * p.sb.smn;
+          }
+          fetch(g.f0);
+        }
+        for (int32_t f = g.f0; f < g.f1; f += Cf::kSegFills) {
           const float x = xa * xb;
+          float* cs = bars.col_scale[warp - 4];
+          if constexpr (KIND == kByteCol) {
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < Cf::kHalfCols / 32; ++j) cs[32 * j + lane] = xc[j];
+            __syncwarp();
+          }
+          if constexpr (Cf::kBytes) fetch(f + 1);
           if (!warp_wait(smem_addr(&bars.tfull[acc]), acc_phase, abort_flag, kSiteEpilogue, lane)) {
             ok = false;
             break;
           }
           tc_fence_after();
           if (warp_ok) {
+            uint32_t w[2][32];
+            const uint32_t ta = tm + (uint32_t)(acc * BN);
+            const uint64_t x2 = pack_f32x2(x, x);
+            tmem_ld_32x32b_x32_issue(ta, w[0]);
 #pragma unroll
             for (int c = 0; c < Cf::kChunks; ++c) {
-              float w[32];
-              tmem_ld_32x32b_x32(tm + (uint32_t)(acc * BN + c * 32), w);
-              if (p.sb.shift) {
+              tmem_ld_wait(w[c & 1]);
+              if (c + 1 < Cf::kChunks) tmem_ld_32x32b_x32_issue(ta + (uint32_t)((c + 1) * 32), w[(c + 1) & 1]);
+              else release(acc);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[c][i] = fmaf(w[i], x, v[c][i]);
-              } else {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                  const int32_t col = min(g.n0 + c_half + c * 32 + i, p.N - 1);
-                  v[c][i] = fmaf(w[i], x * __ldg(sb + (int64_t)col * p.sb.smn + (int64_t)f * p.sb.sk), v[c][i]);
+              for (int i = 0; i < 16; ++i) {
+                const uint64_t u = pack_u32x2(w[c & 1][2 * i], w[c & 1][2 * i + 1]);
+                if constexpr (KIND == kHalfSum) {
+                  sum[c][i] = add_f32x2(sum[c][i], u);
+                } else if constexpr (KIND == kByte) {
+                  sum[c][i] = fma_f32x2(u, x2, sum[c][i]);
+                } else {
+                  const uint64_t y = *reinterpret_cast<const uint64_t*>(cs + c * 32 + 2 * i);
+                  sum[c][i] = fma_f32x2(u, mul_f32x2(x2, y), sum[c][i]);
                 }
               }
             }
+          } else {
+            release(acc);
           }
-          release(acc);
           if (++acc == 2) {
             acc = 0;
             acc_phase ^= 1u;
           }
         }
         if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < Cf::kChunks; ++c)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) unpack_f32x2(sum[c][i], v[c][2 * i], v[c][2 * i + 1]);
       } else {
         if (g.f1 > g.f0) {
           if (!warp_wait(smem_addr(&bars.tfull[acc]), acc_phase, abort_flag, kSiteEpilogue, lane)) {
@@ -641,29 +761,27 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           tc_fence_after();
         }
         if (p.split > 1) {
-#pragma unroll
-          for (int c = 0; c < Cf::kChunks; ++c) {
-            if (g.f1 > g.f0) {
-              tmem_ld_32x32b_x32(tm + (uint32_t)(acc * BN + c * 32), v[c]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[c][i] = 0.f;
-            }
+          // every CTA has read the previous tile's partial sums
+          if (!cluster_wait(&bars.consumed, red_phase ^ 1u)) {
+            ok = false;
+            break;
           }
-        } else {
+        }
 #pragma unroll
-          for (int c = 0; c < Cf::kChunks; ++c) {
-            if (!warp_ok) break;
-            if (g.f1 > g.f0) {
-              tmem_ld_32x32b_x32(tm + (uint32_t)(acc * BN + c * 32), v[0]);
-            } else {
+        for (int c = 0; c < Cf::kChunks; ++c) {
+          if (!warp_ok) break;
+          if (g.f1 > g.f0) {
+            tmem_ld_32x32b_x32(tm + (uint32_t)(acc * BN + c * 32), v[0]);
+          } else {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[0][i] = 0.f;
-            }
-            const int ncol = min(32, g.cols - c_half - c * 32);
-            if (row_ok && ncol > 0) emit32(p, crow + (c_half + c * 32) * el, v[0], ncol);
-            __syncwarp();
+            for (int i = 0; i < 32; ++i) v[0][i] = 0.f;
           }
+          const int ncol = min(32, g.cols - c_half - c * 32);
+          if (row_ok && ncol > 0) {
+            if (p.split > 1) leave(c, v[0]);
+            else emit32(p, crow + (c_half + c * 32) * el, v[0], ncol);
+          }
+          __syncwarp();
         }
         if (g.f1 > g.f0) {
           release(acc);
@@ -675,7 +793,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
       }
 
       if (p.split == 1) {
-        if constexpr (KIND == kByte) {
+        if constexpr (Cf::kSums) {
 #pragma unroll
           for (int c = 0; c < Cf::kChunks; ++c) {
             const int ncol = min(32, g.cols - c_half - c * 32);
@@ -687,43 +805,15 @@ __global__ void __launch_bounds__(kThreadsG, 1)
         // The cluster's CTAs hold partial sums of one tile. Each leaves its
         // own in shared memory; CTA r then adds rows r, r + split, … of all
         // of them, in CTA order, and stores them.
-        auto cluster_wait = [&](uint64_t* bar, uint32_t par) {
-          int good = 1;
-          if (lane == 0) {
-            const uint32_t b = smem_addr(bar);
-            const long long t0 = clock64();
-            while (!mbar_try_wait_cluster(b, par)) {
-              if (*abort_flag) {
-                good = 0;
-                break;
-              }
-              if (clock64() - t0 > kWaitBudgetCycles) {
-                record_error(TB_ERR_DEVICE_TIMEOUT, kSiteCluster);
-                *abort_flag = 1;
-                good = 0;
-                break;
-              }
-            }
+        if constexpr (Cf::kSums) {
+          if (!cluster_wait(&bars.consumed, red_phase ^ 1u)) {
+            ok = false;
+            break;
           }
-          good = __shfl_sync(0xffffffffu, good, 0);
-          return good != 0;
-        };
-        auto cluster_arrive = [&](uint64_t* bar) {
-          __syncwarp();
-          if (lane < p.split) mbar_arrive_cluster(map_to_cta(smem_addr(bar), (uint32_t)lane));
-        };
-        // every CTA has read the previous tile's partial sums
-        if (!cluster_wait(&bars.consumed, red_phase ^ 1u)) {
-          ok = false;
-          break;
-        }
-        if (row_ok) {
+          if (row_ok) {
 #pragma unroll
-          for (int c = 0; c < Cf::kChunks; ++c) {
-            float4* dst = reinterpret_cast<float4*>(red + (size_t)row_in_tile * Cf::kRedStride + (c_half + c * 32) * 4);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              dst[i] = make_float4(v[c][4 * i], v[c][4 * i + 1], v[c][4 * i + 2], v[c][4 * i + 3]);
+            for (int c = 0; c < Cf::kChunks; ++c)
+              if (c_half + c * 32 < g.cols) leave(c, v[c]);
           }
         }
         cluster_arrive(&bars.ready);
@@ -928,6 +1018,15 @@ tbStatus launch(Launch& L, int sms, int dev, cudaStream_t stream) {
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// The kind of a tile's kernel, by the operands' and the output's types.
+template <int BN, int G>
+tbStatus launch_tile(Launch& L, int sms, int dev, cudaStream_t stream) {
+  if (L.el == 1)
+    return L.p.sb.shift ? launch<kByte, BN, G>(L, sms, dev, stream) : launch<kByteCol, BN, G>(L, sms, dev, stream);
+  return L.p.c_dtype == TB_F32 ? launch<kHalfSum, BN, G>(L, sms, dev, stream)
+                               : launch<kHalf, BN, G>(L, sms, dev, stream);
+}
+
 // Tile and K split. `rows`: mean rows of a group that has any.
 tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int dev, cudaStream_t stream) {
   GParams& p = L.p;
@@ -947,7 +1046,7 @@ tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int
   p.split = 1;
   if (m > 128 && 2 * tiles(256, 256) >= sms / 2) {
     set(256, 256);
-    return L.el == 1 ? launch<kByte, 256, 2>(L, sms, dev, stream) : launch<kHalf, 256, 2>(L, sms, dev, stream);
+    return launch_tile<256, 2>(L, sms, dev, stream);
   }
   // An 8-bit B stored along its columns comes in boxes of 128 columns.
   const bool wide = (L.el == 1 && !p.b_kmaj) || tiles(128, 128) >= sms;
@@ -955,9 +1054,7 @@ tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int
   const int64_t fills = cdiv(kmax, 128 / L.el);
   while (p.split < 8 && have * p.split * 2 <= sms && fills >= 4 * p.split) p.split *= 2;
   set(128, wide ? 128 : 64);
-  if (wide)
-    return L.el == 1 ? launch<kByte, 128, 1>(L, sms, dev, stream) : launch<kHalf, 128, 1>(L, sms, dev, stream);
-  return L.el == 1 ? launch<kByte, 64, 1>(L, sms, dev, stream) : launch<kHalf, 64, 1>(L, sms, dev, stream);
+  return wide ? launch_tile<128, 1>(L, sms, dev, stream) : launch_tile<64, 1>(L, sms, dev, stream);
 }
 
 int c_bytes(int32_t dt) { return dt == TB_F32 ? 4 : 2; }

@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
             if (leader) mbar_expect_tx(bar, G * bytes);
             if constexpr (G == 2) {
               bar = map_to_cta(bar, 0);
-              if (p.k_grouped && !leader) mbar_arrive_cluster(bar);
+              if (p.k_grouped && !leader) mbar_arrive_remote(bar);
             }
           }
           auto load2 = [&](uint32_t dst, const CUtensorMap* m, int32_t x, int32_t y) {
@@ -504,11 +504,11 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           // first and last fill of an accumulation
           const bool opens = Cf::kSums ? (f - g.f0) % Cf::kSegFills == 0 : f == g.f0;
           const bool closes = f + 1 == g.f1 || (Cf::kSums && (f + 1 - g.f0) % Cf::kSegFills == 0);
-          if (opens && !warp_wait(smem_addr(&bars.tempty[acc]), acc_phase ^ 1u, abort_flag, kSiteMma, lane)) {
+          if (opens && !warp_poll(smem_addr(&bars.tempty[acc]), acc_phase ^ 1u, abort_flag, kSiteMma, lane)) {
             ok = false;
             break;
           }
-          if (!warp_wait(smem_addr(&bars.full[stage]), phase, abort_flag, kSiteMma, lane)) {
+          if (!warp_poll(smem_addr(&bars.full[stage]), phase, abort_flag, kSiteMma, lane)) {
             ok = false;
             break;
           }
@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        if constexpr (G == 2) mbar_arrive_cluster(tempty0 + acc * 8);
+        if constexpr (G == 2) mbar_arrive_remote(tempty0 + acc * 8);
         else mbar_arrive(tempty0 + acc * 8);
       }
     };
@@ -711,7 +711,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
             __syncwarp();
           }
           if constexpr (Cf::kBytes) fetch(f + 1);
-          if (!warp_wait(smem_addr(&bars.tfull[acc]), acc_phase, abort_flag, kSiteEpilogue, lane)) {
+          if (!warp_poll(smem_addr(&bars.tfull[acc]), acc_phase, abort_flag, kSiteEpilogue, lane)) {
             ok = false;
             break;
           }
@@ -754,7 +754,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           for (int i = 0; i < 16; ++i) unpack_f32x2(sum[c][i], v[c][2 * i], v[c][2 * i + 1]);
       } else {
         if (g.f1 > g.f0) {
-          if (!warp_wait(smem_addr(&bars.tfull[acc]), acc_phase, abort_flag, kSiteEpilogue, lane)) {
+          if (!warp_poll(smem_addr(&bars.tfull[acc]), acc_phase, abort_flag, kSiteEpilogue, lane)) {
             ok = false;
             break;
           }

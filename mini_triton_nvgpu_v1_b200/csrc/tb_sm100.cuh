@@ -227,6 +227,15 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
                : "memory");
 }
 
+// The same arrival without the cluster-scope release: for a barrier that hands
+// over TMEM (ordered by tcgen05.wait / tcgen05.fence) or nothing but the
+// arrival itself. The release waits for the thread's outstanding memory
+// accesses; once per 128 elements of K it doubled the 8-bit product's time
+// (8192³: 829 → 438 µs, epilogue arithmetic left out on both sides).
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
 // ---------------------------------------------------------------- tcgen05
 template <int G>
 __device__ __forceinline__ void tmem_alloc_g(uint32_t dst_smem, uint32_t ncols) {

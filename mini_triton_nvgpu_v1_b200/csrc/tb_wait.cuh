@@ -51,4 +51,27 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
+// warp_wait without the blocking probe: the warp polls until the phase is
+// complete, for waits whose every cycle is on the critical path (a blocked
+// try_wait wakes up hundreds of cycles after the phase completes).
+__device__ __forceinline__ bool warp_poll(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                          uint32_t site, int lane) {
+  if (__all_sync(0xffffffffu, tb::sm100::mbar_test_wait(bar, parity))) return true;
+  const long long t0 = clock64();
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i)
+      if (__all_sync(0xffffffffu, tb::sm100::mbar_test_wait(bar, parity))) return true;
+    int stop = 0;
+    if (lane == 0) {
+      stop = *abort_flag;
+      if (!stop && clock64() - t0 > kWaitBudgetCycles) {
+        record_error(TB_ERR_DEVICE_TIMEOUT, site);
+        *abort_flag = stop = 1;
+      }
+    }
+    if (__shfl_sync(0xffffffffu, stop, 0)) return false;
+  }
+}
+
 }  // namespace

@@ -9,9 +9,11 @@
 //
 // HBM bound: el + 1 bytes per element and nothing read twice. A CTA takes a
 // 128 × 128 tile, which is whole blocks in all three shapes; a thread holds 8
-// columns of 8 rows in registers (all 8 loads in flight at once: 32 KB per
-// CTA of 16-bit inputs), the maxima meet through shuffles and, for blocks
-// that span rows, 4 KB of shared memory.
+// columns of 8 rows in registers as they were read, all 8 loads in flight at
+// once and 32 KB per CTA of 16-bit inputs. The maxima are taken on the bits of
+// |x| as unsigned integers (the order of the magnitudes, with NaN above
+// infinity, two 16-bit values to an instruction) and meet through shuffles
+// and, for blocks that span rows, shared memory.
 //
 // The quotient 448 X / m has to be rounded as the division rounds it: X and m
 // are often multiples of each other's last places, so quotients that lie on
@@ -25,8 +27,9 @@
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
-#include <algorithm>
+#include <cstring>
 #include <string>
+#include <type_traits>
 
 #include "tb_plan.h"
 
@@ -44,61 +47,79 @@ struct QParams {
   int32_t vec_x, vec_q;
 };
 
-__device__ __forceinline__ float max_nan(float a, float b) {  // a NaN stays
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+// Two f32 in a register pair.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
 
+// Eight values of a row as they are in memory: kWords words of kPer values.
 template <typename T>
-struct In;
-template <>
-struct In<float> {
-  static __device__ __forceinline__ float one(const float* p) { return __ldcs(p); }
-  static __device__ __forceinline__ void eight(const float* p, float (&v)[8]) {
-    const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  }
-};
-template <>
-struct In<__half> {
-  static __device__ __forceinline__ float one(const __half* p) {
-    return __half2float(__ushort_as_half(__ldcs(reinterpret_cast<const unsigned short*>(p))));
-  }
-  static __device__ __forceinline__ void eight(const __half* p, float (&v)[8]) {
-    const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+struct In {
+  static constexpr int kPer = 4 / (int)sizeof(T), kWords = 8 / kPer;
+  static __device__ __forceinline__ void eight(const T* p, uint32_t (&w)[kWords]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      __half2 h;
-      memcpy(&h, &w[i], 4);
-      const float2 f = __half22float2(h);
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
+    for (int i = 0; i < kWords / 4; ++i) {
+      const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+      w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
     }
   }
-};
-template <>
-struct In<__nv_bfloat16> {
-  static __device__ __forceinline__ float one(const __nv_bfloat16* p) {
-    return __uint_as_float((uint32_t)__ldcs(reinterpret_cast<const unsigned short*>(p)) << 16);
-  }
-  static __device__ __forceinline__ void eight(const __nv_bfloat16* p, float (&v)[8]) {
-    const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  static __device__ __forceinline__ void some(const T* p, int n, uint32_t (&w)[kWords]) {  // the first n, then zeros
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    for (int i = 0; i < kWords; ++i) {
+      w[i] = 0;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int k = i * kPer + j;
+        if (k < n) {
+          if constexpr (kPer == 1) w[i] = __ldcs(reinterpret_cast<const uint32_t*>(p) + k);
+          else w[i] |= (uint32_t)__ldcs(reinterpret_cast<const unsigned short*>(p) + k) << (16 * j);
+        }
+      }
+    }
+  }
+  static constexpr uint32_t kAbs = kPer == 1 ? 0x7fffffffu : 0x7fff7fffu;
+  static __device__ __forceinline__ uint32_t max3(uint32_t a, uint32_t b, uint32_t c) {
+    if constexpr (kPer == 1) return __vimax3_u32(a, b, c);
+    else return __vimax3_u16x2(a, b, c);
+  }
+  static __device__ __forceinline__ float value(uint32_t bits) {  // of the low 16 (or all 32) bits
+    if constexpr (kPer == 1) return __uint_as_float(bits);
+    else if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short)bits));
+    else return __uint_as_float(bits << 16);
+  }
+  // values 2k and 2k + 1
+  static __device__ __forceinline__ uint64_t pair(const uint32_t (&w)[kWords], int k) {
+    if constexpr (kPer == 1) {
+      return two(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1]));
+    } else if constexpr (std::is_same<T, __half>::value) {
+      __half2 h;
+      memcpy(&h, &w[k], 4);
+      const float2 f = __half22float2(h);
+      return two(f.x, f.y);
+    } else {
+      return two(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
     }
   }
 };
 
-// BR × BC: the block's extent, 1 × 128, 128 × 1 or 128 × 128.
+// BR × BC: the block's extent, 1 × 128, 128 × 1 or 128 × 128. 16-bit inputs:
+// at most 64 registers, so that four CTAs (128 KB of loads) are at work on an SM.
 template <typename T, int BR, int BC>
-__global__ void __launch_bounds__(256) tb_quantize_kernel(const QParams p) {
-  __shared__ float part[8][128];
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) tb_quantize_kernel(const QParams p) {
+  using I = In<T>;
+  constexpr int W = I::kWords;
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int64_t per = (int64_t)p.tiles_r * p.tiles_c;
   const int64_t b = blockIdx.x / per;
@@ -106,77 +127,103 @@ __global__ void __launch_bounds__(256) tb_quantize_kernel(const QParams p) {
   const int32_t tr = u / p.tiles_c, tc = u - tr * p.tiles_c;
   const int64_t r0 = (int64_t)tr * 128 + ty, c0 = (int64_t)tc * 128 + tx * 8;
   const int ncol = (int)min((int64_t)8, max((int64_t)0, p.cols - c0));
-  const T* x = static_cast<const T*>(p.x) + b * p.batch_x + c0;
+  const int nrow = (int)min((int64_t)8, max((int64_t)0, (p.rows - r0 + 15) / 16));  // this thread's rows
+  const T* x = static_cast<const T*>(p.x) + b * p.batch_x + r0 * p.ldx + c0;
 
-  float v[8][8];
+  uint32_t v[8][W];
+  if (p.vec_x && (int64_t)tr * 128 + 128 <= p.rows && (int64_t)tc * 128 + 128 <= p.cols) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t r = r0 + 16 * i;
-    if (r < p.rows && ncol == 8 && p.vec_x) {
-      In<T>::eight(x + r * p.ldx, v[i]);
-    } else {
+    for (int i = 0; i < 8; ++i) I::eight(x + 16 * i * p.ldx, v[i]);
+  } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = r < p.rows && j < ncol ? In<T>::one(x + r * p.ldx + j) : 0.f;
+    for (int i = 0; i < 8; ++i) {
+      const int n = i < nrow ? ncol : 0;
+      if (n == 8 && p.vec_x) I::eight(x + 16 * i * p.ldx, v[i]);
+      else I::some(x + 16 * i * p.ldx, n, v[i]);
     }
   }
 
-  // block maxima: of row i (BR = 1), of column j (BC = 1), or of all
-  float m[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m[i] = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float& d = m[BR == 1 ? i : j];
-      d = max_nan(d, fabsf(v[i][j]));
-    }
+  // block maxima: of row i (BR = 1), of column j (BC = 1), or one of all
+  constexpr int kMaxima = BR == 128 && BC == 128 ? 1 : 8;
+  float m[kMaxima];
   if constexpr (BR == 1) {
+    uint32_t a[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 8; ++i) {
+      a[i] = 0;
 #pragma unroll
-      for (int d = 8; d > 0; d /= 2) m[i] = max_nan(m[i], __shfl_xor_sync(0xffffffffu, m[i], d));
+      for (int j = 0; j < W; j += 2) a[i] = I::max3(a[i], v[i][j] & I::kAbs, v[i][j + 1] & I::kAbs);
+    }
+    if constexpr (I::kPer == 2) {
+      // rows i and i + 1 in one word
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        uint32_t q = __vimax3_u16x2(__byte_perm(a[i], a[i + 1], 0x5410), __byte_perm(a[i], a[i + 1], 0x7632), 0);
+#pragma unroll
+        for (int d = 8; d > 0; d /= 2) q = I::max3(q, __shfl_xor_sync(0xffffffffu, q, d), 0);
+        m[i] = I::value(q & 0xffffu);
+        m[i + 1] = I::value(q >> 16);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+#pragma unroll
+        for (int d = 8; d > 0; d /= 2) a[i] = I::max3(a[i], __shfl_xor_sync(0xffffffffu, a[i], d), 0);
+        m[i] = I::value(a[i]);
+      }
+    }
   } else {
+    __shared__ __align__(16) uint32_t part[8][16 * W];
+    uint32_t a[W];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m[j] = max_nan(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
+    for (int j = 0; j < W; ++j) {
+      a[j] = 0;
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) a[j] = I::max3(a[j], v[i][j] & I::kAbs, v[i + 1][j] & I::kAbs);
+      a[j] = I::max3(a[j], __shfl_xor_sync(0xffffffffu, a[j], 16), 0);
+    }
     if constexpr (BC == 128) {
 #pragma unroll
-      for (int j = 1; j < 8; ++j) m[0] = max_nan(m[0], m[j]);
-#pragma unroll
-      for (int d = 8; d > 0; d /= 2) m[0] = max_nan(m[0], __shfl_xor_sync(0xffffffffu, m[0], d));
-      if (lane == 0) part[warp][0] = m[0];
+      for (int j = 1; j < W; ++j) a[0] = I::max3(a[0], a[j], 0);
+      if constexpr (I::kPer == 2) a[0] = max(a[0] & 0xffffu, a[0] >> 16);
+      a[0] = __reduce_max_sync(0xffffffffu, a[0]);
+      if (lane == 0) part[warp][0] = a[0];
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < 8; ++w) m[0] = max_nan(m[0], part[w][0]);
+      for (int w = 0; w < 8; ++w) a[0] = max(a[0], part[w][0]);
+      m[0] = I::value(a[0]);
     } else {
       if (lane < 16) {
 #pragma unroll
-        for (int j = 0; j < 8; j += 4)
-          *reinterpret_cast<float4*>(&part[warp][tx * 8 + j]) = make_float4(m[j], m[j + 1], m[j + 2], m[j + 3]);
+        for (int j = 0; j < W; j += 4)
+          *reinterpret_cast<uint4*>(&part[warp][tx * W + j]) = make_uint4(a[j], a[j + 1], a[j + 2], a[j + 3]);
       }
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < 8; ++w)
+      for (int w = 0; w < 8; w += 2)
 #pragma unroll
-        for (int j = 0; j < 8; j += 4) {
-          const float4 f = *reinterpret_cast<const float4*>(&part[w][tx * 8 + j]);
-          m[j] = max_nan(m[j], f.x);
-          m[j + 1] = max_nan(m[j + 1], f.y);
-          m[j + 2] = max_nan(m[j + 2], f.z);
-          m[j + 3] = max_nan(m[j + 3], f.w);
+        for (int j = 0; j < W; j += 4) {
+          const uint4 f = *reinterpret_cast<const uint4*>(&part[w][tx * W + j]);
+          const uint4 g = *reinterpret_cast<const uint4*>(&part[w + 1][tx * W + j]);
+          a[j] = I::max3(a[j], f.x, g.x);
+          a[j + 1] = I::max3(a[j + 1], f.y, g.y);
+          a[j + 2] = I::max3(a[j + 2], f.z, g.z);
+          a[j + 3] = I::max3(a[j + 3], f.w, g.w);
         }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        m[j] = I::kPer == 1 ? I::value(a[j / I::kPer]) : I::value(j % 2 ? a[j / I::kPer] >> 16 : a[j / I::kPer] & 0xffffu);
     }
   }
-  constexpr int kMaxima = BR == 128 && BC == 128 ? 1 : 8;
 #pragma unroll
-  for (int i = 0; i < kMaxima; ++i) m[i] = max_nan(m[i], kLeastMax);
+  for (int i = 0; i < kMaxima; ++i) m[i] = m[i] < kLeastMax ? kLeastMax : m[i];  // a NaN stays
 
   float* s = p.s + b * p.batch_s;
   if constexpr (BR == 1) {
     if (tx == 0) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (r0 + 16 * i < p.rows) s[(r0 + 16 * i) * p.s_row + (int64_t)tc * p.s_col] = m[i] / 448.f;
+        if (i < nrow) s[(r0 + 16 * i) * p.s_row + (int64_t)tc * p.s_col] = m[i] / 448.f;
     }
   } else if constexpr (BC == 1) {
     if (ty == 0) {
@@ -188,43 +235,43 @@ __global__ void __launch_bounds__(256) tb_quantize_kernel(const QParams p) {
     if (threadIdx.x == 0) s[(int64_t)tr * p.s_row + (int64_t)tc * p.s_col] = m[0] / 448.f;
   }
 
-  float rcp[kMaxima], den[kMaxima];
+  // per maximum: 1 / d and -d of d = m / 1024
+  float rcp[kMaxima], neg[kMaxima];
 #pragma unroll
   for (int i = 0; i < kMaxima; ++i) {
-    const float d = m[i] * 0.0009765625f;  // m / 1024
+    const float d = m[i] * 0.0009765625f;
     rcp[i] = __frcp_rn(d);
-    den[i] = isinf(d) ? 0.f : d;         // an infinite block: 0, and NaN for the infinities (as X / m)
+    neg[i] = isinf(d) ? 0.f : -d;  // an infinite block: 0, and NaN for the infinities (as X / m)
   }
-  uint8_t* q = p.q + b * p.batch_q + c0;
+  uint8_t* q = p.q + b * p.batch_q + r0 * p.ldq + c0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int64_t r = r0 + 16 * i;
-    uint32_t w[2];
+    uint32_t o[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      uint32_t two[2];
+      uint32_t e[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
+        const int c = 2 * h + k;  // columns 2c and 2c + 1
+        const int g0 = kMaxima == 1 ? 0 : BR == 1 ? i : 2 * c, g1 = kMaxima == 1 ? 0 : BR == 1 ? i : 2 * c + 1;
+        const uint64_t r2 = two(rcp[g0], rcp[g1]), n2 = two(neg[g0], neg[g1]);
+        const uint64_t y = mul2(I::pair(v[i], c), two(0.4375f, 0.4375f));
+        const uint64_t t = mul2(y, r2);
+        const uint64_t z = fma2(fma2(t, n2, y), r2, t);
         float2 f;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int j = 4 * h + 2 * k + e;
-          const int g = kMaxima == 1 ? 0 : BR == 1 ? i : j;
-          const float y = v[i][j] * 0.4375f;
-          const float t = y * rcp[g];
-          (e ? f.y : f.x) = fmaf(fmaf(-t, den[g], y), rcp[g], t);
-        }
-        two[k] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(z));
+        e[k] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
       }
-      w[h] = two[0] | (two[1] << 16);
+      o[h] = __byte_perm(e[0], e[1], 0x5410);
     }
-    if (r >= p.rows) continue;
+    if (i >= nrow) break;
+    uint8_t* row = q + 16 * i * p.ldq;
     if (ncol == 8 && p.vec_q) {
-      *reinterpret_cast<uint2*>(q + r * p.ldq) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint2*>(row) = make_uint2(o[0], o[1]);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (j < ncol) q[r * p.ldq + j] = (uint8_t)(w[j / 4] >> (8 * (j % 4)));
+        if (j < ncol) row[j] = (uint8_t)(o[j / 4] >> (8 * (j % 4)));
     }
   }
 }

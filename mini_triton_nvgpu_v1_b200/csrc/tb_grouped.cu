@@ -12,8 +12,9 @@
 // router's output), so no call waits for the host to learn them:
 // every CTA builds the table of tiles from the offsets when it starts.
 //
-//   warp 0      TMA producer           warp 2   row fixer (K grouped)
-//   warp 1      MMA issuer             warps 4-11  epilogue, two per lane quarter
+//   warp 0   TMA producer              warp 3      scheduler: the next tiles, worked out
+//   warp 1   MMA issuer                            once and handed over in shared memory
+//   warp 2   row fixer (K grouped)     warps 4-11  epilogue, two per lane quarter
 //
 // Rows grouped: a tile's rows begin at any row of A (a TMA coordinate other
 // than the innermost has no alignment rule); the rows past the group's end
@@ -104,10 +105,23 @@ struct GroupTable {
   int32_t cum[kMaxGroups + 1];  // rows grouped: tiles before group e
 };
 
+struct GTile {
+  int32_t e;         // group
+  int32_t row0;      // first row of A and C (rows grouped) or of G[e] (K grouped)
+  int32_t rows, n0, cols;
+  int32_t k0, k_end; // K range of the tile
+  int32_t f0, f1;    // this CTA's ring fills of it
+};
+
+constexpr int kTileSlots = 4;
+
 struct GBars {
   uint64_t full[kMaxStages], empty[kMaxStages], fix[kMaxStages];
   uint64_t tfull[2], tempty[2];
   uint64_t drain, ready, consumed;
+  // tiles that the scheduler warp has worked out for the other roles
+  uint64_t tile_full[kTileSlots], tile_empty[kTileSlots];
+  GTile tile[kTileSlots];
   alignas(16) float col_scale[8][128];  // per epilogue warp: SB of its columns in the block at hand
   uint32_t tmem_holder;
   int abort_flag;
@@ -146,14 +160,6 @@ __device__ __forceinline__ int32_t read_offset(const GParams& p, int32_t i) {
   else v = static_cast<const int32_t*>(p.offsets)[i];
   return (int32_t)(v < 0 ? 0 : v > rows ? rows : v);
 }
-
-struct GTile {
-  int32_t e;         // group
-  int32_t row0;      // first row of A and C (rows grouped) or of G[e] (K grouped)
-  int32_t rows, n0, cols;
-  int32_t k0, k_end; // K range of the tile
-  int32_t f0, f1;    // this CTA's ring fills of it
-};
 
 // Tile t. Inside a group, tiles go in bands of 8 tile rows, rows fastest:
 // the CTAs at work share few panels of A and B.
@@ -358,6 +364,11 @@ __global__ void __launch_bounds__(kThreadsG, 1)
       mbar_init(smem_addr(&bars.tfull[a]), 1);
       mbar_init(smem_addr(&bars.tempty[a]), 8 * G);
     }
+    for (int i = 0; i < kTileSlots; ++i) {
+      mbar_init(smem_addr(&bars.tile_full[i]), 1);
+      // producer, epilogue warps, and those of MMA issuer and fixer that are at work
+      mbar_init(smem_addr(&bars.tile_empty[i]), 9 + (leader ? 1 : 0) + (p.k_grouped ? 1 : 0));
+    }
     mbar_init(smem_addr(&bars.drain), 1);
     mbar_init(smem_addr(&bars.ready), 8 * p.split);
     mbar_init(smem_addr(&bars.consumed), 8 * p.split);
@@ -397,20 +408,40 @@ __global__ void __launch_bounds__(kThreadsG, 1)
   const uint32_t tmem_base = bars.tmem_holder;
   const int32_t tiles = p.k_grouped ? p.groups * p.tiles_m * p.tiles_n : tab.cum[p.groups];
 
+  // The tiles in turn: take() waits for the next one, done() gives its slot back.
+  int slot = 0;
+  uint32_t slot_phase = 0;
+  auto take = [&](uint32_t site) {
+    return warp_poll(smem_addr(&bars.tile_full[slot]), slot_phase, abort_flag, site, lane);
+  };
+  auto done = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_addr(&bars.tile_empty[slot]));
+    if (++slot == kTileSlots) {
+      slot = 0;
+      slot_phase ^= 1u;
+    }
+  };
+  // One read of a field of the tile at hand (not kept in a register).
+  auto field = [&](int32_t GTile::*m) {
+    return *const_cast<const volatile int32_t*>(&(bars.tile[slot].*m));
+  };
+
   // Sums in registers, 256 columns: 128 per epilogue thread. 256 threads ×
-  // 216 + 128 × 72 registers = the launch's 384 × 168.
+  // 224 + 128 × 56 registers = the launch's 384 × 168.
   constexpr bool kMoveRegs = Cf::kSums && BN == 256;
   if (warp < 4) {
-  if constexpr (kMoveRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  if constexpr (kMoveRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     int stage = 0;
     uint32_t phase = 0;
-    long long issued = 0;
-    int32_t cursor = 0;
+    uint32_t issued = 0;
     bool ok = true;
     for (int32_t t = first; t < tiles && ok; t += stride) {
-      const GTile g = tile_at<Cf::kBM, BN, Cf::kKB>(p, tab, t, part, cursor);
+      if (!take(kSiteProducer)) break;
+      const GTile g = bars.tile[slot];
+      done();
       // K-major A of a short tile: only the 32-row boxes that hold its rows
       const int boxes = G == 1 && !p.a_mn ? (min(g.rows, 128) + 31) / 32 : 4;
       const uint32_t bytes = (boxes < 4 ? (uint32_t)boxes * 4096u : Cf::kABytes) + Cf::kBBytes;
@@ -474,10 +505,10 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     }
     if (lane == 0 && leader) {
       // The newest fill of each stage must land before the CTAs exit.
-      const long long last = issued < S ? issued : S;
-      for (long long i = 0; i < last; ++i) {
-        const long long f = issued - 1 - i;
-        const uint32_t par = (uint32_t)((f / S) & 1);
+      const uint32_t last = min(issued, (uint32_t)S);
+      for (uint32_t i = 0; i < last; ++i) {
+        const uint32_t f = issued - 1 - i;
+        const uint32_t par = (f / S) & 1;
         const long long t0 = clock64();
         while (!mbar_try_wait(smem_addr(&bars.full[f % S]), par)) {
           if (clock64() - t0 > kWaitBudgetCycles) {
@@ -496,14 +527,21 @@ __global__ void __launch_bounds__(kThreadsG, 1)
       const uint32_t a_lbo = p.a_mn ? Cf::kMnBoxBytes : 16u, b_lbo = p.b_kmaj ? 16u : Cf::kMnBoxBytes;
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
-      int32_t cursor = 0;
       bool issued_any = false, ok = true;
       for (int32_t t = first; t < tiles && ok; t += stride) {
-        const GTile g = tile_at<Cf::kBM, BN, Cf::kKB>(p, tab, t, part, cursor);
-        for (int32_t f = g.f0; f < g.f1; ++f) {
+        if (!take(kSiteMma)) {
+          ok = false;
+          break;
+        }
+        // this tile's fills, and the MMA steps of the last one
+        const int32_t fills = field(&GTile::f1) - field(&GTile::f0);
+        const int32_t last_valid = min(Cf::kKB, field(&GTile::k_end) - field(&GTile::k0) - (field(&GTile::f1) - 1) * Cf::kKB);
+        const int last_steps = (last_valid + Cf::kMmaK - 1) / Cf::kMmaK;
+        done();
+        for (int32_t f = 0; f < fills; ++f) {
           // first and last fill of an accumulation
-          const bool opens = Cf::kSums ? (f - g.f0) % Cf::kSegFills == 0 : f == g.f0;
-          const bool closes = f + 1 == g.f1 || (Cf::kSums && (f + 1 - g.f0) % Cf::kSegFills == 0);
+          const bool opens = Cf::kSums ? f % Cf::kSegFills == 0 : f == 0;
+          const bool closes = f + 1 == fills || (Cf::kSums && (f + 1) % Cf::kSegFills == 0);
           if (opens && !warp_poll(smem_addr(&bars.tempty[acc]), acc_phase ^ 1u, abort_flag, kSiteMma, lane)) {
             ok = false;
             break;
@@ -513,8 +551,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
             break;
           }
           tc_fence_after();
-          const int32_t valid = min(Cf::kKB, g.k_end - (g.k0 + f * Cf::kKB));
-          const int steps = (valid + Cf::kMmaK - 1) / Cf::kMmaK;
+          const int steps = f + 1 == fills ? last_steps : 4;
           const uint64_t da0 = smem_desc_sw128(smem_addr(sA + (size_t)stage * Cf::kABytes), a_lbo, 1024);
           const uint64_t db0 = smem_desc_sw128(smem_addr(sB + (size_t)stage * Cf::kBBytes), b_lbo, 1024);
           const uint32_t d = tmem_base + (uint32_t)(acc * BN);
@@ -568,20 +605,18 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     if (p.k_grouped) {
       int stage = 0;
       uint32_t fix_phase = 0;  // bit s: parity of stage s's next fix
-      int32_t cursor = 0;
-      bool ok = true;
-      for (int32_t t = first; t < tiles && ok; t += stride) {
-        const GTile g = tile_at<Cf::kBM, BN, Cf::kKB>(p, tab, t, part, cursor);
+      for (int32_t t = first; t < tiles; t += stride) {
+        if (!take(kSiteFixer)) break;
+        const GTile g = bars.tile[slot];
+        done();
         const int32_t n = g.f1 - g.f0;
         if (n <= 0) continue;
         const int32_t last = (stage + n - 1) % S;  // only a tile's last fill can be short
         const int32_t valid = min(Cf::kKB, g.k_end - (g.k0 + (g.f1 - 1) * Cf::kKB));
         stage = (stage + n) % S;
         if (valid % Cf::kMmaK == 0) continue;
-        if (!warp_wait(smem_addr(&bars.fix[last]), (fix_phase >> last) & 1u, abort_flag, kSiteFixer, lane)) {
-          ok = false;
+        if (!warp_wait(smem_addr(&bars.fix[last]), (fix_phase >> last) & 1u, abort_flag, kSiteFixer, lane))
           break;
-        }
         fix_phase ^= 1u << last;
         // K rows [valid, next multiple of the K step) of every box of both
         // operands: 128 bytes per row (the swizzle stays inside a row)
@@ -603,9 +638,24 @@ __global__ void __launch_bounds__(kThreadsG, 1)
         }
       }
     }
+  } else {
+    // ----------------------------------------------------------- scheduler
+    int32_t cursor = 0;
+    for (int32_t t = first; t < tiles; t += stride) {
+      if (!warp_wait(smem_addr(&bars.tile_empty[slot]), slot_phase ^ 1u, abort_flag, kSiteScheduler, lane)) break;
+      const GTile g = tile_at<Cf::kBM, BN, Cf::kKB>(p, tab, t, part, cursor);
+      if (lane == 0) {
+        bars.tile[slot] = g;
+        mbar_arrive(smem_addr(&bars.tile_full[slot]));
+      }
+      if (++slot == kTileSlots) {
+        slot = 0;
+        slot_phase ^= 1u;
+      }
+    }
   }
   } else {
-    if constexpr (kMoveRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if constexpr (kMoveRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     // ------------------------------------------------------------ epilogue
     const int q = warp & 3;               // TMEM lane quarter
     const int half = (warp - 4) >> 2;     // column half
@@ -653,16 +703,21 @@ __global__ void __launch_bounds__(kThreadsG, 1)
 #pragma unroll
       for (int i = 0; i < 8; ++i) dst[i] = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
     };
+    // the tile at hand in C, and this thread's row and column half of it
+    auto tile_at_c = [&]() {
+      const int64_t group = p.k_grouped ? (int64_t)field(&GTile::e) * p.group_c : 0;
+      return static_cast<char*>(p.C) + (group + (int64_t)field(&GTile::row0) * p.ldc + field(&GTile::n0)) * el;
+    };
+    auto row_at = [&]() { return tile_at_c() + ((int64_t)row_in_tile * p.ldc + c_half) * el; };
     int acc = 0;
     uint32_t acc_phase = 0, red_phase = 0;
-    int32_t cursor = 0;
     bool ok = true;
     for (int32_t t = first; t < tiles && ok; t += stride) {
-      const GTile g = tile_at<Cf::kBM, BN, Cf::kKB>(p, tab, t, part, cursor);
-      const bool row_ok = row_in_tile < g.rows;
-      const bool warp_ok = (int)rank * 128 + q * 32 < g.rows && c_half < g.cols;
-      char* crow = static_cast<char*>(p.C) +
-                   ((p.k_grouped ? (int64_t)g.e * p.group_c : 0) + ((int64_t)g.row0 + row_in_tile) * p.ldc + g.n0) * el;
+      if (!take(kSiteEpilogue)) break;
+      // Only the count of accumulations and the scales' places stay in
+      // registers during the sums; the rest is read again for the stores.
+      const int32_t fills = field(&GTile::f1) - field(&GTile::f0);
+      const bool warp_ok = (int)rank * 128 + q * 32 < field(&GTile::rows) && c_half < field(&GTile::cols);
       float v[Cf::kSums ? Cf::kChunks : 1][32];
 
       if constexpr (Cf::kSums) {
@@ -674,34 +729,37 @@ __global__ void __launch_bounds__(kThreadsG, 1)
         for (int c = 0; c < Cf::kChunks; ++c)
 #pragma unroll
           for (int i = 0; i < 16; ++i) sum[c][i] = 0;
+        // Scales of the next block: this row's, and the columns' (one, or this
+        // lane's of the warp's columns); fetched a block ahead.
         const float *sa = nullptr, *sb = nullptr;
         int64_t sb_col[4] = {0, 0, 0, 0};
         float xa = 1.f, xb = 1.f, xc[4] = {0.f, 0.f, 0.f, 0.f};
-        // scales of block f: this row's, and the columns' (one, or this
-        // lane's of the warp's columns); fetched a block ahead
-        auto fetch = [&](int32_t f) {
-          if (f >= g.f1) return;
-          xa = __ldg(sa + (int64_t)f * p.sa.sk);
-          if constexpr (KIND == kByte) xb = __ldg(sb + (int64_t)f * p.sb.sk);
+        auto fetch = [&]() {
+          xa = __ldg(sa);
+          sa += p.sa.sk;
+          if constexpr (KIND == kByte) xb = __ldg(sb);
           if constexpr (KIND == kByteCol) {
 #pragma unroll
-            for (int j = 0; j < Cf::kHalfCols / 32; ++j) xc[j] = __ldg(sb + sb_col[j] + (int64_t)f * p.sb.sk);
+            for (int j = 0; j < Cf::kHalfCols / 32; ++j) xc[j] = __ldg(sb + sb_col[j]);
           }
+          sb += p.sb.sk;
         };
         if constexpr (Cf::kBytes) {
-          const int32_t arow = min(g.row0 + row_in_tile, p.M - 1);  // masked rows read some valid scale
-          sa = p.sa.p + (int64_t)(arow >> p.sa.shift) * p.sa.smn;
-          sb = p.sb.p + (int64_t)g.e * p.sb.sg;
+          const int32_t f0 = field(&GTile::f0);
+          const int32_t arow = min(field(&GTile::row0) + row_in_tile, p.M - 1);  // masked rows read some valid scale
+          const int32_t col0 = field(&GTile::n0) + c_half;
+          sa = p.sa.p + (int64_t)(arow >> p.sa.shift) * p.sa.smn + (int64_t)f0 * p.sa.sk;
+          sb = p.sb.p + (int64_t)field(&GTile::e) * p.sb.sg + (int64_t)f0 * p.sb.sk;
           if constexpr (KIND == kByte) {
-            sb += (int64_t)(min(g.n0 + c_half, p.N - 1) >> 7) * p.sb.smn;
+            sb += (int64_t)(min(col0, p.N - 1) >> 7) * p.sb.smn;
           } else {
 #pragma unroll
             for (int j = 0; j < Cf::kHalfCols / 32; ++j)
-              sb_col[j] = (int64_t)min(g.n0 + c_half + 32 * j + lane, p.N - 1) * p.sb.smn;
+              sb_col[j] = (int64_t)min(col0 + 32 * j + lane, p.N - 1) * p.sb.smn;
           }
-          fetch(g.f0);
+          if (fills > 0) fetch();
         }
-        for (int32_t f = g.f0; f < g.f1; f += Cf::kSegFills) {
+        for (int32_t left = fills; left > 0; left -= Cf::kSegFills) {
           const float x = xa * xb;
           float* cs = bars.col_scale[warp - 4];
           if constexpr (KIND == kByteCol) {
@@ -710,7 +768,9 @@ __global__ void __launch_bounds__(kThreadsG, 1)
             for (int j = 0; j < Cf::kHalfCols / 32; ++j) cs[32 * j + lane] = xc[j];
             __syncwarp();
           }
-          if constexpr (Cf::kBytes) fetch(f + 1);
+          if constexpr (Cf::kBytes) {
+            if (left > 1) fetch();
+          }
           if (!warp_poll(smem_addr(&bars.tfull[acc]), acc_phase, abort_flag, kSiteEpilogue, lane)) {
             ok = false;
             break;
@@ -753,13 +813,16 @@ __global__ void __launch_bounds__(kThreadsG, 1)
 #pragma unroll
           for (int i = 0; i < 16; ++i) unpack_f32x2(sum[c][i], v[c][2 * i], v[c][2 * i + 1]);
       } else {
-        if (g.f1 > g.f0) {
+        if (fills > 0) {
           if (!warp_poll(smem_addr(&bars.tfull[acc]), acc_phase, abort_flag, kSiteEpilogue, lane)) {
             ok = false;
             break;
           }
           tc_fence_after();
         }
+        const bool row_ok = row_in_tile < field(&GTile::rows);
+        const int32_t cols = field(&GTile::cols) - c_half;
+        char* row = row_at();
         if (p.split > 1) {
           // every CTA has read the previous tile's partial sums
           if (!cluster_wait(&bars.consumed, red_phase ^ 1u)) {
@@ -770,20 +833,20 @@ __global__ void __launch_bounds__(kThreadsG, 1)
 #pragma unroll
         for (int c = 0; c < Cf::kChunks; ++c) {
           if (!warp_ok) break;
-          if (g.f1 > g.f0) {
+          if (fills > 0) {
             tmem_ld_32x32b_x32(tm + (uint32_t)(acc * BN + c * 32), v[0]);
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[0][i] = 0.f;
           }
-          const int ncol = min(32, g.cols - c_half - c * 32);
+          const int ncol = min(32, cols - c * 32);
           if (row_ok && ncol > 0) {
             if (p.split > 1) leave(c, v[0]);
-            else emit32(p, crow + (c_half + c * 32) * el, v[0], ncol);
+            else emit32(p, row + c * 32 * el, v[0], ncol);
           }
           __syncwarp();
         }
-        if (g.f1 > g.f0) {
+        if (fills > 0) {
           release(acc);
           if (++acc == 2) {
             acc = 0;
@@ -794,10 +857,13 @@ __global__ void __launch_bounds__(kThreadsG, 1)
 
       if (p.split == 1) {
         if constexpr (Cf::kSums) {
+          const bool row_ok = row_in_tile < field(&GTile::rows);
+          const int32_t cols = field(&GTile::cols) - c_half;
+          char* row = row_at();
 #pragma unroll
           for (int c = 0; c < Cf::kChunks; ++c) {
-            const int ncol = min(32, g.cols - c_half - c * 32);
-            if (row_ok && ncol > 0) emit32(p, crow + (c_half + c * 32) * el, v[c], ncol);
+            const int ncol = min(32, cols - c * 32);
+            if (row_ok && ncol > 0) emit32(p, row + c * 32 * el, v[c], ncol);
           }
           __syncwarp();
         }
@@ -810,10 +876,11 @@ __global__ void __launch_bounds__(kThreadsG, 1)
             ok = false;
             break;
           }
-          if (row_ok) {
+          if (row_in_tile < field(&GTile::rows)) {
+            const int32_t cols = field(&GTile::cols) - c_half;
 #pragma unroll
             for (int c = 0; c < Cf::kChunks; ++c)
-              if (c_half + c * 32 < g.cols) leave(c, v[c]);
+              if (c * 32 < cols) leave(c, v[c]);
           }
         }
         cluster_arrive(&bars.ready);
@@ -822,7 +889,8 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           break;
         }
         constexpr int kLaneCols = BN / 32;
-        const int rows = min(g.rows, 128);
+        const int rows = field(&GTile::rows), cols = field(&GTile::cols);
+        char* tile = tile_at_c();
         for (int r = part + p.split * (warp - 4); r < rows; r += p.split * 8) {
           const uint32_t src = smem_addr(red) + (uint32_t)r * Cf::kRedStride + (uint32_t)lane * kLaneCols * 4;
           float s[kLaneCols];
@@ -839,15 +907,15 @@ __global__ void __launch_bounds__(kThreadsG, 1)
             }
           }
           const int c0 = lane * kLaneCols;
-          char* dst = static_cast<char*>(p.C) +
-                      ((p.k_grouped ? (int64_t)g.e * p.group_c : 0) + ((int64_t)g.row0 + r) * p.ldc + g.n0 + c0) * el;
+          char* dst = tile + ((int64_t)r * p.ldc + c0) * el;
 #pragma unroll
           for (int i = 0; i < kLaneCols; ++i)
-            if (c0 + i < g.cols) store_out(p, dst + i * el, p.beta ? s[i] + load_out(p, dst + i * el) : s[i]);
+            if (c0 + i < cols) store_out(p, dst + i * el, p.beta ? s[i] + load_out(p, dst + i * el) : s[i]);
         }
         cluster_arrive(&bars.consumed);
         red_phase ^= 1u;
       }
+      done();
     }
   }
 

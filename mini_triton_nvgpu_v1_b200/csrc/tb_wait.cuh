@@ -15,7 +15,7 @@ namespace {
 constexpr long long kWaitBudgetCycles = 2000000000LL;  // ≈1 s at 1.9 GHz
 
 constexpr uint32_t kSiteProducer = 1, kSiteMma = 2, kSiteEpilogue = 3, kSiteDrain = 4,
-                   kSiteSelfTest = 5, kSiteFixer = 6, kSiteCluster = 7;
+                   kSiteSelfTest = 5, kSiteFixer = 6, kSiteCluster = 7, kSiteScheduler = 8;
 
 __device__ __forceinline__ void record_error(uint32_t code, uint32_t site) {
   const uint32_t v = (code << 24) | (site << 16) | (blockIdx.x & 0xFFFFu);

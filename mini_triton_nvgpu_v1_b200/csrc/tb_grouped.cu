@@ -353,34 +353,37 @@ __global__ void __launch_bounds__(kThreadsG, 1)
   const bool leader = rank == 0;
   const int32_t first = blockIdx.x / cluster, stride = gridDim.x / cluster;
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < S; ++s) {
-      // K grouped pairs: both producers (or fixers) arrive for each fill
-      mbar_init(smem_addr(&bars.full[s]), p.k_grouped ? G : 1);
-      mbar_init(smem_addr(&bars.empty[s]), 1);
-      mbar_init(smem_addr(&bars.fix[s]), 1);
-    }
-    for (int a = 0; a < 2; ++a) {
-      mbar_init(smem_addr(&bars.tfull[a]), 1);
-      mbar_init(smem_addr(&bars.tempty[a]), 8 * G);
-    }
-    for (int i = 0; i < kTileSlots; ++i) {
-      mbar_init(smem_addr(&bars.tile_full[i]), 1);
-      // producer, epilogue warps, and those of MMA issuer and fixer that are at work
-      mbar_init(smem_addr(&bars.tile_empty[i]), 9 + (leader ? 1 : 0) + (p.k_grouped ? 1 : 0));
-    }
-    mbar_init(smem_addr(&bars.drain), 1);
-    mbar_init(smem_addr(&bars.ready), 8 * p.split);
-    mbar_init(smem_addr(&bars.consumed), 8 * p.split);
-    bars.abort_flag = 0;
+  if (warp == 0) {
+    // one barrier to a lane
+    auto init = [&](uint64_t* bar, int n, uint32_t count) {
+      if (lane < n) mbar_init(smem_addr(bar + lane), count);
+    };
+    init(bars.full, S, p.k_grouped ? G : 1);  // K grouped pairs: both producers (or fixers) arrive for each fill
+    init(bars.empty, S, 1);
+    init(bars.fix, S, 1);
+    init(bars.tfull, 2, 1);
+    init(bars.tempty, 2, 8 * G);
+    init(bars.tile_full, kTileSlots, 1);
+    // producer, epilogue warps, and those of MMA issuer and fixer that are at work
+    init(bars.tile_empty, kTileSlots, 9 + (leader ? 1 : 0) + (p.k_grouped ? 1 : 0));
+    init(&bars.drain, 1, 1);
+    init(&bars.ready, 1, 8 * p.split);
+    init(&bars.consumed, 1, 8 * p.split);
+    if (lane == 0) bars.abort_flag = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&tmA);
-    tma_prefetch_desc(&tmB);
+    if (lane == 0) {
+      tma_prefetch_desc(&tmA);
+      tma_prefetch_desc(&tmA32);
+      tma_prefetch_desc(&tmB);
+    }
   }
   if (warp == 1) {
     tmem_alloc_g<G>(smem_addr(&bars.tmem_holder), Cf::kTmemCols);
     tmem_relinquish_g<G>();
   }
+  // What this launch reads may be written by the kernel before it in the
+  // stream, which it does not wait for until here (programmatic launch).
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int32_t e = threadIdx.x; e < p.groups; e += kThreadsG) {
     const int32_t s = read_offset(p, e), n = max(0, read_offset(p, e + 1) - s);
     tab.start[e] = s;
@@ -405,6 +408,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
   if (cluster > 1) cluster_sync();
   __syncthreads();
   tc_fence_after();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem_base = bars.tmem_holder;
   const int32_t tiles = p.k_grouped ? p.groups * p.tiles_m * p.tiles_n : tab.cum[p.groups];
 
@@ -448,7 +452,8 @@ __global__ void __launch_bounds__(kThreadsG, 1)
       const int32_t bn = g.n0 + (int32_t)rank * Cf::kBnCta;
       const int32_t be = p.k_grouped ? 0 : g.e;
       for (int32_t f = g.f0; f < g.f1; ++f) {
-        if (!warp_wait(smem_addr(&bars.empty[stage]), phase ^ 1u, abort_flag, kSiteProducer, lane)) {
+        if (issued >= (uint32_t)S &&
+            !warp_wait(smem_addr(&bars.empty[stage]), phase ^ 1u, abort_flag, kSiteProducer, lane)) {
           ok = false;
           break;
         }
@@ -523,8 +528,17 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     if (leader) {
       const uint32_t idesc = idesc_f16_f32(Cf::kBM, BN, p.a_mn ? 1 : 0, p.b_kmaj ? 0 : 1) | (p.fmt << 7) |
                              (p.fmt << 10);
-      const uint32_t a_step = p.a_mn ? Cf::kMnStep : 32u, b_step = p.b_kmaj ? 32u : Cf::kMnStep;
-      const uint32_t a_lbo = p.a_mn ? Cf::kMnBoxBytes : 16u, b_lbo = p.b_kmaj ? 16u : Cf::kMnBoxBytes;
+      // descriptor words: the start address (16-byte units) moves in the low one
+      const uint32_t a_step = (p.a_mn ? Cf::kMnStep : 32u) >> 4, b_step = (p.b_kmaj ? 32u : Cf::kMnStep) >> 4;
+      const uint64_t da = smem_desc_sw128(smem_addr(sA), p.a_mn ? Cf::kMnBoxBytes : 16u, 1024);
+      const uint64_t db = smem_desc_sw128(smem_addr(sB), p.b_kmaj ? 16u : Cf::kMnBoxBytes, 1024);
+      const uint32_t a_hi = (uint32_t)(da >> 32), b_hi = (uint32_t)(db >> 32);
+      const uint32_t full0 = smem_addr(&bars.full[0]), empty0 = smem_addr(&bars.empty[0]),
+                     tfull0 = smem_addr(&bars.tfull[0]), tempty0 = smem_addr(&bars.tempty[0]);
+      auto commit = [&](uint32_t bar) {
+        if constexpr (G == 2) umma_commit_pair(bar, 0x3);
+        else umma_commit(bar);
+      };
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool issued_any = false, ok = true;
@@ -538,51 +552,46 @@ __global__ void __launch_bounds__(kThreadsG, 1)
         const int32_t last_valid = min(Cf::kKB, field(&GTile::k_end) - field(&GTile::k0) - (field(&GTile::f1) - 1) * Cf::kKB);
         const int last_steps = (last_valid + Cf::kMmaK - 1) / Cf::kMmaK;
         done();
+        bool here = false;  // the fill at hand was seen to have landed
         for (int32_t f = 0; f < fills; ++f) {
           // first and last fill of an accumulation
           const bool opens = Cf::kSums ? f % Cf::kSegFills == 0 : f == 0;
           const bool closes = f + 1 == fills || (Cf::kSums && (f + 1) % Cf::kSegFills == 0);
-          if (opens && !warp_poll(smem_addr(&bars.tempty[acc]), acc_phase ^ 1u, abort_flag, kSiteMma, lane)) {
-            ok = false;
-            break;
-          }
-          if (!warp_poll(smem_addr(&bars.full[stage]), phase, abort_flag, kSiteMma, lane)) {
+          if ((opens && !warp_poll(tempty0 + acc * 8, acc_phase ^ 1u, abort_flag, kSiteMma, lane)) ||
+              (!here && !warp_poll(full0 + stage * 8, phase, abort_flag, kSiteMma, lane))) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const int steps = f + 1 == fills ? last_steps : 4;
-          const uint64_t da0 = smem_desc_sw128(smem_addr(sA + (size_t)stage * Cf::kABytes), a_lbo, 1024);
-          const uint64_t db0 = smem_desc_sw128(smem_addr(sB + (size_t)stage * Cf::kBBytes), b_lbo, 1024);
+          const uint32_t a_lo = (uint32_t)da + (uint32_t)stage * (Cf::kABytes >> 4);
+          const uint32_t b_lo = (uint32_t)db + (uint32_t)stage * (Cf::kBBytes >> 4);
           const uint32_t d = tmem_base + (uint32_t)(acc * BN);
-          if (elect_one()) {
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-              if (kk < steps) {
-                const uint64_t da = da0 + (uint64_t)((a_step * kk) >> 4);
-                const uint64_t db = db0 + (uint64_t)((b_step * kk) >> 4);
-                const uint32_t add = (!opens || kk > 0) ? 1u : 0u;
-                if constexpr (Cf::kBytes) umma_f8<G>(d, da, db, idesc, add);
-                else if constexpr (G == 2) umma_f16_pair(d, da, db, idesc, add);
-                else umma_f16(d, da, db, idesc, add);
-              }
-            }
-            if constexpr (G == 2) umma_commit_pair(smem_addr(&bars.empty[stage]), 0x3);
-            else umma_commit(smem_addr(&bars.empty[stage]));
-            if (closes) {
-              if constexpr (G == 2) umma_commit_pair(smem_addr(&bars.tfull[acc]), 0x3);
-              else umma_commit(smem_addr(&bars.tfull[acc]));
-            }
+          const uint32_t empty = empty0 + stage * 8;
+          if (++stage == S) {
+            stage = 0;
+            phase ^= 1u;
           }
-          __syncwarp();
+          // the next fill's barrier is read while this one's MMAs are issued
+          const bool peek = f + 1 < fills && mbar_test_wait(full0 + stage * 8, phase);
+          if (elect_one()) {
+            if (f + 1 < fills || last_steps == 4) {
+#pragma unroll
+              for (uint32_t kk = 0; kk < 4; ++kk)
+                umma_words<G, Cf::kBytes>(d, a_lo + a_step * kk, a_hi, b_lo + b_step * kk, b_hi, idesc,
+                                          (!opens || kk > 0) ? 1u : 0u);
+            } else {
+              for (uint32_t kk = 0; kk < (uint32_t)last_steps; ++kk)
+                umma_words<G, Cf::kBytes>(d, a_lo + a_step * kk, a_hi, b_lo + b_step * kk, b_hi, idesc,
+                                          (!opens || kk > 0) ? 1u : 0u);
+            }
+            commit(empty);
+            if (closes) commit(tfull0 + acc * 8);
+          }
+          here = __all_sync(0xffffffffu, peek);
           issued_any = true;
           if (closes && ++acc == 2) {
             acc = 0;
             acc_phase ^= 1u;
-          }
-          if (++stage == S) {
-            stage = 0;
-            phase ^= 1u;
           }
         }
       }
@@ -1071,13 +1080,16 @@ tbStatus launch(Launch& L, int sms, int dev, cudaStream_t stream) {
   cfg.blockDim = dim3(kThreadsG, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)cluster;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  // The set-up (barriers, TMEM) overlaps the end of the kernel before.
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ta, ta32, tb_, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return tb_fail(TB_ERR_CUDA, std::string("tb_grouped launch: ") + cudaGetErrorString(e));

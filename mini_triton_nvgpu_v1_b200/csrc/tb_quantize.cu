@@ -129,6 +129,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) tb_quantize_kerne
   const int ncol = (int)min((int64_t)8, max((int64_t)0, p.cols - c0));
   const int nrow = (int)min((int64_t)8, max((int64_t)0, (p.rows - r0 + 15) / 16));  // this thread's rows
   const T* x = static_cast<const T*>(p.x) + b * p.batch_x + r0 * p.ldx + c0;
+  // Launched while the kernel before it in the stream ends: nothing of memory
+  // is touched before that one's writes are there. The next may do the same.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   uint32_t v[8][W];
   if (p.vec_x && (int64_t)tr * 128 + 128 <= p.rows && (int64_t)tc * 128 + 128 <= p.cols) {
@@ -278,10 +282,19 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) tb_quantize_kerne
 
 template <typename T>
 cudaError_t launch_q(const QParams& p, int br, int bc, unsigned grid, cudaStream_t st) {
-  if (br == 1) tb_quantize_kernel<T, 1, 128><<<grid, 256, 0, st>>>(p);
-  else if (bc == 1) tb_quantize_kernel<T, 128, 1><<<grid, 256, 0, st>>>(p);
-  else tb_quantize_kernel<T, 128, 128><<<grid, 256, 0, st>>>(p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  auto kern = br == 1 ? tb_quantize_kernel<T, 1, 128> : bc == 1 ? tb_quantize_kernel<T, 128, 1>
+                                                                : tb_quantize_kernel<T, 128, 128>;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+  return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
 }  // namespace

@@ -361,25 +361,25 @@ __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
   for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
 }
 
-// D[tmem] (+)= A[smem] · B[smem], kind::f8f6f4 (e4m3 inputs, f32 accumulate),
-// on one CTA (G = 1) or a CTA pair.
-template <int G>
-__device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
-                                        uint32_t idesc, uint32_t accumulate) {
-  if constexpr (G == 2)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
+// D[tmem] (+)= A[smem] · B[smem] on one CTA (G = 1) or a pair, kind::f8f6f4
+// (BYTES: e4m3) or kind::f16. The descriptors come as their two words: the
+// start address is in the low one, so that a loop adds to that word alone.
+template <int G, bool BYTES>
+__device__ __forceinline__ void umma_words(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
+                                           uint32_t idesc, uint32_t accumulate) {
+#define TB_UMMA(GROUP, KIND)                                                                            \
+  asm volatile(                                                                                         \
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"                                                     \
+      "setp.ne.b32 p, %6, 0;\n\t"                                                                       \
+      "mov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"                                              \
+      "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], da, db, %5, p;\n\t}\n" ::"r"(d_tmem),       \
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)                           \
+      : "memory")
+  if constexpr (G == 2 && BYTES) TB_UMMA("2", "f8f6f4");
+  else if constexpr (G == 2) TB_UMMA("2", "f16");
+  else if constexpr (BYTES) TB_UMMA("1", "f8f6f4");
+  else TB_UMMA("1", "f16");
+#undef TB_UMMA
 }
 
 // Shared-memory matrix descriptor (tcgen05 "matrix descriptor"):

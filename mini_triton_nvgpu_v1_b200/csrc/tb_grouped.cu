@@ -124,6 +124,7 @@ struct GBars {
   GTile tile[kTileSlots];
   alignas(16) float col_scale[8][128];  // per epilogue warp: SB of its columns in the block at hand
   uint32_t tmem_holder;
+  uint32_t issued;  // the producer's fills
   int abort_flag;
 };
 
@@ -148,7 +149,9 @@ struct GParams {
   void* C;
   int64_t ldc, group_c;
   GScale sa, sb;
-  int32_t stages, split;  // ring depth; CTAs per cluster that share a tile's K range (G = 1)
+  int32_t stages;         // ring depth
+  int32_t split, split_log2;  // CTAs per cluster that share a tile's K range (G = 1)
+  int32_t small_rows;     // rows of tmAs's boxes: a K-major A tile of few rows comes in these (G = 1)
 };
 
 __device__ __forceinline__ int32_t read_offset(const GParams& p, int32_t i) {
@@ -161,42 +164,53 @@ __device__ __forceinline__ int32_t read_offset(const GParams& p, int32_t i) {
   return (int32_t)(v < 0 ? 0 : v > rows ? rows : v);
 }
 
-// Tile t. Inside a group, tiles go in bands of 8 tile rows, rows fastest:
-// the CTAs at work share few panels of A and B.
+// Tile t, worked out by a whole warp. Inside a group, tiles go in bands of 8
+// tile rows, rows fastest: the CTAs at work share few panels of A and B.
+// `cursor`: a group at or before the tile's; it moves on with t.
 template <int BM, int BN, int KB>
 __device__ __forceinline__ GTile tile_at(const GParams& p, const GroupTable& tab, int32_t t, int32_t part,
-                                         int32_t& cursor) {
+                                         int32_t& cursor, int lane) {
   GTile g;
-  int32_t u, group_rows, tiles_m;
+  uint32_t u;
+  int32_t group_rows, tiles_m;
   if (p.k_grouped) {
-    const int32_t per = p.tiles_m * p.tiles_n;
-    g.e = t / per;
-    u = t - g.e * per;
+    const uint32_t per = (uint32_t)p.tiles_m * (uint32_t)p.tiles_n;
+    g.e = (int32_t)((uint32_t)t / per);
+    u = (uint32_t)t - (uint32_t)g.e * per;
     tiles_m = p.tiles_m;
     group_rows = p.M;
     g.row0 = 0;
     g.k0 = tab.start[g.e];
     g.k_end = g.k0 + tab.rows[g.e];
   } else {
-    while (tab.cum[cursor + 1] <= t) ++cursor;  // t < cum[groups], and t only grows
+    uint32_t before;  // groups from the cursor on that end at or before t: 32 looked at together
+    do {
+      const int32_t i = cursor + lane;
+      before = __ballot_sync(0xffffffffu, i < p.groups && tab.cum[i + 1] <= t);
+      cursor += __popc(before);
+    } while (before == 0xffffffffu);
     g.e = cursor;
-    u = t - tab.cum[cursor];
+    u = (uint32_t)(t - tab.cum[cursor]);
     group_rows = tab.rows[cursor];
     tiles_m = (group_rows + BM - 1) / BM;
     g.row0 = tab.start[cursor];
     g.k0 = 0;
     g.k_end = p.K;
   }
-  const int32_t band = u / (8 * p.tiles_n), v = u - band * 8 * p.tiles_n;
-  const int32_t height = min(8, tiles_m - band * 8);
-  const int32_t n = v / height, m = band * 8 + v - n * height;
-  g.row0 += m * BM;
-  g.rows = min(BM, group_rows - m * BM);
-  g.n0 = n * BN;
+  uint32_t m = 0, n = u;
+  if (tiles_m > 1) {
+    const uint32_t band = u / (8u * (uint32_t)p.tiles_n), v = u - band * 8u * (uint32_t)p.tiles_n;
+    const uint32_t height = min(8u, (uint32_t)tiles_m - band * 8u);
+    n = v / height;
+    m = band * 8u + v - n * height;
+  }
+  g.row0 += (int32_t)m * BM;
+  g.rows = min(BM, group_rows - (int32_t)m * BM);
+  g.n0 = (int32_t)n * BN;
   g.cols = min(BN, p.N - g.n0);
-  const int32_t fills = (g.k_end - g.k0 + KB - 1) / KB;
-  g.f0 = (int32_t)((int64_t)fills * part / p.split);
-  g.f1 = (int32_t)((int64_t)fills * (part + 1) / p.split);
+  const uint32_t fills = (uint32_t)(g.k_end - g.k0 + KB - 1) / KB;  // < 2^25: 8 parts of it fit in 32 bits
+  g.f0 = (int32_t)(fills * (uint32_t)part >> p.split_log2);
+  g.f1 = (int32_t)(fills * (uint32_t)(part + 1) >> p.split_log2);
   return g;
 }
 
@@ -329,7 +343,7 @@ __device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c
 
 template <int KIND, int BN, int G>
 __global__ void __launch_bounds__(kThreadsG, 1)
-    tb_grouped_sm100_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA32,
+    tb_grouped_sm100_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmAs,
                             const __grid_constant__ CUtensorMap tmB, const __grid_constant__ GParams p) {
   using Cf = GCfg<KIND, BN, G>;
   extern __shared__ uint8_t smem_raw[];
@@ -373,7 +387,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     fence_mbar_init();
     if (lane == 0) {
       tma_prefetch_desc(&tmA);
-      tma_prefetch_desc(&tmA32);
+      tma_prefetch_desc(&tmAs);
       tma_prefetch_desc(&tmB);
     }
   }
@@ -381,28 +395,33 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     tmem_alloc_g<G>(smem_addr(&bars.tmem_holder), Cf::kTmemCols);
     tmem_relinquish_g<G>();
   }
-  // What this launch reads may be written by the kernel before it in the
-  // stream, which it does not wait for until here (programmatic launch).
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (int32_t e = threadIdx.x; e < p.groups; e += kThreadsG) {
-    const int32_t s = read_offset(p, e), n = max(0, read_offset(p, e + 1) - s);
-    tab.start[e] = s;
-    tab.rows[e] = n;
-  }
-  __syncthreads();
-  if (warp == 0 && !p.k_grouped) {
+  if (warp == 3) {
+    // The scheduler builds the table of tiles meanwhile. What this launch
+    // reads may be written by the kernel before it in the stream, which each
+    // role waits for before its first access to memory (programmatic launch).
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     int32_t before = 0;
     for (int32_t e0 = 0; e0 < p.groups; e0 += 32) {
-      int32_t v = e0 + lane < p.groups ? (tab.rows[e0 + lane] + Cf::kBM - 1) / Cf::kBM * p.tiles_n : 0;
+      const int32_t e = e0 + lane;
+      int32_t start = 0, rows = 0;
+      if (e < p.groups) {
+        const int32_t lo = read_offset(p, e), hi = read_offset(p, e + 1);
+        start = lo;
+        rows = max(0, hi - lo);
+        tab.start[e] = start;
+        tab.rows[e] = rows;
+      }
+      int32_t v = (rows + Cf::kBM - 1) / Cf::kBM * p.tiles_n;
 #pragma unroll
       for (int d = 1; d < 32; d *= 2) {
         const int32_t o = __shfl_up_sync(0xffffffffu, v, d);
         if (lane >= d) v += o;
       }
-      if (e0 + lane < p.groups) tab.cum[e0 + lane + 1] = before + v;
+      if (e < p.groups) tab.cum[e + 1] = before + v;
       before += __shfl_sync(0xffffffffu, v, 31);
     }
     if (lane == 0) tab.cum[0] = 0;
+    __syncwarp();
   }
   tc_fence_before();
   if (cluster > 1) cluster_sync();
@@ -410,14 +429,10 @@ __global__ void __launch_bounds__(kThreadsG, 1)
   tc_fence_after();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem_base = bars.tmem_holder;
-  const int32_t tiles = p.k_grouped ? p.groups * p.tiles_m * p.tiles_n : tab.cum[p.groups];
-
-  // The tiles in turn: take() waits for the next one, done() gives its slot back.
+  // The tiles in turn, up to one without columns: take() waits for the next
+  // (and says no after the last, or when it gave up), done() gives its slot back.
   int slot = 0;
   uint32_t slot_phase = 0;
-  auto take = [&](uint32_t site) {
-    return warp_poll(smem_addr(&bars.tile_full[slot]), slot_phase, abort_flag, site, lane);
-  };
   auto done = [&]() {
     __syncwarp();
     if (lane == 0) mbar_arrive(smem_addr(&bars.tile_empty[slot]));
@@ -430,6 +445,11 @@ __global__ void __launch_bounds__(kThreadsG, 1)
   auto field = [&](int32_t GTile::*m) {
     return *const_cast<const volatile int32_t*>(&(bars.tile[slot].*m));
   };
+  bool ok = true;  // false: a wait gave up
+  auto take = [&](uint32_t site) {
+    ok = ok && warp_poll(smem_addr(&bars.tile_full[slot]), slot_phase, abort_flag, site, lane);
+    return ok && field(&GTile::cols) > 0;
+  };
 
   // Sums in registers, 256 columns: 128 per epilogue thread. 256 threads ×
   // 224 + 128 × 56 registers = the launch's 384 × 168.
@@ -441,14 +461,14 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     int stage = 0;
     uint32_t phase = 0;
     uint32_t issued = 0;
-    bool ok = true;
-    for (int32_t t = first; t < tiles && ok; t += stride) {
-      if (!take(kSiteProducer)) break;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    while (take(kSiteProducer)) {
       const GTile g = bars.tile[slot];
       done();
-      // K-major A of a short tile: only the 32-row boxes that hold its rows
-      const int boxes = G == 1 && !p.a_mn ? (min(g.rows, 128) + 31) / 32 : 4;
-      const uint32_t bytes = (boxes < 4 ? (uint32_t)boxes * 4096u : Cf::kABytes) + Cf::kBBytes;
+      // K-major A of a tile with few rows: only the small boxes that hold them
+      const int sr = p.small_rows;
+      const bool few = G == 1 && !p.a_mn && g.rows <= 3 * sr;
+      const uint32_t bytes = (few ? (uint32_t)((g.rows + sr - 1) / sr * sr) * 128u : Cf::kABytes) + Cf::kBBytes;
       const int32_t bn = g.n0 + (int32_t)rank * Cf::kBnCta;
       const int32_t be = p.k_grouped ? 0 : g.e;
       for (int32_t f = g.f0; f < g.f1; ++f) {
@@ -487,10 +507,10 @@ __global__ void __launch_bounds__(kThreadsG, 1)
 #pragma unroll
             for (int j = 0; j < 128 / Cf::kMnBox; ++j)
               load2(dA + j * Cf::kMnBoxBytes, &tmA, am + Cf::kMnBox * j, kx);
-          } else if (boxes == 4) {
+          } else if (!few) {
             load2(dA, &tmA, kx, am);
           } else {
-            for (int j = 0; j < boxes; ++j) load2(dA + j * 4096, &tmA32, kx, am + 32 * j);
+            for (int r = 0; r < g.rows; r += sr) load2(dA + r * 128, &tmAs, kx, am + r);
           }
           if (p.b_kmaj) {
             load3(dB, kx, bn);
@@ -508,21 +528,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
         }
       }
     }
-    if (lane == 0 && leader) {
-      // The newest fill of each stage must land before the CTAs exit.
-      const uint32_t last = min(issued, (uint32_t)S);
-      for (uint32_t i = 0; i < last; ++i) {
-        const uint32_t f = issued - 1 - i;
-        const uint32_t par = (f / S) & 1;
-        const long long t0 = clock64();
-        while (!mbar_try_wait(smem_addr(&bars.full[f % S]), par)) {
-          if (clock64() - t0 > kWaitBudgetCycles) {
-            record_error(TB_ERR_DEVICE_TIMEOUT, kSiteDrain);
-            break;
-          }
-        }
-      }
-    }
+    if (lane == 0) bars.issued = issued;
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
     if (leader) {
@@ -541,12 +547,8 @@ __global__ void __launch_bounds__(kThreadsG, 1)
       };
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
-      bool issued_any = false, ok = true;
-      for (int32_t t = first; t < tiles && ok; t += stride) {
-        if (!take(kSiteMma)) {
-          ok = false;
-          break;
-        }
+      bool issued_any = false;
+      while (take(kSiteMma)) {
         // this tile's fills, and the MMA steps of the last one
         const int32_t fills = field(&GTile::f1) - field(&GTile::f0);
         const int32_t last_valid = min(Cf::kKB, field(&GTile::k_end) - field(&GTile::k0) - (field(&GTile::f1) - 1) * Cf::kKB);
@@ -614,8 +616,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     if (p.k_grouped) {
       int stage = 0;
       uint32_t fix_phase = 0;  // bit s: parity of stage s's next fix
-      for (int32_t t = first; t < tiles; t += stride) {
-        if (!take(kSiteFixer)) break;
+      while (take(kSiteFixer)) {
         const GTile g = bars.tile[slot];
         done();
         const int32_t n = g.f1 - g.f0;
@@ -624,8 +625,10 @@ __global__ void __launch_bounds__(kThreadsG, 1)
         const int32_t valid = min(Cf::kKB, g.k_end - (g.k0 + (g.f1 - 1) * Cf::kKB));
         stage = (stage + n) % S;
         if (valid % Cf::kMmaK == 0) continue;
-        if (!warp_wait(smem_addr(&bars.fix[last]), (fix_phase >> last) & 1u, abort_flag, kSiteFixer, lane))
+        if (!warp_wait(smem_addr(&bars.fix[last]), (fix_phase >> last) & 1u, abort_flag, kSiteFixer, lane)) {
+          ok = false;
           break;
+        }
         fix_phase ^= 1u << last;
         // K rows [valid, next multiple of the K step) of every box of both
         // operands: 128 bytes per row (the swizzle stays inside a row)
@@ -649,14 +652,17 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     }
   } else {
     // ----------------------------------------------------------- scheduler
+    const int32_t tiles = p.k_grouped ? p.groups * p.tiles_m * p.tiles_n : tab.cum[p.groups];
     int32_t cursor = 0;
-    for (int32_t t = first; t < tiles; t += stride) {
+    for (int32_t t = first;; t += stride) {
+      GTile g = {};
+      if (t < tiles) g = tile_at<Cf::kBM, BN, Cf::kKB>(p, tab, t, part, cursor, lane);
       if (!warp_wait(smem_addr(&bars.tile_empty[slot]), slot_phase ^ 1u, abort_flag, kSiteScheduler, lane)) break;
-      const GTile g = tile_at<Cf::kBM, BN, Cf::kKB>(p, tab, t, part, cursor);
       if (lane == 0) {
         bars.tile[slot] = g;
         mbar_arrive(smem_addr(&bars.tile_full[slot]));
       }
+      if (t >= tiles) break;  // the tile without columns
       if (++slot == kTileSlots) {
         slot = 0;
         slot_phase ^= 1u;
@@ -720,9 +726,8 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     auto row_at = [&]() { return tile_at_c() + ((int64_t)row_in_tile * p.ldc + c_half) * el; };
     int acc = 0;
     uint32_t acc_phase = 0, red_phase = 0;
-    bool ok = true;
-    for (int32_t t = first; t < tiles && ok; t += stride) {
-      if (!take(kSiteEpilogue)) break;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    while (take(kSiteEpilogue)) {
       // Only the count of accumulations and the scales' places stay in
       // registers during the sums; the rest is read again for the stores.
       const int32_t fills = field(&GTile::f1) - field(&GTile::f0);
@@ -822,6 +827,9 @@ __global__ void __launch_bounds__(kThreadsG, 1)
 #pragma unroll
           for (int i = 0; i < 16; ++i) unpack_f32x2(sum[c][i], v[c][2 * i], v[c][2 * i + 1]);
       } else {
+        const bool row_ok = row_in_tile < field(&GTile::rows);
+        const int32_t cols = field(&GTile::cols) - c_half;
+        char* row = row_at();
         if (fills > 0) {
           if (!warp_poll(smem_addr(&bars.tfull[acc]), acc_phase, abort_flag, kSiteEpilogue, lane)) {
             ok = false;
@@ -829,9 +837,6 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           }
           tc_fence_after();
         }
-        const bool row_ok = row_in_tile < field(&GTile::rows);
-        const int32_t cols = field(&GTile::cols) - c_half;
-        char* row = row_at();
         if (p.split > 1) {
           // every CTA has read the previous tile's partial sums
           if (!cluster_wait(&bars.consumed, red_phase ^ 1u)) {
@@ -929,6 +934,21 @@ __global__ void __launch_bounds__(kThreadsG, 1)
   }
 
   __syncthreads();
+  if (*abort_flag && threadIdx.x == 0 && leader) {
+    // Given up: the newest fill of each stage must land before the CTAs exit.
+    // (Otherwise the MMAs have waited for every fill.)
+    const uint32_t last = min(bars.issued, (uint32_t)S);
+    for (uint32_t i = 0; i < last; ++i) {
+      const uint32_t f = bars.issued - 1 - i;
+      const long long t0 = clock64();
+      while (!mbar_try_wait(smem_addr(&bars.full[f % S]), (f / S) & 1)) {
+        if (clock64() - t0 > kWaitBudgetCycles) {
+          record_error(TB_ERR_DEVICE_TIMEOUT, kSiteDrain);
+          break;
+        }
+      }
+    }
+  }
   if (cluster > 1) cluster_sync();
   if (warp == 1) {
     tc_fence_after();
@@ -1048,6 +1068,7 @@ struct Launch {
   Operand a, b;
   int el, bf16;
   int64_t tiles;  // an upper bound of the tiles
+  int64_t rows;   // mean rows of a group that has any
   GParams p;
 };
 
@@ -1055,13 +1076,15 @@ template <int KIND, int BN, int G>
 tbStatus launch(Launch& L, int sms, int dev, cudaStream_t stream) {
   using Cf = GCfg<KIND, BN, G>;
   GParams& p = L.p;
-  CUtensorMap ta, ta32, tb_;
-  std::memset(&ta32, 0, sizeof(ta32));
+  CUtensorMap ta, tas, tb_;
+  std::memset(&tas, 0, sizeof(tas));
   tbStatus st = encode(&ta, 2, L.a, L.el, L.bf16, p.a_mn ? Cf::kMnBox : Cf::kKB, p.a_mn ? Cf::kKB : 128, "A");
-  if (st == TB_OK && !p.a_mn) st = encode(&ta32, 2, L.a, L.el, L.bf16, Cf::kKB, 32, "A");
+  p.small_rows = L.rows <= 16 ? 8 : 32;
+  if (st == TB_OK && !p.a_mn && G == 1) st = encode(&tas, 2, L.a, L.el, L.bf16, Cf::kKB, (uint32_t)p.small_rows, "A");
   if (st == TB_OK)
     st = encode(&tb_, 3, L.b, L.el, L.bf16, p.b_kmaj ? Cf::kKB : Cf::kMnBox, p.b_kmaj ? Cf::kBnCta : Cf::kKB, "B");
   if (st != TB_OK) return st;
+  p.split_log2 = p.split == 8 ? 3 : p.split == 4 ? 2 : p.split == 2 ? 1 : 0;
   const size_t fixed = 1024 + kTailBytes + (p.split > 1 ? Cf::kRedBytes : 0);
   p.stages = (int)std::min<size_t>(kMaxStages, (kSmemLimitG - fixed) / Cf::kStageBytes);
   const size_t smem = fixed + (size_t)p.stages * Cf::kStageBytes;
@@ -1090,7 +1113,7 @@ tbStatus launch(Launch& L, int sms, int dev, cudaStream_t stream) {
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ta, ta32, tb_, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ta, tas, tb_, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return tb_fail(TB_ERR_CUDA, std::string("tb_grouped launch: ") + cudaGetErrorString(e));
   return TB_OK;
@@ -1110,6 +1133,7 @@ tbStatus launch_tile(Launch& L, int sms, int dev, cudaStream_t stream) {
 // Tile and K split. `rows`: mean rows of a group that has any.
 tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int dev, cudaStream_t stream) {
   GParams& p = L.p;
+  L.rows = rows;
   const int64_t n = p.N;
   const int64_t kmax = p.k_grouped ? cdiv(p.K, std::max<int64_t>(1, groups)) : p.K;
   const int64_t m = p.k_grouped ? p.M : rows;

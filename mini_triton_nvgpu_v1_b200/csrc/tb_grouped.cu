@@ -458,6 +458,18 @@ __global__ void __launch_bounds__(kThreadsG, 1)
   if constexpr (kMoveRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   if (warp == 0) {
     // ------------------------------------------------------------ producer
+    // An operand's fill is a few boxes: box j of fill f lies at coordinates
+    // (x + f·fx + j·jx, y + f·fy + j·jy) and goes to dst + j·step. What
+    // decides them is worked out once per tile; with the parameters read and
+    // tested inside the loop a fill took 475 cycles to issue.
+    const bool a_mn = p.a_mn, b_mn = !p.b_kmaj, grouped_k = p.k_grouped;
+    const int32_t a_fx = a_mn ? 0 : Cf::kKB, a_fy = a_mn ? Cf::kKB : 0;
+    const int32_t b_fx = b_mn ? 0 : Cf::kKB, b_fy = b_mn ? Cf::kKB : 0;
+    const int32_t b_boxes = b_mn ? Cf::kBnCta / Cf::kMnBox : 1;
+    const int32_t sr = p.small_rows;
+    const uint32_t full0 = smem_addr(&bars.full[0]), empty0 = smem_addr(&bars.empty[0]), fix0 = smem_addr(&bars.fix[0]);
+    const uint32_t full0_leader = G == 2 ? map_to_cta(full0, 0) : full0;
+    const uint32_t sa0 = smem_addr(sA), sb0 = smem_addr(sB);
     int stage = 0;
     uint32_t phase = 0;
     uint32_t issued = 0;
@@ -466,61 +478,51 @@ __global__ void __launch_bounds__(kThreadsG, 1)
       const GTile g = bars.tile[slot];
       done();
       // K-major A of a tile with few rows: only the small boxes that hold them
-      const int sr = p.small_rows;
-      const bool few = G == 1 && !p.a_mn && g.rows <= 3 * sr;
-      const uint32_t bytes = (few ? (uint32_t)((g.rows + sr - 1) / sr * sr) * 128u : Cf::kABytes) + Cf::kBBytes;
-      const int32_t bn = g.n0 + (int32_t)rank * Cf::kBnCta;
-      const int32_t be = p.k_grouped ? 0 : g.e;
+      const bool few = G == 1 && !a_mn && g.rows <= 3 * sr;
+      const CUtensorMap* const map_a = few ? &tmAs : &tmA;
+      const int32_t a_boxes = a_mn ? 128 / Cf::kMnBox : few ? (g.rows + sr - 1) / sr : 1;
+      const uint32_t a_step = a_mn ? Cf::kMnBoxBytes : (uint32_t)sr * 128u;
+      const int32_t a_jx = a_mn ? Cf::kMnBox : 0, a_jy = a_mn ? 0 : sr;
+      const uint32_t bytes = (few ? (uint32_t)a_boxes * a_step : Cf::kABytes) + Cf::kBBytes;
+      const int32_t am = g.row0 + (int32_t)rank * 128, bn = g.n0 + (int32_t)rank * Cf::kBnCta;
+      const int32_t k_first = g.k0 + g.f0 * Cf::kKB;
+      int32_t ax = a_mn ? am : k_first, ay = a_mn ? k_first : am;
+      int32_t bx = b_mn ? bn : k_first, by = b_mn ? k_first : bn;
+      const int32_t be = grouped_k ? 0 : g.e;
+      // the fill (if any) whose last rows the fixer takes out
+      const int32_t fix_at = grouped_k && (g.k_end - g.k0) % Cf::kMmaK != 0 && g.f1 * Cf::kKB > g.k_end - g.k0 - Cf::kMmaK
+                                 ? (g.k_end - g.k0) / Cf::kKB : -1;
       for (int32_t f = g.f0; f < g.f1; ++f) {
-        if (issued >= (uint32_t)S &&
-            !warp_wait(smem_addr(&bars.empty[stage]), phase ^ 1u, abort_flag, kSiteProducer, lane)) {
+        if (issued >= (uint32_t)S && !warp_wait(empty0 + stage * 8, phase ^ 1u, abort_flag, kSiteProducer, lane)) {
           ok = false;
           break;
         }
-        const int32_t kx = g.k0 + f * Cf::kKB;
-        const bool fix = p.k_grouped && (min(Cf::kKB, g.k_end - kx) % Cf::kMmaK) != 0;
-        const uint32_t dA = smem_addr(sA + (size_t)stage * Cf::kABytes);
-        const uint32_t dB = smem_addr(sB + (size_t)stage * Cf::kBBytes);
         if (elect_one()) {
           uint32_t bar;
-          if (fix) {  // this CTA's fixer takes the fill on from here
-            bar = smem_addr(&bars.fix[stage]);
+          if (f == fix_at) {  // this CTA's fixer takes the fill on from here
+            bar = fix0 + stage * 8;
             mbar_expect_tx(bar, bytes);
           } else {
-            bar = smem_addr(&bars.full[stage]);
-            if (leader) mbar_expect_tx(bar, G * bytes);
-            if constexpr (G == 2) {
-              bar = map_to_cta(bar, 0);
-              if (p.k_grouped && !leader) mbar_arrive_remote(bar);
-            }
+            bar = full0_leader + stage * 8;
+            if (leader) mbar_expect_tx(full0 + stage * 8, G * bytes);
+            else if (grouped_k) mbar_arrive_remote(bar);
           }
-          auto load2 = [&](uint32_t dst, const CUtensorMap* m, int32_t x, int32_t y) {
-            if constexpr (G == 2) tma_load_2d_pair(dst, m, bar, x, y);
-            else tma_load_2d(dst, m, bar, x, y);
-          };
-          auto load3 = [&](uint32_t dst, int32_t x, int32_t y) {
-            if constexpr (G == 2) tma_load_3d_pair(dst, &tmB, bar, x, y, be);
-            else tma_load_3d(dst, &tmB, bar, x, y, be);
-          };
-          const int32_t am = g.row0 + (int32_t)rank * 128;
-          if (p.a_mn) {
-#pragma unroll
-            for (int j = 0; j < 128 / Cf::kMnBox; ++j)
-              load2(dA + j * Cf::kMnBoxBytes, &tmA, am + Cf::kMnBox * j, kx);
-          } else if (!few) {
-            load2(dA, &tmA, kx, am);
-          } else {
-            for (int r = 0; r < g.rows; r += sr) load2(dA + r * 128, &tmAs, kx, am + r);
+          uint32_t dst = sa0 + (uint32_t)stage * Cf::kABytes;
+          for (int32_t j = 0; j < a_boxes; ++j, dst += a_step) {
+            if constexpr (G == 2) tma_load_2d_pair(dst, map_a, bar, ax + j * a_jx, ay + j * a_jy);
+            else tma_load_2d(dst, map_a, bar, ax + j * a_jx, ay + j * a_jy);
           }
-          if (p.b_kmaj) {
-            load3(dB, kx, bn);
-          } else {
-#pragma unroll
-            for (int j = 0; j < Cf::kBnCta / Cf::kMnBox; ++j)
-              load3(dB + j * Cf::kMnBoxBytes, bn + Cf::kMnBox * j, kx);
+          dst = sb0 + (uint32_t)stage * Cf::kBBytes;
+          for (int32_t j = 0; j < b_boxes; ++j, dst += Cf::kMnBoxBytes) {
+            if constexpr (G == 2) tma_load_3d_pair(dst, &tmB, bar, bx + j * Cf::kMnBox, by, be);
+            else tma_load_3d(dst, &tmB, bar, bx + j * Cf::kMnBox, by, be);
           }
         }
         __syncwarp();
+        ax += a_fx;
+        ay += a_fy;
+        bx += b_fx;
+        by += b_fy;
         ++issued;
         if (++stage == S) {
           stage = 0;

@@ -95,7 +95,7 @@ struct GCfg {
   static constexpr int kHalfCols = BN / 2;              // columns per epilogue warp
   static constexpr int kChunks = kHalfCols / 32;
   static constexpr uint32_t kRedStride = (BN + 4) * 4;  // bytes per row of the cluster's partial sums
-  static constexpr uint32_t kRedBytes = 128 * kRedStride;
+  static constexpr uint32_t kRedBytes = 32 * kRedStride;  // 32 rows at a time
 };
 
 // Tiles of every group, built by each CTA from the offsets.
@@ -310,6 +310,20 @@ __device__ __forceinline__ void emit32(const GParams& p, char* q, float (&v)[32]
   }
 }
 
+// beta·C + v of `ncol` (at most 4) consecutive columns at q.
+__device__ __forceinline__ void emit4(const GParams& p, char* q, float4 s, int ncol) {
+  const float v[4] = {s.x, s.y, s.z, s.w};
+  if (ncol >= 4 && p.vec && !p.beta) {
+    if (p.c_dtype == TB_F32) *reinterpret_cast<float4*>(q) = s;
+    else *reinterpret_cast<uint2*>(q) = make_uint2(pack2(p, s.x, s.y), pack2(p, s.z, s.w));
+    return;
+  }
+  const int el = p.c_dtype == TB_F32 ? 4 : 2;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < ncol) store_out(p, q + i * el, p.beta ? v[i] + load_out(p, q + i * el) : v[i]);
+}
+
 // Two f32 in one register pair.
 __device__ __forceinline__ uint64_t pack_u32x2(uint32_t a, uint32_t b) {
   uint64_t r;
@@ -381,7 +395,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     // producer, epilogue warps, and those of MMA issuer and fixer that are at work
     init(bars.tile_empty, kTileSlots, 9 + (leader ? 1 : 0) + (p.k_grouped ? 1 : 0));
     init(&bars.drain, 1, 1);
-    init(&bars.ready, 1, 8 * p.split);
+    init(&bars.ready, 1, 1);
     init(&bars.consumed, 1, 8 * p.split);
     if (lane == 0) bars.abort_flag = 0;
     fence_mbar_init();
@@ -689,45 +703,74 @@ __global__ void __launch_bounds__(kThreadsG, 1)
         else mbar_arrive(tempty0 + acc * 8);
       }
     };
-    auto cluster_wait = [&](uint64_t* bar, uint32_t par) {
-      int good = 1;
-      if (lane == 0) {
-        const uint32_t b = smem_addr(bar);
-        const long long t0 = clock64();
-        while (!mbar_try_wait_cluster(b, par)) {
-          if (*abort_flag) {
-            good = 0;
-            break;
-          }
-          if (clock64() - t0 > kWaitBudgetCycles) {
-            record_error(TB_ERR_DEVICE_TIMEOUT, kSiteCluster);
-            *abort_flag = 1;
-            good = 0;
-            break;
-          }
-        }
-      }
-      good = __shfl_sync(0xffffffffu, good, 0);
-      return good != 0;
-    };
-    auto cluster_arrive = [&](uint64_t* bar) {
-      __syncwarp();
-      if (lane < p.split) mbar_arrive_cluster(map_to_cta(smem_addr(bar), (uint32_t)lane));
-    };
-    // this row's partial sums of chunk c, for the cluster
-    auto leave = [&](int c, const float (&s)[32]) {
-      float4* dst = reinterpret_cast<float4*>(red + (size_t)row_in_tile * Cf::kRedStride + (c_half + c * 32) * 4);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) dst[i] = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
-    };
     // the tile at hand in C, and this thread's row and column half of it
     auto tile_at_c = [&]() {
       const int64_t group = p.k_grouped ? (int64_t)field(&GTile::e) * p.group_c : 0;
       return static_cast<char*>(p.C) + (group + (int64_t)field(&GTile::row0) * p.ldc + field(&GTile::n0)) * el;
     };
     auto row_at = [&]() { return tile_at_c() + ((int64_t)row_in_tile * p.ldc + c_half) * el; };
+    // The cluster's CTAs hold partial sums of one tile. 32 rows at a time,
+    // each sends row r of its own (sums(c): this warp's chunk c) to CTA
+    // r mod split, which adds them in CTA order and stores the row. The rows
+    // come as st.async, counted on the receiver's barrier: no fence, and the
+    // sums are read from the CTA's own shared memory. (Partial sums left
+    // behind a cluster-scope release and read by the others took 4100 cycles
+    // from the last fill to the stores.) False: a wait gave up.
+    uint32_t red_phase = 0;
+    auto share = [&](auto&& sums) -> bool {
+      const int rows = field(&GTile::rows), cols = field(&GTile::cols);
+      char* tile = tile_at_c();
+      const int per = 32 >> p.split_log2;  // rows of each CTA in 32
+      const uint32_t red0 = smem_addr(red), ready0 = smem_addr(&bars.ready), consumed0 = smem_addr(&bars.consumed);
+      for (int r0 = 0; r0 < rows; r0 += 32) {
+        const int here = min(32, rows - r0);
+        const int mine = (here - part + p.split - 1) >> p.split_log2;  // rows part, part + split, … below `here`
+        if (warp == 4 && lane == 0)
+          mbar_expect_tx(ready0, (uint32_t)(mine * p.split) * (uint32_t)((cols + 31) / 32 * 128));
+        if (q * 32 == r0) {
+          // every CTA has read the rows before
+          if (!warp_poll(consumed0, red_phase ^ 1u, abort_flag, kSiteCluster, lane)) return false;
+          const uint32_t owner = (uint32_t)lane & (uint32_t)(p.split - 1);
+          const uint32_t to = map_to_cta(red0 + (uint32_t)(part * per + (lane >> p.split_log2)) * Cf::kRedStride, owner);
+          const uint32_t bar = map_to_cta(ready0, owner);
+#pragma unroll
+          for (int c = 0; c < Cf::kChunks; ++c) {
+            if (c_half + c * 32 < cols) {
+              const float(&s)[32] = sums(c);
+              if (lane < here) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  st_async_f4(to + (uint32_t)(c_half + c * 32 + 4 * i) * 4, bar, s[4 * i], s[4 * i + 1], s[4 * i + 2],
+                              s[4 * i + 3]);
+              }
+              __syncwarp();
+            }
+          }
+        }
+        if (!warp_poll(ready0, red_phase, abort_flag, kSiteCluster, lane)) return false;
+        for (int i = warp - 4; i < mine; i += 8) {
+#pragma unroll
+          for (int h = 0; h < BN / 128; ++h) {  // four columns of each 128 to a lane
+            const int c0 = h * 128 + lane * 4;
+            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              if (j < p.split) {
+                const float4 x = *reinterpret_cast<const float4*>(red + (size_t)(j * per + i) * Cf::kRedStride + c0 * 4);
+                s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+              }
+            }
+            emit4(p, tile + ((int64_t)(r0 + part + (i << p.split_log2)) * p.ldc + c0) * el, s, cols - c0);
+          }
+        }
+        __syncwarp();
+        if (lane < p.split) mbar_arrive_remote(map_to_cta(consumed0, (uint32_t)lane));
+        red_phase ^= 1u;
+      }
+      return true;
+    };
     int acc = 0;
-    uint32_t acc_phase = 0, red_phase = 0;
+    uint32_t acc_phase = 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     while (take(kSiteEpilogue)) {
       // Only the count of accumulations and the scales' places stay in
@@ -839,13 +882,18 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           }
           tc_fence_after();
         }
-        if (p.split > 1) {
-          // every CTA has read the previous tile's partial sums
-          if (!cluster_wait(&bars.consumed, red_phase ^ 1u)) {
-            ok = false;
+        if (G == 1 && p.split > 1) {
+          if (!(ok = share([&](int c) -> const float (&)[32] {
+                  if (fills > 0) {
+                    tmem_ld_32x32b_x32(tm + (uint32_t)(acc * BN + c * 32), v[0]);
+                  } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[0][i] = 0.f;
+                  }
+                  return v[0];
+                })))
             break;
-          }
-        }
+        } else {
 #pragma unroll
         for (int c = 0; c < Cf::kChunks; ++c) {
           if (!warp_ok) break;
@@ -856,11 +904,9 @@ __global__ void __launch_bounds__(kThreadsG, 1)
             for (int i = 0; i < 32; ++i) v[0][i] = 0.f;
           }
           const int ncol = min(32, cols - c * 32);
-          if (row_ok && ncol > 0) {
-            if (p.split > 1) leave(c, v[0]);
-            else emit32(p, row + c * 32 * el, v[0], ncol);
-          }
+          if (row_ok && ncol > 0) emit32(p, row + c * 32 * el, v[0], ncol);
           __syncwarp();
+        }
         }
         if (fills > 0) {
           release(acc);
@@ -871,8 +917,10 @@ __global__ void __launch_bounds__(kThreadsG, 1)
         }
       }
 
-      if (p.split == 1) {
-        if constexpr (Cf::kSums) {
+      if constexpr (Cf::kSums) {
+        if (G == 1 && p.split > 1) {
+          if (!(ok = share([&](int c) -> const float (&)[32] { return v[c]; }))) break;
+        } else {
           const bool row_ok = row_in_tile < field(&GTile::rows);
           const int32_t cols = field(&GTile::cols) - c_half;
           char* row = row_at();
@@ -883,53 +931,6 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           }
           __syncwarp();
         }
-      } else if constexpr (G == 1) {
-        // The cluster's CTAs hold partial sums of one tile. Each leaves its
-        // own in shared memory; CTA r then adds rows r, r + split, … of all
-        // of them, in CTA order, and stores them.
-        if constexpr (Cf::kSums) {
-          if (!cluster_wait(&bars.consumed, red_phase ^ 1u)) {
-            ok = false;
-            break;
-          }
-          if (row_in_tile < field(&GTile::rows)) {
-            const int32_t cols = field(&GTile::cols) - c_half;
-#pragma unroll
-            for (int c = 0; c < Cf::kChunks; ++c)
-              if (c * 32 < cols) leave(c, v[c]);
-          }
-        }
-        cluster_arrive(&bars.ready);
-        if (!cluster_wait(&bars.ready, red_phase)) {
-          ok = false;
-          break;
-        }
-        constexpr int kLaneCols = BN / 32;
-        const int rows = field(&GTile::rows), cols = field(&GTile::cols);
-        char* tile = tile_at_c();
-        for (int r = part + p.split * (warp - 4); r < rows; r += p.split * 8) {
-          const uint32_t src = smem_addr(red) + (uint32_t)r * Cf::kRedStride + (uint32_t)lane * kLaneCols * 4;
-          float s[kLaneCols];
-#pragma unroll
-          for (int i = 0; i < kLaneCols; ++i) s[i] = 0.f;
-          for (int j = 0; j < p.split; ++j) {
-            const uint32_t a = map_to_cta(src, (uint32_t)j);
-            if constexpr (kLaneCols == 4) {
-              const float4 x = ld_cluster_f4(a);
-              s[0] += x.x; s[1] += x.y; s[2] += x.z; s[3] += x.w;
-            } else {
-              const float2 x = ld_cluster_f2(a);
-              s[0] += x.x; s[1] += x.y;
-            }
-          }
-          const int c0 = lane * kLaneCols;
-          char* dst = tile + ((int64_t)r * p.ldc + c0) * el;
-#pragma unroll
-          for (int i = 0; i < kLaneCols; ++i)
-            if (c0 + i < cols) store_out(p, dst + i * el, p.beta ? s[i] + load_out(p, dst + i * el) : s[i]);
-        }
-        cluster_arrive(&bars.consumed);
-        red_phase ^= 1u;
       }
       done();
     }
@@ -1132,35 +1133,65 @@ tbStatus launch_tile(Launch& L, int sms, int dev, cudaStream_t stream) {
                                : launch<kHalf, BN, G>(L, sms, dev, stream);
 }
 
-// Tile and K split. `rows`: mean rows of a group that has any.
+// The kinds that a 128 × 256 tile is built for: with 128 sums per thread the
+// cluster's exchange does not fit into the registers.
+template <>
+tbStatus launch_tile<256, 1>(Launch& L, int sms, int dev, cudaStream_t stream) {
+  return launch<kHalf, 256, 1>(L, sms, dev, stream);
+}
+
+// Tile and K split, by estimated cycles. `rows`: mean rows of a group that has any.
+//
+// One ring fill takes 512 cycles of MMAs whatever the tile's width: a
+// tcgen05.mma of 128 (or a pair's 256) rows was measured at 118–132 cycles for
+// 64, 128 and 256 columns alike, so a narrower tile only lowers the rate. A
+// fill takes longer where its bytes do: 23 bytes a cycle and SM are an SM's
+// share of HBM, 45 the most that one SM was seen to draw while others idle,
+// and L2 feeds an SM 60 bytes a cycle.
+// Storing a tile (16 bytes a cycle and SM) overlaps the next tile's fills.
 tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int dev, cudaStream_t stream) {
   GParams& p = L.p;
   L.rows = rows;
   const int64_t n = p.N;
-  const int64_t kmax = p.k_grouped ? cdiv(p.K, std::max<int64_t>(1, groups)) : p.K;
   const int64_t m = p.k_grouped ? p.M : rows;
   const int64_t busy = p.k_grouped ? groups : std::min<int64_t>(groups, p.M);
-  auto tiles = [&](int bm, int bn) { return busy * cdiv(m, bm) * cdiv(n, bn); };
-  auto bound = [&](int bm, int bn) {
-    return p.k_grouped ? groups * cdiv(p.M, bm) * cdiv(n, bn) : (p.M / bm + std::min<int64_t>(groups, p.M)) * cdiv(n, bn);
+  const int64_t fills = std::max<int64_t>(1, cdiv(p.k_grouped ? cdiv(p.K, std::max<int64_t>(1, groups)) : p.K, 128 / L.el));
+  const int ce = p.c_dtype == TB_F32 ? 4 : 2;
+  double best = 0;
+  int bn = 0, split = 1;
+  bool pair = false;
+  auto consider = [&](bool is_pair, int b, int s) {
+    const int64_t tiles = busy * cdiv(m, is_pair ? 256 : 128) * cdiv(n, b);
+    const int64_t slots = std::max<int64_t>(1, sms / (is_pair ? 2 : s));
+    const double rounds = (double)cdiv(tiles, slots);
+    const double used = std::min(1.0, (double)tiles / (double)slots);
+    const double tile_rows = (double)std::min<int64_t>(m, 128);
+    // bytes of a fill from HBM: B's share of a tile whose other tiles read the same B, and A's rows
+    const double bytes = 128.0 * ((double)(is_pair ? b / 2 : b) / (double)cdiv(m, is_pair ? 256 : 128) + tile_rows / (double)cdiv(n, b));
+    const double near = 128.0 * (is_pair ? 256 : b + tile_rows);  // into the SM, from L2
+    const double fill = std::max(std::max(512.0, near / 60.0), bytes / std::min(45.0, 23.0 / used));
+    const double main = (double)cdiv(fills, s) * fill + (s > 1 ? 300.0 + 300.0 * cdiv((int64_t)tile_rows, 32) : 0.0);
+    const double store = tile_rows * b * ce / 16.0 / (s > 1 ? s : 1);
+    const double cycles = rounds * std::max(main, store) + std::min(main, store);
+    if (!bn || cycles < best) {
+      best = cycles;
+      bn = b;
+      split = s;
+      pair = is_pair;
+    }
   };
-  auto set = [&](int bm, int bn) {
-    p.tiles_m = (int32_t)cdiv(p.M, bm);
-    p.tiles_n = (int32_t)cdiv(n, bn);
-    L.tiles = bound(bm, bn);
-  };
-  p.split = 1;
-  if (m > 128 && 2 * tiles(256, 256) >= sms / 2) {
-    set(256, 256);
-    return launch_tile<256, 2>(L, sms, dev, stream);
-  }
-  // An 8-bit B stored along its columns comes in boxes of 128 columns.
-  const bool wide = (L.el == 1 && !p.b_kmaj) || tiles(128, 128) >= sms;
-  const int64_t have = tiles(128, wide ? 128 : 64);
-  const int64_t fills = cdiv(kmax, 128 / L.el);
-  while (p.split < 8 && have * p.split * 2 <= sms && fills >= 4 * p.split) p.split *= 2;
-  set(128, wide ? 128 : 64);
-  return wide ? launch_tile<128, 1>(L, sms, dev, stream) : launch_tile<64, 1>(L, sms, dev, stream);
+  if (m > 128) consider(true, 256, 1);
+  const bool sums = L.el == 1 || p.c_dtype == TB_F32;
+  for (int b : {256, 128})
+    for (int s = sums && b == 256 ? 16 : 1; s <= 8 && (s == 1 || fills >= 4 * s); s *= 2) consider(false, b, s);
+  p.split = split;
+  p.tiles_m = (int32_t)cdiv(p.M, pair ? 256 : 128);
+  p.tiles_n = (int32_t)cdiv(n, bn);
+  L.tiles = p.k_grouped ? groups * p.tiles_m * p.tiles_n
+                        : (p.M / (pair ? 256 : 128) + std::min<int64_t>(groups, p.M)) * p.tiles_n;
+  return pair        ? launch_tile<256, 2>(L, sms, dev, stream)
+         : bn == 256 ? launch_tile<256, 1>(L, sms, dev, stream)
+                     : launch_tile<128, 1>(L, sms, dev, stream);
 }
 
 int c_bytes(int32_t dt) { return dt == TB_F32 ? 4 : 2; }

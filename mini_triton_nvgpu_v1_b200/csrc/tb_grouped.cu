@@ -154,7 +154,7 @@ struct GParams {
   GScale sa, sb;
   int32_t stages;         // ring depth
   int32_t split, split_log2;  // CTAs per cluster that share a tile's K range (G = 1)
-  int32_t small_rows;     // rows of tmAs's boxes: a K-major A tile of few rows comes in these (G = 1)
+  int32_t small_log2;     // log2 of the rows of tmAs's boxes: a K-major A tile of few rows comes in these (G = 1)
 };
 
 __device__ __forceinline__ int32_t read_offset(const GParams& p, int32_t i) {
@@ -408,44 +408,29 @@ __global__ void __launch_bounds__(kThreadsG, 1)
       tma_prefetch_desc(&tmB);
     }
   }
-  if (warp == 1) {
+  if (G == 2 && warp == 1) {  // (one CTA: the MMA issuer allocates while the first fill is on its way)
     tmem_alloc_g<G>(smem_addr(&bars.tmem_holder), Cf::kTmemCols);
     tmem_relinquish_g<G>();
   }
-  if (warp == 3) {
-    // The scheduler builds the table of tiles meanwhile. What this launch
-    // reads may be written by the kernel before it in the stream, which each
-    // role waits for before its first access to memory (programmatic launch).
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    int32_t before = 0;
-    for (int32_t e0 = 0; e0 < p.groups; e0 += 32) {
-      const int32_t e = e0 + lane;
-      int32_t start = 0, rows = 0;
-      if (e < p.groups) {
-        const int32_t lo = read_offset(p, e), hi = read_offset(p, e + 1);
-        start = lo;
-        rows = max(0, hi - lo);
-        tab.start[e] = start;
-        tab.rows[e] = rows;
-      }
-      int32_t v = (rows + Cf::kBM - 1) / Cf::kBM * p.tiles_n;
-#pragma unroll
-      for (int d = 1; d < 32; d *= 2) {
-        const int32_t o = __shfl_up_sync(0xffffffffu, v, d);
-        if (lane >= d) v += o;
-      }
-      if (e < p.groups) tab.cum[e + 1] = before + v;
-      before += __shfl_sync(0xffffffffu, v, 31);
-    }
-    if (lane == 0) tab.cum[0] = 0;
-    __syncwarp();
+  if (warp == 2) {
+    // Every launch's parameters come into the constant cache anew, a miss of
+    // some hundred cycles to a line: all lines are asked for at once here.
+    uint32_t all = 0;
+    for (int i = lane; i < (int)(sizeof(GParams) / 4); i += 32) all ^= reinterpret_cast<const uint32_t*>(&p)[i];
+    asm volatile("" ::"r"(all));
   }
-  tc_fence_before();
-  if (cluster > 1) cluster_sync();
-  __syncthreads();
-  tc_fence_after();
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const uint32_t tmem_base = bars.tmem_holder;
+  // Barriers (and a pair's TMEM) are there. The scheduler joins when it has the first tile.
+  auto start = [&]() {
+    if constexpr (G == 2) {
+      tc_fence_before();
+      cluster_sync();
+    }
+    __syncthreads();
+    if constexpr (G == 2) tc_fence_after();
+    else if (cluster > 1) cluster_arrive();  // the epilogue waits before it sends to other CTAs
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  };
+
   // The tiles in turn, up to one without columns: take() waits for the next
   // (and says no after the last, or when it gave up), done() gives its slot back.
   int slot = 0;
@@ -473,6 +458,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
   constexpr bool kMoveRegs = Cf::kSums && BN == 256;
   if (warp < 4) {
   if constexpr (kMoveRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+  if (warp != 3) start();
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     // An operand's fill is a few boxes: box j of fill f lies at coordinates
@@ -483,7 +469,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     const int32_t a_fx = a_mn ? 0 : Cf::kKB, a_fy = a_mn ? Cf::kKB : 0;
     const int32_t b_fx = b_mn ? 0 : Cf::kKB, b_fy = b_mn ? Cf::kKB : 0;
     const int32_t b_boxes = b_mn ? Cf::kBnCta / Cf::kMnBox : 1;
-    const int32_t sr = p.small_rows;
+    const int32_t sr = 1 << p.small_log2;
     const uint32_t full0 = smem_addr(&bars.full[0]), empty0 = smem_addr(&bars.empty[0]), fix0 = smem_addr(&bars.fix[0]);
     const uint32_t full0_leader = G == 2 ? map_to_cta(full0, 0) : full0;
     const uint32_t sa0 = smem_addr(sA), sb0 = smem_addr(sB);
@@ -497,7 +483,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
       // K-major A of a tile with few rows: only the small boxes that hold them
       const bool few = G == 1 && !a_mn && g.rows <= 3 * sr;
       const CUtensorMap* const map_a = few ? &tmAs : &tmA;
-      const int32_t a_boxes = a_mn ? 128 / Cf::kMnBox : few ? (g.rows + sr - 1) / sr : 1;
+      const int32_t a_boxes = a_mn ? 128 / Cf::kMnBox : few ? (g.rows + sr - 1) >> p.small_log2 : 1;
       const uint32_t a_step = a_mn ? Cf::kMnBoxBytes : (uint32_t)sr * 128u;
       const int32_t a_jx = a_mn ? Cf::kMnBox : 0, a_jy = a_mn ? 0 : sr;
       const uint32_t bytes = (few ? (uint32_t)a_boxes * a_step : Cf::kABytes) + Cf::kBBytes;
@@ -550,7 +536,12 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     if (lane == 0) bars.issued = issued;
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
+    if constexpr (G == 1) {
+      tmem_alloc_g<G>(smem_addr(&bars.tmem_holder), Cf::kTmemCols);
+      tmem_relinquish_g<G>();
+    }
     if (leader) {
+      const uint32_t tmem_base = *const_cast<volatile uint32_t*>(&bars.tmem_holder);
       const uint32_t idesc = idesc_f16_f32(Cf::kBM, BN, p.a_mn ? 1 : 0, p.b_kmaj ? 0 : 1) | (p.fmt << 7) |
                              (p.fmt << 10);
       // descriptor words: the start address (16-byte units) moves in the low one
@@ -671,17 +662,43 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     }
   } else {
     // ----------------------------------------------------------- scheduler
-    const int32_t tiles = p.k_grouped ? p.groups * p.tiles_m * p.tiles_n : tab.cum[p.groups];
+    // What this launch reads may be written by the kernel before it in the
+    // stream, which each role waits for before its first access to memory
+    // (programmatic launch).
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    int32_t before = 0;
+    for (int32_t e0 = 0; e0 < p.groups; e0 += 32) {
+      const int32_t e = e0 + lane;
+      int32_t lo = 0, rows = 0;
+      if (e < p.groups) {
+        lo = read_offset(p, e);
+        rows = max(0, read_offset(p, e + 1) - lo);
+        tab.start[e] = lo;
+        tab.rows[e] = rows;
+      }
+      int32_t v = (rows + Cf::kBM - 1) / Cf::kBM * p.tiles_n;
+#pragma unroll
+      for (int d = 1; d < 32; d *= 2) {
+        const int32_t o = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += o;
+      }
+      if (e < p.groups) tab.cum[e + 1] = before + v;
+      before += __shfl_sync(0xffffffffu, v, 31);
+    }
+    if (lane == 0) tab.cum[0] = 0;
+    __syncwarp();
+    const int32_t tiles = p.k_grouped ? p.groups * p.tiles_m * p.tiles_n : before;
     int32_t cursor = 0;
     for (int32_t t = first;; t += stride) {
-      GTile g = {};
-      if (t < tiles) g = tile_at<Cf::kBM, BN, Cf::kKB>(p, tab, t, part, cursor, lane);
+      GTile tile = {};
+      if (t < tiles) tile = tile_at<Cf::kBM, BN, Cf::kKB>(p, tab, t, part, cursor, lane);
+      if (t == first) start();
       if (!warp_wait(smem_addr(&bars.tile_empty[slot]), slot_phase ^ 1u, abort_flag, kSiteScheduler, lane)) break;
       if (lane == 0) {
-        bars.tile[slot] = g;
+        bars.tile[slot] = tile;
         mbar_arrive(smem_addr(&bars.tile_full[slot]));
       }
-      if (t >= tiles) break;  // the tile without columns
+      if (t >= tiles) break;  // that was the tile without columns
       if (++slot == kTileSlots) {
         slot = 0;
         slot_phase ^= 1u;
@@ -690,12 +707,19 @@ __global__ void __launch_bounds__(kThreadsG, 1)
   }
   } else {
     if constexpr (kMoveRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    start();
     // ------------------------------------------------------------ epilogue
     const int q = warp & 3;               // TMEM lane quarter
     const int half = (warp - 4) >> 2;     // column half
     const int row_in_tile = (int)rank * 128 + q * 32 + lane;
     const int c_half = half * Cf::kHalfCols;
-    const uint32_t tm = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)c_half;
+    // this warp's lanes and columns of TMEM (one CTA: known once an accumulation is complete)
+    const uint32_t tm_off = ((uint32_t)(q * 32) << 16) + (uint32_t)c_half;
+    const uint32_t tm_pair = G == 2 ? bars.tmem_holder + tm_off : 0u;
+    auto tm = [&]() {
+      if constexpr (G == 2) return tm_pair;
+      else return *const_cast<volatile uint32_t*>(&bars.tmem_holder) + tm_off;
+    };
     const int el = p.c_dtype == TB_F32 ? 4 : 2;
     const uint32_t tempty0 = G == 2 ? map_to_cta(smem_addr(&bars.tempty[0]), 0) : smem_addr(&bars.tempty[0]);
     auto release = [&](int acc) {
@@ -774,6 +798,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     };
     int acc = 0;
     uint32_t acc_phase = 0;
+    if (G == 1 && cluster > 1) cluster_wait();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     while (take(kSiteEpilogue)) {
       // Only the count of accumulations and the scales' places stay in
@@ -840,7 +865,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           tc_fence_after();
           if (warp_ok) {
             uint32_t w[2][32];
-            const uint32_t ta = tm + (uint32_t)(acc * BN);
+            const uint32_t ta = tm() + (uint32_t)(acc * BN);
             const uint64_t x2 = pack_f32x2(x, x);
             tmem_ld_32x32b_x32_issue(ta, w[0]);
 #pragma unroll
@@ -888,7 +913,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
         if (G == 1 && p.split > 1) {
           if (!(ok = share([&](int c) -> const float (&)[32] {
                   if (fills > 0) {
-                    tmem_ld_32x32b_x32(tm + (uint32_t)(acc * BN + c * 32), v[0]);
+                    tmem_ld_32x32b_x32(tm() + (uint32_t)(acc * BN + c * 32), v[0]);
                   } else {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[0][i] = 0.f;
@@ -901,7 +926,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
         for (int c = 0; c < Cf::kChunks; ++c) {
           if (!warp_ok) break;
           if (fills > 0) {
-            tmem_ld_32x32b_x32(tm + (uint32_t)(acc * BN + c * 32), v[0]);
+            tmem_ld_32x32b_x32(tm() + (uint32_t)(acc * BN + c * 32), v[0]);
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[0][i] = 0.f;
@@ -937,6 +962,9 @@ __global__ void __launch_bounds__(kThreadsG, 1)
       }
       done();
     }
+    // Nothing of another CTA is on its way to this one any more (a cluster
+    // barrier at the end took 1200 cycles).
+    if (G == 1 && p.split > 1 && ok) warp_poll(smem_addr(&bars.consumed), red_phase ^ 1u, abort_flag, kSiteCluster, lane);
   }
 
   __syncthreads();
@@ -955,10 +983,16 @@ __global__ void __launch_bounds__(kThreadsG, 1)
       }
     }
   }
-  if (cluster > 1) cluster_sync();
+  if (G == 2) {
+    cluster_sync();
+  } else if (cluster > 1 && *abort_flag) {
+    // given up: no CTA leaves while another one may still send to it
+    if (warp < 4) cluster_wait();
+    cluster_sync();
+  }
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc_g<G>(tmem_base, Cf::kTmemCols);
+    tmem_dealloc_g<G>(bars.tmem_holder, Cf::kTmemCols);
   }
 }
 
@@ -1085,8 +1119,8 @@ tbStatus launch(Launch& L, int sms, int dev, cudaStream_t stream) {
   CUtensorMap ta, tas, tb_;
   std::memset(&tas, 0, sizeof(tas));
   tbStatus st = encode(&ta, 2, L.a, L.el, L.bf16, p.a_mn ? Cf::kMnBox : Cf::kKB, p.a_mn ? Cf::kKB : 128, "A");
-  p.small_rows = L.rows <= 16 ? 8 : 32;
-  if (st == TB_OK && !p.a_mn && G == 1) st = encode(&tas, 2, L.a, L.el, L.bf16, Cf::kKB, (uint32_t)p.small_rows, "A");
+  p.small_log2 = L.rows <= 16 ? 3 : 5;
+  if (st == TB_OK && !p.a_mn && G == 1) st = encode(&tas, 2, L.a, L.el, L.bf16, Cf::kKB, 1u << p.small_log2, "A");
   if (st == TB_OK)
     st = encode(&tb_, 3, L.b, L.el, L.bf16, p.b_kmaj ? Cf::kKB : Cf::kMnBox, p.b_kmaj ? Cf::kBnCta : Cf::kKB, "B");
   if (st != TB_OK) return st;

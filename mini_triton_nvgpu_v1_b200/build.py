@@ -1,7 +1,8 @@
 """Builds the in-tree shared library ``libtbgemm.so`` (the C ABI of
-``include/tb_gemm.h``) with nvcc for sm_100a.
+``include/tb_gemm.h``) with nvcc for sm_100a, and ``_tbtorch.so`` (the calls of
+``grouped.py`` on torch tensors) with g++ against torch's headers.
 
-The library is written next to this file so it travels with the source tree;
+Both are written next to this file so they travel with the source tree;
 ``python -m mini_triton_nvgpu_v1_b200.build`` rebuilds it.
 """
 from __future__ import annotations
@@ -16,6 +17,7 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libtbgemm.so"
+TORCH_LIB = PKG / "_tbtorch.so"
 
 SOURCES = ["tb_plan.cpp", "tb_dynamic.cpp", "tb_shard.cpp", "tb_launch.cu", "tb_grouped.cu", "tb_quantize.cu", "tb_peer.cu", "tb_nccl.cpp"]
 HEADERS = ["tb_plan.h", "tb_mapping.h", "tb_sm100.cuh", "tb_wait.cuh"]
@@ -44,11 +46,31 @@ def _run(cmd: list[str], verbose: bool) -> str:
     return r.stdout + r.stderr
 
 
+def build_torch(force: bool = False, verbose: bool = False) -> Path:
+    """``_tbtorch.so``: torch is only looked up here, not imported."""
+    import importlib.util
+    import sysconfig
+    src = CSRC / "tb_torch.cpp"
+    if not force and not _stale(TORCH_LIB, [src, ROOT / "include" / "tb_gemm.h", Path(__file__)]):
+        return TORCH_LIB
+    torch = Path(importlib.util.find_spec("torch").origin).parent
+    cuda = Path(nvcc()).resolve().parents[1]
+    tmp = TORCH_LIB.with_suffix(".so.tmp")
+    _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wno-unknown-pragmas",
+          "-I", sysconfig.get_paths()["include"], "-I", str(torch / "include"),
+          "-I", str(torch / "include" / "torch" / "csrc" / "api" / "include"), "-I", str(cuda / "include"),
+          str(src), "-o", str(tmp), "-L", str(torch / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"],
+         verbose)
+    os.replace(tmp, TORCH_LIB)
+    return TORCH_LIB
+
+
 def build(force: bool = False, verbose: bool = False, ptxas_v: bool = False) -> Path:
     """Compiles each source to an object (in parallel, under ``_build/``) and
     links ``libtbgemm.so``; skipped when the library is newer than every input."""
     inputs = [CSRC / s for s in SOURCES] + [CSRC / h for h in HEADERS] + [ROOT / "include" / "tb_gemm.h",
                                                                            Path(__file__)]
+    build_torch(force, verbose)
     if not force and not _stale(LIB, inputs):
         return LIB
     objdir = ROOT / "_build"

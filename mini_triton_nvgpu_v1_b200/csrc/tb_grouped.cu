@@ -997,19 +997,43 @@ __global__ void __launch_bounds__(kThreadsG, 1)
 }
 
 // Copies rows of `row_bytes` to rows of ld_dst bytes (a multiple of 16), the
-// rest of each row zero: operands whose rows TMA cannot address.
+// rest of each row zero: operands whose rows TMA cannot address. HBM bound: a
+// lane reads the one or two aligned 16-byte words that hold its 16 bytes (they
+// lie in the rows' own allocation: no word without a byte of the row is
+// touched) and shifts them into place. A warp takes a row at a time.
 __global__ void __launch_bounds__(256)
     tb_grouped_pack_kernel(const uint8_t* __restrict__ src, int64_t ld_src, int64_t batch_src, uint8_t* __restrict__ dst,
                            int64_t ld_dst, int64_t batch_dst, int64_t rows, int64_t row_bytes) {
   src += (int64_t)blockIdx.z * batch_src;
   dst += (int64_t)blockIdx.z * batch_dst;
-  const int64_t words = ld_dst / 16;
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    for (int64_t w = threadIdx.x; w < words; w += blockDim.x) {
-      __align__(16) uint8_t b[16];
+  const int lane = threadIdx.x % 32;
+  for (int64_t r = blockIdx.x * 8 + threadIdx.x / 32; r < rows; r += (int64_t)gridDim.x * 8) {
+    const uint8_t* row = src + r * ld_src;
+    for (int64_t w = lane; w * 16 < ld_dst; w += 32) {
+      const int64_t left = row_bytes - w * 16;  // bytes of the row from here on
+      uint32_t v[5] = {0, 0, 0, 0, 0};
+      if (left > 0) {
+        const uint8_t* at = row + w * 16;
+        const int shift = (int)(reinterpret_cast<uintptr_t>(at) & 15);
+        const uint4* word = reinterpret_cast<const uint4*>(at - shift);
+        const uint4 lo = __ldg(word);
+        uint4 hi = make_uint4(0, 0, 0, 0);
+        if (shift + (left < 16 ? left : 16) > 16) hi = __ldg(word + 1);
+        const uint32_t x[9] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w, 0};
+        const int first = shift >> 2, bits = (shift & 3) * 8;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) b[i] = w * 16 + i < row_bytes ? src[r * ld_src + w * 16 + i] : 0;
-      *reinterpret_cast<uint4*>(dst + r * ld_dst + w * 16) = *reinterpret_cast<const uint4*>(b);
+        for (int i = 0; i < 5; ++i)
+#pragma unroll
+          for (int f = 0; f < 4; ++f)
+            if (first == f) v[i] = x[i + f];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[i] = __funnelshift_r(v[i], v[i + 1], bits);
+          const int64_t here = left - 4 * i;  // bytes of the row in this word
+          if (here < 4) v[i] = here <= 0 ? 0u : v[i] & (0xffffffffu >> (32 - 8 * (int)here));
+        }
+      }
+      *reinterpret_cast<uint4*>(dst + r * ld_dst + w * 16) = make_uint4(v[0], v[1], v[2], v[3]);
     }
   }
 }
@@ -1051,6 +1075,7 @@ tbStatus current_device(int* dev, int* sms) {
   return TB_OK;
 }
 
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 bool al(const void* p, int64_t n) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)n == 0; }
 
 // One operand as the kernel reads it: `rows` rows of `cols` contiguous
@@ -1070,7 +1095,7 @@ struct Operand {
 tbStatus pack(Operand* o, int el, void* ws, cudaStream_t stream) {
   if (o->batch > 65535) return tb_fail(TB_ERR_UNSUPPORTED, "too many groups to repack");
   const int64_t ld = o->packed_ld(el);
-  const unsigned gx = (unsigned)std::min<int64_t>(std::max<int64_t>(1, o->rows), 4096);
+  const unsigned gx = (unsigned)std::min<int64_t>(std::max<int64_t>(1, cdiv(o->rows, 8)), 4096);
   tb_grouped_pack_kernel<<<dim3(gx, 1, (unsigned)o->batch), 256, 0, stream>>>(
       static_cast<const uint8_t*>(o->p), o->ld * el, o->stride * el, static_cast<uint8_t*>(ws), ld, ld * o->rows,
       o->rows, o->cols * el);
@@ -1158,8 +1183,6 @@ tbStatus launch(Launch& L, int sms, int dev, cudaStream_t stream) {
   if (e != cudaSuccess) return tb_fail(TB_ERR_CUDA, std::string("tb_grouped launch: ") + cudaGetErrorString(e));
   return TB_OK;
 }
-
-int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // The kind of a tile's kernel, by the operands' and the output's types.
 template <int BN, int G>

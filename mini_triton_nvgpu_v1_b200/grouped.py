@@ -36,19 +36,29 @@ _HALF = {torch.float16: TB_F16, torch.bfloat16: TB_BF16}
 _OUT = {torch.float32: TB_F32, torch.float16: TB_F16, torch.bfloat16: TB_BF16}
 _FP8 = torch.float8_e4m3fn
 
-# What a call's shapes, strides and types decide, by those (never by address).
-_SETUP: dict = {}
+
+def _load_calls():
+    """Module _tbtorch (csrc/tb_torch.cpp), given the library's entry points."""
+    try:
+        from . import _tbtorch
+    except ImportError as e:
+        raise ImportError("_tbtorch.so is missing or of another torch: build it with "
+                          "`python -m mini_triton_nvgpu_v1_b200.build`") from e
+    _tbtorch.library(*(C.cast(f, C.c_void_p).value for f in (
+        _lib.tb_grouped_matmul, _lib.tb_grouped_matmul_wgrad, _lib.tb_quantize_blocks, _lib.tb_matmul_blockscaled,
+        _lib.tb_grouped_matmul_blockscaled)))
+    return _tbtorch
+
+
+# Calls like an earlier one, by the tensors' sizes, strides, types and device:
+# _call0(op, tensors..., x, y) is 0 when it ran them, -1 when it knows no such call.
+_calls = _load_calls()
+_call0, _remember = _calls.call, _calls.remember
+_ROWS, _WGRAD, _QUANTIZE, _BYTES, _ROWS_BYTES = range(5)
 
 
 def _bad(message: str, code: int = TB_ERR_INVALID_ARGUMENT):
     return TBError(code, message)
-
-
-def _keep(key, made):
-    if len(_SETUP) > 1024:
-        _SETUP.clear()
-    _SETUP[key] = made
-    return made
 
 
 def _same_device(**tensors) -> int:
@@ -131,31 +141,31 @@ def _scratch(need: int, workspace, device, stream):
 
 def _call(dev: int, stream, fn, *args) -> None:
     """fn(*args, stream) with `dev` current."""
-    sp = stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(dev)
-    if torch._C._cuda_getDevice() == dev:
-        code = fn(*args, sp or None)
+    s = stream if stream is not None else torch.cuda.current_stream(dev)
+    if torch.cuda.current_device() == dev:
+        code = fn(*args, s.cuda_stream or None)
     else:
         with torch.cuda.device(dev):
-            code = fn(*args, sp or None)
-    if code:
-        _check(code)
+            code = fn(*args, s.cuda_stream or None)
+    _check(code)
 
 
-def _setup_grouped(key, A, B, Cm, offsets, beta, fp8_scales):
+def _setup_grouped(A, B, Cm, offsets, beta, eight_bit: bool):
+    """(device, desc, lda, ldb, stride_b, ldc, whether every row begins on 16 bytes if the bases do)."""
     if A.dim() != 2 or B.dim() != 3 or Cm.dim() != 2:
         raise _bad("grouped products take A [rows, k], B [groups, k, n] and C [rows, n]")
     rows, k = A.shape
     groups, kb, n = B.shape
     if kb != k or tuple(Cm.shape) != (rows, n):
         raise _bad("operand shapes disagree: A [rows, k], B [groups, k, n], C [rows, n]")
-    if fp8_scales is None:
-        if A.dtype not in _HALF or B.dtype != A.dtype:
-            raise _bad("A and B must both be f16 or both be bf16")
-        ab = _HALF[A.dtype]
-    else:
+    if eight_bit:
         if A.dtype != _FP8 or B.dtype != _FP8:
             raise _bad("A and B must be float8_e4m3fn")
         ab = TB_E4M3
+    else:
+        if A.dtype not in _HALF or B.dtype != A.dtype:
+            raise _bad("A and B must both be f16 or both be bf16")
+        ab = _HALF[A.dtype]
     if Cm.dtype not in _OUT:
         raise _bad("C must be f32, f16 or bf16")
     long_ = _check_offsets(offsets, groups)
@@ -163,14 +173,12 @@ def _setup_grouped(key, A, B, Cm, offsets, beta, fp8_scales):
     lda, ldc = _rows(A, "A"), _rows(Cm, "C")
     d = _desc(groups, rows, n, k, ab, _OUT[Cm.dtype], beta, False, b_col, long_)
     stride_b = _batch(B, "B")
-    el = 1 if fp8_scales is not None else 2
+    el = 1 if eight_bit else 2
     even = not (lda * el % 16 or ldb * el % 16 or stride_b * el % 16)
     return d, lda, ldb, stride_b, ldc, even
 
 
-def _need(even, d, A, lda, B, ldb, stride_b) -> int:
-    if even and not (A.data_ptr() | B.data_ptr()) & 15:
-        return 0
+def _need(d, A, lda, B, ldb, stride_b) -> int:
     return _lib.tb_grouped_matmul_workspace_bytes(C.byref(d), A.data_ptr(), lda, B.data_ptr(), ldb, stride_b)
 
 
@@ -180,16 +188,19 @@ def grouped_matmul(A, B, Cm, offsets, *, beta: int = 1, workspace=None, stream=N
     bf16 (B row-major, or a transposed view of weights kept as n × k), C
     [rows, n] f32, f16 or bf16, offsets groups + 1 int32 or int64 on the
     device. Rows outside every group keep what C held. Returns C."""
-    key = ("g", A.shape, B.shape, Cm.shape, A.stride(), B.stride(), Cm.stride(), A.dtype, B.dtype, Cm.dtype,
-           A.device, B.device, Cm.device, offsets.shape, offsets.stride(), offsets.dtype, offsets.device, beta)
-    hit = _SETUP.get(key)
-    if hit is None:
-        dev = _same_device(A=A, B=B, C=Cm, offsets=offsets)
-        hit = _keep(key, (dev, *_setup_grouped(key, A, B, Cm, offsets, beta, None)))
-    dev, d, lda, ldb, stride_b, ldc, even = hit
-    ws, nbytes, _kept = _scratch(_need(even, d, A, lda, B, ldb, stride_b), workspace, Cm.device, stream)
+    if stream is None:
+        code = _call0(_ROWS, A, B, Cm, offsets, beta, 0)
+        if code >= 0:
+            if code:
+                _check(code)
+            return Cm
+    dev = _same_device(A=A, B=B, C=Cm, offsets=offsets)
+    d, lda, ldb, stride_b, ldc, even = _setup_grouped(A, B, Cm, offsets, beta, False)
+    ws, nbytes, _kept = _scratch(_need(d, A, lda, B, ldb, stride_b), workspace, Cm.device, stream)
     _call(dev, stream, _lib.tb_grouped_matmul, d, A.data_ptr(), lda, B.data_ptr(), ldb, stride_b, Cm.data_ptr(), ldc,
           offsets.data_ptr(), ws, nbytes)
+    if even:
+        _remember(_ROWS, A, B, Cm, offsets, beta, 0, d, (lda, ldb, stride_b, ldc), None, None)
     return Cm
 
 
@@ -198,32 +209,33 @@ def grouped_matmul_wgrad(A, D, G, offsets, *, beta: int = 1, workspace=None, str
     weights of :func:`grouped_matmul` from the gradient D of its output.
     A [rows, k] and D [rows, n] f16 or bf16, G [groups, k, n] f32, f16 or
     bf16. A group without rows gets beta·G[e]. Returns G."""
-    key = ("w", A.shape, D.shape, G.shape, A.stride(), D.stride(), G.stride(), A.dtype, D.dtype, G.dtype,
-           A.device, D.device, G.device, offsets.shape, offsets.stride(), offsets.dtype, offsets.device, beta)
-    hit = _SETUP.get(key)
-    if hit is None:
-        dev = _same_device(A=A, D=D, G=G, offsets=offsets)
-        if A.dim() != 2 or D.dim() != 2 or G.dim() != 3:
-            raise _bad("the weight gradient takes A [rows, k], D [rows, n] and G [groups, k, n]")
-        rows, k = A.shape
-        groups, n = G.shape[0], D.shape[1]
-        if D.shape[0] != rows or tuple(G.shape) != (groups, k, n):
-            raise _bad("operand shapes disagree: A [rows, k], D [rows, n], G [groups, k, n]")
-        if A.dtype not in _HALF or D.dtype != A.dtype:
-            raise _bad("A and D must both be f16 or both be bf16")
-        if G.dtype not in _OUT:
-            raise _bad("G must be f32, f16 or bf16")
-        long_ = _check_offsets(offsets, groups)
-        lda, ldd, ldg = _rows(A, "A"), _rows(D, "D"), _rows(G, "G")
-        d = _desc(groups, rows, n, k, _HALF[A.dtype], _OUT[G.dtype], beta, False, False, long_)
-        hit = _keep(key, (dev, d, lda, ldd, ldg, _batch(G, "G"), not (lda * 2 % 16 or ldd * 2 % 16)))
-    dev, d, lda, ldd, ldg, stride_g, even = hit
-    need = 0
-    if not even or (A.data_ptr() | D.data_ptr()) & 15:
-        need = _lib.tb_grouped_matmul_wgrad_workspace_bytes(C.byref(d), A.data_ptr(), lda, D.data_ptr(), ldd)
+    if stream is None:
+        code = _call0(_WGRAD, A, D, G, offsets, beta, 0)
+        if code >= 0:
+            if code:
+                _check(code)
+            return G
+    dev = _same_device(A=A, D=D, G=G, offsets=offsets)
+    if A.dim() != 2 or D.dim() != 2 or G.dim() != 3:
+        raise _bad("the weight gradient takes A [rows, k], D [rows, n] and G [groups, k, n]")
+    rows, k = A.shape
+    groups, n = G.shape[0], D.shape[1]
+    if D.shape[0] != rows or tuple(G.shape) != (groups, k, n):
+        raise _bad("operand shapes disagree: A [rows, k], D [rows, n], G [groups, k, n]")
+    if A.dtype not in _HALF or D.dtype != A.dtype:
+        raise _bad("A and D must both be f16 or both be bf16")
+    if G.dtype not in _OUT:
+        raise _bad("G must be f32, f16 or bf16")
+    long_ = _check_offsets(offsets, groups)
+    lda, ldd, ldg = _rows(A, "A"), _rows(D, "D"), _rows(G, "G")
+    stride_g = _batch(G, "G")
+    d = _desc(groups, rows, n, k, _HALF[A.dtype], _OUT[G.dtype], beta, False, False, long_)
+    need = _lib.tb_grouped_matmul_wgrad_workspace_bytes(C.byref(d), A.data_ptr(), lda, D.data_ptr(), ldd)
     ws, nbytes, _kept = _scratch(need, workspace, G.device, stream)
     _call(dev, stream, _lib.tb_grouped_matmul_wgrad, d, A.data_ptr(), lda, D.data_ptr(), ldd, G.data_ptr(), ldg,
           stride_g, offsets.data_ptr(), ws, nbytes)
+    if not (lda * 2 % 16 or ldd * 2 % 16):
+        _remember(_WGRAD, A, D, G, offsets, beta, 0, d, (lda, ldd, ldg, stride_g), None, None)
     return G
 
 
@@ -239,47 +251,47 @@ def quantize_fp8(X, Q=None, S=None, *, block=(1, 128), stream=None):
     not given is made with rows that begin on 16-byte boundaries, as the
     8-bit products read them without a copy. Returns (Q, S)."""
     br, bc = block
+    if Q is not None and S is not None and stream is None:
+        code = _call0(_QUANTIZE, X, Q, S, br, bc)
+        if code >= 0:
+            if code:
+                _check(code)
+            return Q, S
     if (br, bc) not in ((1, 128), (128, 1), (128, 128)):
         raise _bad("blocks are (1, 128), (128, 1) or (128, 128)")
     if X.dim() not in (2, 3):
         raise _bad("X must be [rows, cols] or [batch, rows, cols]")
     if not X.is_cuda:
         raise _bad("X must be a CUDA tensor")
+    if X.dtype not in _OUT:
+        raise _bad("X must be f32, f16 or bf16")
+    rows, cols = X.shape[-2:]
     if Q is None:
-        rows, cols = X.shape[-2:]
         Q = torch.empty(*X.shape[:-1], (cols + 15) // 16 * 16, dtype=torch.uint8, device=X.device).view(_FP8)
         Q = Q[..., :cols]
         if stream is not None:
             Q.record_stream(stream)
     if S is None:
-        S = torch.empty(*X.shape[:-2], -(-X.shape[-2] // br), -(-X.shape[-1] // bc), device=X.device,
-                        dtype=torch.float32)
+        S = torch.empty(*X.shape[:-2], -(-rows // br), -(-cols // bc), device=X.device, dtype=torch.float32)
         if stream is not None:
             S.record_stream(stream)
-    key = ("q", X.shape, Q.shape, S.shape, X.stride(), Q.stride(), S.stride(), X.dtype, Q.dtype, S.dtype,
-           X.device, Q.device, S.device, br, bc)
-    hit = _SETUP.get(key)
-    if hit is None:
-        dev = _same_device(X=X, Q=Q, S=S)
-        if X.dtype not in _OUT:
-            raise _bad("X must be f32, f16 or bf16")
-        if Q.dtype != _FP8 or Q.shape != X.shape:
-            raise _bad("Q must be float8_e4m3fn of X's shape")
-        rows, cols = X.shape[-2:]
-        if S.dtype != torch.float32 or tuple(S.shape) != (*X.shape[:-2], -(-rows // br), -(-cols // bc)):
-            raise _bad("S must be f32 with one entry for each block")
-        d = _capi.tb_quantize_desc()
-        d.batch, d.rows, d.cols = (X.shape[0] if X.dim() == 3 else 1), rows, cols
-        d.block_rows, d.block_cols, d.x_dtype = br, bc, _OUT[X.dtype]
-        batched = X.dim() == 3
-        if batched:
-            _batch(Q, "Q")
-            _batch(S, "S")
-        hit = _keep(key, (dev, d, _rows(X, "X"), X.stride(0) if batched else 0, _rows(Q, "Q"),
-                          Q.stride(0) if batched else 0, S.stride(0) if batched else 0, S.stride(-2), S.stride(-1)))
-    dev, d, ldx, bx, ldq, bq, bs, s_row, s_col = hit
-    _call(dev, stream, _lib.tb_quantize_blocks, d, X.data_ptr(), ldx, bx, Q.data_ptr(), ldq, bq, S.data_ptr(), bs,
-          s_row, s_col)
+    dev = _same_device(X=X, Q=Q, S=S)
+    if Q.dtype != _FP8 or Q.shape != X.shape:
+        raise _bad("Q must be float8_e4m3fn of X's shape")
+    if S.dtype != torch.float32 or tuple(S.shape) != (*X.shape[:-2], -(-rows // br), -(-cols // bc)):
+        raise _bad("S must be f32 with one entry for each block")
+    batched = X.dim() == 3
+    d = _capi.tb_quantize_desc()
+    d.batch, d.rows, d.cols = (X.shape[0] if batched else 1), rows, cols
+    d.block_rows, d.block_cols, d.x_dtype = br, bc, _OUT[X.dtype]
+    if batched:
+        _batch(Q, "Q")
+        _batch(S, "S")
+    ints = (_rows(X, "X"), X.stride(0) if batched else 0, _rows(Q, "Q"), Q.stride(0) if batched else 0,
+            S.stride(0) if batched else 0, S.stride(-2), S.stride(-1))
+    _call(dev, stream, _lib.tb_quantize_blocks, d, X.data_ptr(), *ints[:2], Q.data_ptr(), *ints[2:4], S.data_ptr(),
+          *ints[4:])
+    _remember(_QUANTIZE, X, Q, S, br, bc, d, ints, None, None)
     return Q, S
 
 
@@ -290,6 +302,7 @@ def _scales(s, name: str, mn: int, k: int, mn_axis: int, k_axis: int, lead: tupl
     if s.shape[k_axis] != _blocks(k) or per not in (mn, _blocks(mn)):
         raise _bad(f"{name} must hold one scale for 1 or 128 rows or columns and 128 elements along k")
     sc = _capi.tb_scales()
+    sc.ptr = s.data_ptr()
     sc.stride_group = s.stride(0) if lead else 0
     sc.stride_mn, sc.stride_k = s.stride(mn_axis), s.stride(k_axis)
     sc.block = 1 if per == mn else 128
@@ -302,40 +315,34 @@ def matmul_fp8(A, SA, B, SB, Cm, *, beta: int = 1, workspace=None, stream=None):
     view; SA f32 [m or ceil(m / 128), ceil(k / 128)]; SB f32 [ceil(k / 128),
     n or ceil(n / 128)]; C [m, n] f32, f16 or bf16. The sum over a block and
     over the blocks is in f32. Returns C."""
-    key = ("f", A.shape, B.shape, Cm.shape, SA.shape, SB.shape, A.stride(), B.stride(), Cm.stride(), SA.stride(),
-           SB.stride(), A.dtype, B.dtype, Cm.dtype, SA.dtype, SB.dtype, A.device, B.device, Cm.device, SA.device,
-           SB.device, beta)
-    hit = _SETUP.get(key)
-    if hit is None:
-        dev = _same_device(A=A, SA=SA, B=B, SB=SB, C=Cm)
-        if A.dim() != 2 or B.dim() != 2 or Cm.dim() != 2:
-            raise _bad("matmul_fp8 takes A [m, k], B [k, n] and C [m, n]")
-        m, k = A.shape
-        n = B.shape[1]
-        if B.shape[0] != k or tuple(Cm.shape) != (m, n):
-            raise _bad("operand shapes disagree: A [m, k], B [k, n], C [m, n]")
-        if A.dtype != _FP8 or B.dtype != _FP8:
-            raise _bad("A and B must be float8_e4m3fn")
-        if Cm.dtype not in _OUT:
-            raise _bad("C must be f32, f16 or bf16")
-        a_col, lda = _either(A, "A")
-        b_col, ldb = _either(B, "B")
-        d = _desc(1, m, n, k, TB_E4M3, _OUT[Cm.dtype], beta, a_col, b_col, 0)
-        hit = _keep(key, (dev, d, lda, ldb, _rows(Cm, "C"), _scales(SA, "SA", m, k, 0, 1, ()),
-                          _scales(SB, "SB", n, k, 1, 0, ()), not (lda % 16 or ldb % 16)))
-    dev, d, lda, ldb, ldc, sa, sb, even = hit
-    ws, nbytes, _kept = _scratch(_need(even, d, A, lda, B, ldb, 0), workspace, Cm.device, stream)
-    sa, sb = _at(sa, SA), _at(sb, SB)
+    if stream is None:
+        code = _call0(_BYTES, A, SA, B, SB, Cm, beta, 0)
+        if code >= 0:
+            if code:
+                _check(code)
+            return Cm
+    dev = _same_device(A=A, SA=SA, B=B, SB=SB, C=Cm)
+    if A.dim() != 2 or B.dim() != 2 or Cm.dim() != 2:
+        raise _bad("matmul_fp8 takes A [m, k], B [k, n] and C [m, n]")
+    m, k = A.shape
+    n = B.shape[1]
+    if B.shape[0] != k or tuple(Cm.shape) != (m, n):
+        raise _bad("operand shapes disagree: A [m, k], B [k, n], C [m, n]")
+    if A.dtype != _FP8 or B.dtype != _FP8:
+        raise _bad("A and B must be float8_e4m3fn")
+    if Cm.dtype not in _OUT:
+        raise _bad("C must be f32, f16 or bf16")
+    a_col, lda = _either(A, "A")
+    b_col, ldb = _either(B, "B")
+    ldc = _rows(Cm, "C")
+    d = _desc(1, m, n, k, TB_E4M3, _OUT[Cm.dtype], beta, a_col, b_col, 0)
+    sa, sb = _scales(SA, "SA", m, k, 0, 1, ()), _scales(SB, "SB", n, k, 1, 0, ())
+    ws, nbytes, _kept = _scratch(_need(d, A, lda, B, ldb, 0), workspace, Cm.device, stream)
     _call(dev, stream, _lib.tb_matmul_blockscaled, d, A.data_ptr(), lda, sa, B.data_ptr(), ldb, sb, Cm.data_ptr(), ldc,
           ws, nbytes)
+    if not (lda % 16 or ldb % 16):
+        _remember(_BYTES, A, SA, B, SB, Cm, beta, 0, d, (lda, ldb, ldc), sa, sb)
     return Cm
-
-
-def _at(scales, tensor) -> _capi.tb_scales:
-    """The layout `scales` at a tensor's address (a copy: threads share the layout)."""
-    s = _capi.tb_scales.from_buffer_copy(scales)
-    s.ptr = tensor.data_ptr()
-    return s
 
 
 def grouped_matmul_fp8(A, SA, B, SB, Cm, offsets, *, beta: int = 1, workspace=None, stream=None):
@@ -343,22 +350,22 @@ def grouped_matmul_fp8(A, SA, B, SB, Cm, offsets, *, beta: int = 1, workspace=No
     A [rows, k] with SA [rows, ceil(k / 128)], B [groups, k, n] (row-major, or a
     transposed view) with SB [groups, ceil(k / 128), n or ceil(n / 128)].
     Returns C."""
-    key = ("h", A.shape, B.shape, Cm.shape, SA.shape, SB.shape, A.stride(), B.stride(), Cm.stride(), SA.stride(),
-           SB.stride(), A.dtype, B.dtype, Cm.dtype, SA.dtype, SB.dtype, A.device, B.device, Cm.device, SA.device,
-           SB.device, offsets.shape, offsets.stride(), offsets.dtype, offsets.device, beta)
-    hit = _SETUP.get(key)
-    if hit is None:
-        dev = _same_device(A=A, SA=SA, B=B, SB=SB, C=Cm, offsets=offsets)
-        made = _setup_grouped(key, A, B, Cm, offsets, beta, (SA, SB))
-        rows, k = A.shape
-        groups, _, n = B.shape
-        if SA.dim() != 2 or SA.shape[0] != rows:
-            raise _bad("SA must hold a scale for each row of A and 128 elements along k")
-        hit = _keep(key, (dev, *made, _scales(SA, "SA", rows, k, 0, 1, ()),
-                          _scales(SB, "SB", n, k, 2, 1, (groups,))))
-    dev, d, lda, ldb, stride_b, ldc, even, sa, sb = hit
-    ws, nbytes, _kept = _scratch(_need(even, d, A, lda, B, ldb, stride_b), workspace, Cm.device, stream)
-    sa, sb = _at(sa, SA), _at(sb, SB)
+    if stream is None:
+        code = _call0(_ROWS_BYTES, A, SA, B, SB, Cm, offsets, beta, 0)
+        if code >= 0:
+            if code:
+                _check(code)
+            return Cm
+    dev = _same_device(A=A, SA=SA, B=B, SB=SB, C=Cm, offsets=offsets)
+    d, lda, ldb, stride_b, ldc, even = _setup_grouped(A, B, Cm, offsets, beta, True)
+    rows, k = A.shape
+    groups, _, n = B.shape
+    if SA.dim() != 2 or SA.shape[0] != rows:
+        raise _bad("SA must hold a scale for each row of A and 128 elements along k")
+    sa, sb = _scales(SA, "SA", rows, k, 0, 1, ()), _scales(SB, "SB", n, k, 2, 1, (groups,))
+    ws, nbytes, _kept = _scratch(_need(d, A, lda, B, ldb, stride_b), workspace, Cm.device, stream)
     _call(dev, stream, _lib.tb_grouped_matmul_blockscaled, d, A.data_ptr(), lda, sa, B.data_ptr(), ldb, stride_b, sb,
           Cm.data_ptr(), ldc, offsets.data_ptr(), ws, nbytes)
+    if even:
+        _remember(_ROWS_BYTES, A, SA, B, SB, Cm, offsets, beta, 0, d, (lda, ldb, stride_b, ldc), sa, sb)
     return Cm

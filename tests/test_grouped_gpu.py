@@ -183,6 +183,69 @@ def test_strided_and_unaligned_operands(cuda):
     tb.device_status()
 
 
+def test_calls_like_an_earlier_one(cuda):
+    """The same properties at other addresses, aligned or not, in turn with other layouts, types and beta."""
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(14)
+    off, ends = _offsets([9, 0, 140, 3])
+    rows, k, n = ends[-1], 72, 88
+    for i in range(24):
+        dt = (torch.float16, torch.bfloat16)[i % 2]
+        buf = _ints((rows * k + 8,), g, dt)
+        A = buf[(0, 8, 1, 3)[i % 4]:][:rows * k].view(rows, k)
+        B = _ints((4, k, n), g, dt) if i % 3 else _ints((4, n, k), g, dt).transpose(1, 2)
+        C = _ints((rows, n), g, (torch.float32, dt)[i // 12], 7)
+        want = _reference(A, B, C, ends, i % 2).to(C.dtype)
+        assert torch.equal(tb.grouped_matmul(A, B, C, off, beta=i % 2), want)
+        D = _ints((rows, n), g, dt)
+        G = _ints((4, k, n), g, torch.float32, 7)
+        ref = torch.stack([A[lo:hi].double().t() @ D[lo:hi].double() for lo, hi in zip(ends, ends[1:])])
+        want = ref + (i % 2) * G.double()
+        assert torch.equal(tb.grouped_matmul_wgrad(A, D, G, off, beta=i % 2).double(), want)
+    with pytest.raises(tb.TBError, match="beta"):
+        tb.grouped_matmul(A, B, C, off, beta=2)
+    with pytest.raises(tb.TBError, match="disagree"):
+        tb.grouped_matmul(A, B, C[1:], off)
+    with pytest.raises(tb.TBError, match="entries"):
+        tb.grouped_matmul(A, B, C, off[:-1])
+    with pytest.raises(tb.TBError, match="both be"):
+        tb.grouped_matmul(A.float(), B, C, off)
+    with pytest.raises(tb.TBError, match="CUDA tensor"):
+        tb.grouped_matmul(A, B, C, off.cpu())
+    tb.device_status()
+
+
+def test_threads(cuda):
+    """Calls from two threads at once, each on a stream of its own."""
+    import threading
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(15)
+    off, ends = _offsets([90, 0, 33, 130])
+    bad = []
+    sets = [(_ints((ends[-1], k), g, torch.float16), _ints((4, k, 136), g, torch.float16)) for k in (64, 200)]
+    torch.cuda.synchronize()
+
+    def work(A, B):
+        want = _reference(A, B, torch.zeros(ends[-1], 136, device="cuda"), ends, 0)
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(50):
+                C = tb.grouped_matmul(A, B, torch.zeros(ends[-1], 136, device="cuda"), off, beta=0)
+                if not torch.equal(C.double(), want):
+                    bad.append(A.shape)
+
+    threads = [threading.Thread(target=work, args=s) for s in sets]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 def test_weights_in_interleaved_layouts(cuda):
     """B [groups, k, n] as a view of (k, groups, n) and of (n, groups, k) storage; G as a view of (k, groups, n)."""
     import torch

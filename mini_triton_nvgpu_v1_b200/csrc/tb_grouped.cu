@@ -1007,33 +1007,42 @@ __global__ void __launch_bounds__(256)
   src += (int64_t)blockIdx.z * batch_src;
   dst += (int64_t)blockIdx.z * batch_dst;
   const int lane = threadIdx.x % 32;
+  const int words = (int)(ld_dst / 16);
   for (int64_t r = blockIdx.x * 8 + threadIdx.x / 32; r < rows; r += (int64_t)gridDim.x * 8) {
     const uint8_t* row = src + r * ld_src;
-    for (int64_t w = lane; w * 16 < ld_dst; w += 32) {
-      const int64_t left = row_bytes - w * 16;  // bytes of the row from here on
-      uint32_t v[5] = {0, 0, 0, 0, 0};
-      if (left > 0) {
-        const uint8_t* at = row + w * 16;
-        const int shift = (int)(reinterpret_cast<uintptr_t>(at) & 15);
-        const uint4* word = reinterpret_cast<const uint4*>(at - shift);
-        const uint4 lo = __ldg(word);
-        uint4 hi = make_uint4(0, 0, 0, 0);
-        if (shift + (left < 16 ? left : 16) > 16) hi = __ldg(word + 1);
-        const uint32_t x[9] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w, 0};
-        const int first = shift >> 2, bits = (shift & 3) * 8;
+    // every 16 bytes of a row are off a boundary by as much as its first
+    const int shift = (int)(reinterpret_cast<uintptr_t>(row) & 15);
+    const uint4* word = reinterpret_cast<const uint4*>(row - shift);
+    const int have = (int)((shift + row_bytes + 15) / 16);  // words that hold bytes of the row
+    const int first = shift >> 2, bits = (shift & 3) * 8;
+    for (int w0 = lane; w0 < words; w0 += 128) {
+      uint4 lo[4], hi[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {  // all loads at once
+        const int w = w0 + 32 * u;
+        lo[u] = w < have ? __ldg(word + w) : make_uint4(0, 0, 0, 0);
+        hi[u] = shift && w + 1 < have ? __ldg(word + w + 1) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int w = w0 + 32 * u;
+        if (w >= words) break;
+        const uint32_t x[9] = {lo[u].x, lo[u].y, lo[u].z, lo[u].w, hi[u].x, hi[u].y, hi[u].z, hi[u].w, 0};
+        uint32_t v[5] = {0, 0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < 5; ++i)
 #pragma unroll
           for (int f = 0; f < 4; ++f)
             if (first == f) v[i] = x[i + f];
+        const int64_t left = row_bytes - (int64_t)w * 16;  // bytes of the row from here on
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           v[i] = __funnelshift_r(v[i], v[i + 1], bits);
-          const int64_t here = left - 4 * i;  // bytes of the row in this word
+          const int64_t here = left - 4 * i;
           if (here < 4) v[i] = here <= 0 ? 0u : v[i] & (0xffffffffu >> (32 - 8 * (int)here));
         }
+        *reinterpret_cast<uint4*>(dst + r * ld_dst + (int64_t)w * 16) = make_uint4(v[0], v[1], v[2], v[3]);
       }
-      *reinterpret_cast<uint4*>(dst + r * ld_dst + w * 16) = make_uint4(v[0], v[1], v[2], v[3]);
     }
   }
 }

@@ -97,6 +97,9 @@ struct GCfg {
   static constexpr uint32_t kTmemCols = kAccs * BN;
   static constexpr int kHalfCols = BN / 2;              // columns per epilogue warp
   static constexpr int kChunks = kHalfCols / 32;
+  // One CTA's tile may be shared by a cluster, but not with 128 sums per
+  // thread: the exchange does not fit beside them into the registers.
+  static constexpr bool kShares = G == 1 && !(kSums && BN == 256);
   static constexpr uint32_t kRedStride = (BN + 4) * 4;  // bytes per row of the cluster's partial sums
   static constexpr uint32_t kRedBytes = 32 * kRedStride;  // 32 rows at a time
 };
@@ -798,7 +801,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     };
     int acc = 0;
     uint32_t acc_phase = 0;
-    if (G == 1 && cluster > 1) cluster_wait();
+    if (Cf::kShares && cluster > 1) cluster_wait();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     while (take(kSiteEpilogue)) {
       // Only the count of accumulations and the scales' places stay in
@@ -910,7 +913,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           }
           tc_fence_after();
         }
-        if (G == 1 && p.split > 1) {
+        if (Cf::kShares && p.split > 1) {
           if (!(ok = share([&](int c) -> const float (&)[32] {
                   if (fills > 0) {
                     tmem_ld_32x32b_x32(tm() + (uint32_t)(acc * BN + c * 32), v[0]);
@@ -946,7 +949,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
       }
 
       if constexpr (Cf::kSums) {
-        if (G == 1 && p.split > 1) {
+        if (Cf::kShares && p.split > 1) {
           if (!(ok = share([&](int c) -> const float (&)[32] { return v[c]; }))) break;
         } else {
           const bool row_ok = row_in_tile < field(&GTile::rows);
@@ -964,7 +967,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     }
     // Nothing of another CTA is on its way to this one any more (a cluster
     // barrier at the end took 1200 cycles).
-    if (G == 1 && p.split > 1 && ok) warp_poll(smem_addr(&bars.consumed), red_phase ^ 1u, abort_flag, kSiteCluster, lane);
+    if (Cf::kShares && p.split > 1 && ok) warp_poll(smem_addr(&bars.consumed), red_phase ^ 1u, abort_flag, kSiteCluster, lane);
   }
 
   __syncthreads();
@@ -1202,13 +1205,6 @@ tbStatus launch_tile(Launch& L, int sms, int dev, cudaStream_t stream) {
                                : launch<kHalf, BN, G>(L, sms, dev, stream);
 }
 
-// The kinds that a 128 × 256 tile is built for: with 128 sums per thread the
-// cluster's exchange does not fit into the registers.
-template <>
-tbStatus launch_tile<256, 1>(Launch& L, int sms, int dev, cudaStream_t stream) {
-  return launch<kHalf, 256, 1>(L, sms, dev, stream);
-}
-
 // Tile and K split, by estimated cycles. `rows`: mean rows of a group that has any.
 //
 // One ring fill takes 512 cycles of MMAs whatever the tile's width: a
@@ -1252,7 +1248,7 @@ tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int
   if (m > 128) consider(true, 256, 1);
   const bool sums = L.el == 1 || p.c_dtype == TB_F32;
   for (int b : {256, 128})
-    for (int s = sums && b == 256 ? 16 : 1; s <= 8 && (s == 1 || fills >= 4 * s); s *= 2) consider(false, b, s);
+    for (int s = 1; s <= (sums && b == 256 ? 1 : 8) && (s == 1 || fills >= 4 * s); s *= 2) consider(false, b, s);
   p.split = split;
   p.tiles_m = (int32_t)cdiv(p.M, pair ? 256 : 128);
   p.tiles_n = (int32_t)cdiv(n, bn);

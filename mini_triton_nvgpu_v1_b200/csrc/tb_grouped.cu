@@ -46,6 +46,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstring>
 #include <string>
 
@@ -1212,7 +1213,7 @@ tbStatus launch_tile(Launch& L, int sms, int dev, cudaStream_t stream) {
 // 64, 128 and 256 columns alike, so a narrower tile only lowers the rate. A
 // fill takes longer where its bytes do: 23 bytes a cycle and SM are an SM's
 // share of HBM, 45 the most that one SM was seen to draw while others idle,
-// and L2 feeds an SM 60 bytes a cycle.
+// and L2 feeds all SMs together 46 bytes a cycle each.
 // Storing a tile (16 bytes a cycle and SM) overlaps the next tile's fills.
 tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int dev, cudaStream_t stream) {
   GParams& p = L.p;
@@ -1222,19 +1223,23 @@ tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int
   const int64_t busy = p.k_grouped ? groups : std::min<int64_t>(groups, p.M);
   const int64_t fills = std::max<int64_t>(1, cdiv(p.k_grouped ? cdiv(p.K, std::max<int64_t>(1, groups)) : p.K, 128 / L.el));
   const int ce = p.c_dtype == TB_F32 ? 4 : 2;
+  const bool even = p.k_grouped || !p.offsets;  // every group has m rows
   double best = 0;
   int bn = 0, split = 1;
   bool pair = false;
   auto consider = [&](bool is_pair, int b, int s) {
-    const int64_t tiles = busy * cdiv(m, is_pair ? 256 : 128) * cdiv(n, b);
+    // Groups of uneven sizes fill their last tile by half on average.
+    const int64_t high = is_pair ? 256 : 128;
+    const double tiles_high = even ? (double)cdiv(m, high) : std::max(1.0, (double)m / (double)high + 0.5);
+    const int64_t tiles = (int64_t)std::ceil((double)busy * tiles_high) * cdiv(n, b);
     const int64_t slots = std::max<int64_t>(1, sms / (is_pair ? 2 : s));
     const double rounds = (double)cdiv(tiles, slots);
     const double used = std::min(1.0, (double)tiles / (double)slots);
     const double tile_rows = (double)std::min<int64_t>(m, 128);
     // bytes of a fill from HBM: B's share of a tile whose other tiles read the same B, and A's rows
-    const double bytes = 128.0 * ((double)(is_pair ? b / 2 : b) / (double)cdiv(m, is_pair ? 256 : 128) + tile_rows / (double)cdiv(n, b));
+    const double bytes = 128.0 * ((double)(is_pair ? b / 2 : b) / tiles_high + tile_rows / (double)cdiv(n, b));
     const double near = 128.0 * (is_pair ? 256 : b + tile_rows);  // into the SM, from L2
-    const double fill = std::max(std::max(512.0, near / 60.0), bytes / std::min(45.0, 23.0 / used));
+    const double fill = std::max(std::max(512.0, near / 46.0), bytes / std::min(45.0, 23.0 / used));
     const double main = (double)cdiv(fills, s) * fill + (s > 1 ? 300.0 + 300.0 * cdiv((int64_t)tile_rows, 32) : 0.0);
     const double store = tile_rows * b * ce / 16.0 / (s > 1 ? s : 1);
     const double cycles = rounds * std::max(main, store) + std::min(main, store);
@@ -1245,7 +1250,7 @@ tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int
       pair = is_pair;
     }
   };
-  if (m > 128) consider(true, 256, 1);
+  if (m > 64) consider(true, 256, 1);
   const bool sums = L.el == 1 || p.c_dtype == TB_F32;
   for (int b : {256, 128})
     for (int s = 1; s <= (sums && b == 256 ? 1 : 8) && (s == 1 || fills >= 4 * s); s *= 2) consider(false, b, s);

@@ -1053,6 +1053,8 @@ __global__ void __launch_bounds__(256)
 
 // ------------------------------------------------------------------- host
 
+constexpr int kMaxDev = 64;
+
 std::atomic<PFN_cuTensorMapEncodeTiled_v12000> g_encode_fn{nullptr};
 
 tbStatus encoder(PFN_cuTensorMapEncodeTiled_v12000* out) {
@@ -1070,7 +1072,6 @@ tbStatus encoder(PFN_cuTensorMapEncodeTiled_v12000* out) {
   return TB_OK;
 }
 
-constexpr int kMaxDev = 64;
 std::atomic<int> g_sms[kMaxDev];
 
 tbStatus current_device(int* dev, int* sms) {
@@ -1089,6 +1090,10 @@ tbStatus current_device(int* dev, int* sms) {
 }
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// Clusters of 2^i CTAs (one CTA to an SM) that the device holds at once: fewer
+// than its SMs divide into, since a cluster stays inside a GPC.
+std::atomic<int> g_clusters[kMaxDev][4];
+
 bool al(const void* p, int64_t n) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)n == 0; }
 
 // One operand as the kernel reads it: `rows` rows of `cols` contiguous
@@ -1147,11 +1152,12 @@ struct Launch {
   int el, bf16;
   int64_t tiles;  // an upper bound of the tiles
   int64_t rows;   // mean rows of a group that has any
+  int64_t slots;  // clusters at once
   GParams p;
 };
 
 template <int KIND, int BN, int G>
-tbStatus launch(Launch& L, int sms, int dev, cudaStream_t stream) {
+tbStatus launch(Launch& L, int dev, cudaStream_t stream) {
   using Cf = GCfg<KIND, BN, G>;
   GParams& p = L.p;
   CUtensorMap ta, tas, tb_;
@@ -1175,9 +1181,8 @@ tbStatus launch(Launch& L, int sms, int dev, cudaStream_t stream) {
     ready[dev].store(true);
   }
   const int cluster = G * p.split;
-  const int64_t slots = std::max(1, sms / cluster);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(std::min<int64_t>(slots, L.tiles) * cluster), 1, 1);
+  cfg.gridDim = dim3((unsigned)(std::min<int64_t>(L.slots, L.tiles) * cluster), 1, 1);
   cfg.blockDim = dim3(kThreadsG, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -1199,11 +1204,39 @@ tbStatus launch(Launch& L, int sms, int dev, cudaStream_t stream) {
 
 // The kind of a tile's kernel, by the operands' and the output's types.
 template <int BN, int G>
-tbStatus launch_tile(Launch& L, int sms, int dev, cudaStream_t stream) {
+tbStatus launch_tile(Launch& L, int dev, cudaStream_t stream) {
   if (L.el == 1)
-    return L.p.sb.shift ? launch<kByte, BN, G>(L, sms, dev, stream) : launch<kByteCol, BN, G>(L, sms, dev, stream);
-  return L.p.c_dtype == TB_F32 ? launch<kHalfSum, BN, G>(L, sms, dev, stream)
-                               : launch<kHalf, BN, G>(L, sms, dev, stream);
+    return L.p.sb.shift ? launch<kByte, BN, G>(L, dev, stream) : launch<kByteCol, BN, G>(L, dev, stream);
+  return L.p.c_dtype == TB_F32 ? launch<kHalfSum, BN, G>(L, dev, stream)
+                               : launch<kHalf, BN, G>(L, dev, stream);
+}
+
+tbStatus resident_clusters(int dev, int sms, int (&out)[4]) {
+  for (int i = 0; i < 4; ++i) {
+    int n = g_clusters[dev][i].load();
+    if (!n) {
+      auto kern = tb_grouped_sm100_kernel<kHalf, 128, 1>;
+      cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemLimitG);
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((unsigned)(sms >> i << i), 1, 1);
+      cfg.blockDim = dim3(kThreadsG, 1, 1);
+      cfg.dynamicSmemBytes = kSmemLimitG;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 1u << i;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
+      if (e != cudaSuccess)
+        return tb_fail(TB_ERR_CUDA, std::string("cudaOccupancyMaxActiveClusters: ") + cudaGetErrorString(e));
+      n = std::max(1, std::min(n, sms >> i));
+      g_clusters[dev][i].store(n);
+    }
+    out[i] = n;
+  }
+  return TB_OK;
 }
 
 // Tile and K split, by estimated cycles. `rows`: mean rows of a group that has any.
@@ -1217,6 +1250,9 @@ tbStatus launch_tile(Launch& L, int sms, int dev, cudaStream_t stream) {
 // Storing a tile (16 bytes a cycle and SM) overlaps the next tile's fills.
 tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int dev, cudaStream_t stream) {
   GParams& p = L.p;
+  int resident[4];  // clusters of 1, 2, 4 and 8 CTAs
+  tbStatus st = resident_clusters(dev, sms, resident);
+  if (st != TB_OK) return st;
   L.rows = rows;
   const int64_t n = p.N;
   const int64_t m = p.k_grouped ? p.M : rows;
@@ -1232,7 +1268,7 @@ tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int
     const int64_t high = is_pair ? 256 : 128;
     const double tiles_high = even ? (double)cdiv(m, high) : std::max(1.0, (double)m / (double)high + 0.5);
     const int64_t tiles = (int64_t)std::ceil((double)busy * tiles_high) * cdiv(n, b);
-    const int64_t slots = std::max<int64_t>(1, sms / (is_pair ? 2 : s));
+    const int64_t slots = resident[is_pair || s == 2 ? 1 : s == 1 ? 0 : s == 4 ? 2 : 3];
     const double rounds = (double)cdiv(tiles, slots);
     const double used = std::min(1.0, (double)tiles / (double)slots);
     const double tile_rows = (double)std::min<int64_t>(m, 128);
@@ -1255,13 +1291,14 @@ tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int
   for (int b : {256, 128})
     for (int s = 1; s <= (sums && b == 256 ? 1 : 8) && (s == 1 || fills >= 4 * s); s *= 2) consider(false, b, s);
   p.split = split;
+  L.slots = resident[pair || split == 2 ? 1 : split == 1 ? 0 : split == 4 ? 2 : 3];
   p.tiles_m = (int32_t)cdiv(p.M, pair ? 256 : 128);
   p.tiles_n = (int32_t)cdiv(n, bn);
   L.tiles = p.k_grouped ? groups * p.tiles_m * p.tiles_n
                         : (p.M / (pair ? 256 : 128) + std::min<int64_t>(groups, p.M)) * p.tiles_n;
-  return pair        ? launch_tile<256, 2>(L, sms, dev, stream)
-         : bn == 256 ? launch_tile<256, 1>(L, sms, dev, stream)
-                     : launch_tile<128, 1>(L, sms, dev, stream);
+  return pair        ? launch_tile<256, 2>(L, dev, stream)
+         : bn == 256 ? launch_tile<256, 1>(L, dev, stream)
+                     : launch_tile<128, 1>(L, dev, stream);
 }
 
 int c_bytes(int32_t dt) { return dt == TB_F32 ? 4 : 2; }

@@ -46,7 +46,7 @@ struct Signature {
   int n;
 };
 
-bool sign(PyObject* const* args, int op, int64_t x, int64_t y, Signature* s, const at::Tensor** t) {
+bool sign(PyObject* const* args, int op, int64_t x, int64_t y, Signature* s, const at::Tensor** t) try {
   s->n = 0;
   for (int i = 0; i < kTensors[op]; ++i) {
     if (!THPVariable_Check(args[i])) return false;
@@ -67,6 +67,8 @@ bool sign(PyObject* const* args, int op, int64_t x, int64_t y, Signature* s, con
   s->w[s->n++] = x;
   s->w[s->n++] = y;
   return true;
+} catch (const std::exception&) {  // tensors without plain sizes or strides
+  return false;
 }
 
 struct Known {

@@ -126,14 +126,20 @@ def _desc(groups, rows, n, k, ab, c, beta, a_col, b_col, long_) -> _capi.tb_grou
     return d
 
 
+def _empty(shape, dtype, device, stream):
+    """Memory of the stream it is used on: the allocator orders reuse by stream."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
 def _scratch(need: int, workspace, device, stream):
     """(address, bytes, tensor to keep) of a call's workspace."""
     if not need:
         return None, 0, None
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-        if stream is not None:
-            workspace.record_stream(stream)
+        workspace = _empty((need,), torch.uint8, device, stream)
     elif not workspace.is_cuda or workspace.device != device or not workspace.is_contiguous():
         raise _bad("workspace must be a contiguous CUDA tensor on the operands' device")
     return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
@@ -249,7 +255,8 @@ def quantize_fp8(X, Q=None, S=None, *, block=(1, 128), stream=None):
     [batch, rows, cols] (f32, f16 or bf16). Q: float8_e4m3fn of X's shape; S:
     f32 [(batch,) ceil(rows / block[0]), ceil(cols / block[1])]. A Q that is
     not given is made with rows that begin on 16-byte boundaries, as the
-    8-bit products read them without a copy. Returns (Q, S)."""
+    8-bit products read them without a copy; what is not given belongs to
+    ``stream``. Returns (Q, S)."""
     br, bc = block
     if Q is not None and S is not None and stream is None:
         code = _call0(_QUANTIZE, X, Q, S, br, bc)
@@ -267,14 +274,9 @@ def quantize_fp8(X, Q=None, S=None, *, block=(1, 128), stream=None):
         raise _bad("X must be f32, f16 or bf16")
     rows, cols = X.shape[-2:]
     if Q is None:
-        Q = torch.empty(*X.shape[:-1], (cols + 15) // 16 * 16, dtype=torch.uint8, device=X.device).view(_FP8)
-        Q = Q[..., :cols]
-        if stream is not None:
-            Q.record_stream(stream)
+        Q = _empty((*X.shape[:-1], (cols + 15) // 16 * 16), torch.uint8, X.device, stream).view(_FP8)[..., :cols]
     if S is None:
-        S = torch.empty(*X.shape[:-2], -(-rows // br), -(-cols // bc), device=X.device, dtype=torch.float32)
-        if stream is not None:
-            S.record_stream(stream)
+        S = _empty((*X.shape[:-2], -(-rows // br), -(-cols // bc)), torch.float32, X.device, stream)
     dev = _same_device(X=X, Q=Q, S=S)
     if Q.dtype != _FP8 or Q.shape != X.shape:
         raise _bad("Q must be float8_e4m3fn of X's shape")

@@ -403,3 +403,64 @@ def test_gradients_against_the_formula_and_differences(cuda):
         moved = B.clone()
         moved[e, i, j] += 1
         assert value(A, moved) - base == dB[e, i, j].double()
+
+
+@pytest.mark.parametrize("sizes,k,n", [([4099], 136, 120), ([2000, 0, 1, 3000], 72, 256), ([515, 512, 510], 128, 128)])
+def test_wgrad_of_few_tiles_over_many_rows(cuda, sizes, k, n):
+    """K ranges shared by the CTAs of a cluster, ending inside a fill."""
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(16)
+    off, ends = _offsets(sizes, 2)
+    A, D = _ints((ends[-1] + 9, k), g, torch.bfloat16, 2), _ints((ends[-1] + 9, n), g, torch.bfloat16, 2)
+    A[ends[-1]:] = float("nan")
+    for out, beta in ((torch.float32, 1), (torch.bfloat16, 0)):
+        G = _ints((len(sizes), k, n), g, out, 7)
+        ref = torch.stack([A[lo:hi].double().t() @ D[lo:hi].double() for lo, hi in zip(ends, ends[1:])])
+        want = (ref + beta * G.double()).to(out)
+        tb.grouped_matmul_wgrad(A, D, G, off, beta=beta)
+        assert torch.equal(G, want)
+    tb.device_status()
+
+
+def test_more_elements_than_32_bits_count(cuda):
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(17)
+    rows, k, n = 270_000, 64, 8192   # C: 2.2e9 elements
+    A, B = _ints((rows, k), g, torch.float16), _ints((3, k, n), g, torch.float16)
+    off, ends = _offsets([5, 269_500, 300], 100)
+    C = torch.full((rows, n), 3.0, device="cuda", dtype=torch.float16)
+    tb.grouped_matmul(A, B, C, off, beta=0)
+    for lo, hi, e in ((100, 105, 0), (200, 300, 1), (269_400, 269_605, 1), (269_605, 269_905, 2)):
+        assert torch.equal(C[lo:hi].double(), A[lo:hi].double() @ B[e].double())
+    assert (C[269_905:] == 3).all() and (C[:100] == 3).all()
+    G = torch.zeros(3, k, n, device="cuda")
+    tb.grouped_matmul_wgrad(A, C, G, off)
+    for e in (0, 2):
+        assert torch.equal(G[e].double(), A[ends[e]:ends[e + 1]].double().t() @ C[ends[e]:ends[e + 1]].double())
+    tb.device_status()
+
+
+def test_calls_follow_the_work_before_them(cuda):
+    """Operands written by the kernel just before, outputs read by the one just after, without a wait between."""
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(18)
+    off, ends = _offsets([3, 0, 200, 40])
+    k = 256
+    A, W = torch.zeros(ends[-1], k, device="cuda", dtype=torch.bfloat16), _ints((4, k, k), g, torch.bfloat16, 1)
+    values = [_ints((ends[-1], k), g, torch.bfloat16, 1) for _ in range(6)]
+    C, out = torch.zeros(ends[-1], k, device="cuda"), []
+    for i in range(60):
+        A.copy_(values[i % 6])
+        tb.grouped_matmul(A, W, C, off, beta=0)
+        Q, S = tb.quantize_fp8(C)
+        out.append((C.clone(), Q.float() * S.repeat_interleave(128, 1)))
+    for i, (c, v) in enumerate(out):
+        assert torch.equal(c.double(), _reference(values[i % 6], W, torch.zeros_like(c), ends, 0))
+        # e4m3: off by at most 2^-4 relative, and half its least step (2^-10) in units of the scale below that
+        assert ((v - c).abs() <= 2.0 ** -4 * c.abs() + 2.0 ** -10 * c.abs().amax() / 448).all()

@@ -161,13 +161,12 @@ struct GParams {
   int32_t small_log2;     // log2 of the rows of tmAs's boxes: a K-major A tile of few rows comes in these (G = 1)
 };
 
-__device__ __forceinline__ int32_t read_offset(const GParams& p, int32_t i) {
-  // Offsets out of [0, rows] are clamped: no access leaves the operands.
-  const int32_t rows = p.k_grouped ? p.K : p.M;
+// Offset i, clamped to [0, rows]: whatever the offsets are, no access leaves the operands.
+__device__ __forceinline__ int32_t read_offset(const void* offsets, bool wide, int32_t rows, int32_t i) {
   long long v;
-  if (!p.offsets) v = i ? rows : 0;
-  else if (p.offsets_64) v = static_cast<const long long*>(p.offsets)[i];
-  else v = static_cast<const int32_t*>(p.offsets)[i];
+  if (!offsets) v = i ? rows : 0;
+  else if (wide) v = static_cast<const long long*>(offsets)[i];
+  else v = static_cast<const int32_t*>(offsets)[i];
   return (int32_t)(v < 0 ? 0 : v > rows ? rows : v);
 }
 
@@ -666,32 +665,37 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     }
   } else {
     // ----------------------------------------------------------- scheduler
+    const void* const offsets = p.offsets;
+    const bool wide = p.offsets_64;
+    const int32_t groups = p.groups, all_rows = p.k_grouped ? p.K : p.M, tiles_n = p.tiles_n;
     // What this launch reads may be written by the kernel before it in the
     // stream, which each role waits for before its first access to memory
     // (programmatic launch).
     asm volatile("griddepcontrol.wait;" ::: "memory");
     int32_t before = 0;
-    for (int32_t e0 = 0; e0 < p.groups; e0 += 32) {
+    for (int32_t e0 = 0; e0 < groups; e0 += 32) {
       const int32_t e = e0 + lane;
-      int32_t lo = 0, rows = 0;
-      if (e < p.groups) {
-        lo = read_offset(p, e);
-        rows = max(0, read_offset(p, e + 1) - lo);
+      // every lane loads one offset; the last also the one behind its 32
+      int32_t lo = e <= groups ? read_offset(offsets, wide, all_rows, e) : all_rows;
+      const int32_t behind = lane == 31 && e < groups ? read_offset(offsets, wide, all_rows, e + 1) : 0;
+      const int32_t up = __shfl_down_sync(0xffffffffu, lo, 1);
+      const int32_t rows = e < groups ? max(0, (lane == 31 ? behind : up) - lo) : 0;
+      if (e < groups) {
         tab.start[e] = lo;
         tab.rows[e] = rows;
       }
-      int32_t v = (rows + Cf::kBM - 1) / Cf::kBM * p.tiles_n;
+      int32_t v = (rows + Cf::kBM - 1) / Cf::kBM * tiles_n;
 #pragma unroll
       for (int d = 1; d < 32; d *= 2) {
         const int32_t o = __shfl_up_sync(0xffffffffu, v, d);
         if (lane >= d) v += o;
       }
-      if (e < p.groups) tab.cum[e + 1] = before + v;
+      if (e < groups) tab.cum[e + 1] = before + v;
       before += __shfl_sync(0xffffffffu, v, 31);
     }
     if (lane == 0) tab.cum[0] = 0;
     __syncwarp();
-    const int32_t tiles = p.k_grouped ? p.groups * p.tiles_m * p.tiles_n : before;
+    const int32_t tiles = p.k_grouped ? groups * p.tiles_m * tiles_n : before;
     int32_t cursor = 0;
     for (int32_t t = first;; t += stride) {
       GTile tile = {};

@@ -1250,7 +1250,8 @@ tbStatus resident_clusters(int dev, int sms, int (&out)[4]) {
 // 64, 128 and 256 columns alike, so a narrower tile only lowers the rate. A
 // fill takes longer where its bytes do: 23 bytes a cycle and SM are an SM's
 // share of HBM, 45 the most that one SM was seen to draw while others idle,
-// and L2 feeds all SMs together 46 bytes a cycle each.
+// and L2 feeds all SMs together 46 bytes a cycle each (42 where a CTA takes
+// 48 KB at a time). A pair's two cluster barriers take 600 cycles.
 // Storing a tile (16 bytes a cycle and SM) overlaps the next tile's fills.
 tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int dev, cudaStream_t stream) {
   GParams& p = L.p;
@@ -1279,10 +1280,10 @@ tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int
     // bytes of a fill from HBM: B's share of a tile whose other tiles read the same B, and A's rows
     const double bytes = 128.0 * ((double)(is_pair ? b / 2 : b) / tiles_high + tile_rows / (double)cdiv(n, b));
     const double near = 128.0 * (is_pair ? 256 : b + tile_rows);  // into the SM, from L2
-    const double fill = std::max(std::max(512.0, near / 46.0), bytes / std::min(45.0, 23.0 / used));
+    const double fill = std::max(std::max(512.0, near / (is_pair || b == 128 ? 46.0 : 42.0)), bytes / std::min(45.0, 23.0 / used));
     const double main = (double)cdiv(fills, s) * fill + (s > 1 ? 300.0 + 300.0 * cdiv((int64_t)tile_rows, 32) : 0.0);
     const double store = tile_rows * b * ce / 16.0 / (s > 1 ? s : 1);
-    const double cycles = rounds * std::max(main, store) + std::min(main, store);
+    const double cycles = rounds * std::max(main, store) + std::min(main, store) + (is_pair ? 600.0 : 0.0);
     if (!bn || cycles < best) {
       best = cycles;
       bn = b;
@@ -1292,7 +1293,7 @@ tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int
   };
   if (m > 64) consider(true, 256, 1);
   const bool sums = L.el == 1 || p.c_dtype == TB_F32;
-  for (int b : {256, 128})
+  for (int b : {128, 256})
     for (int s = 1; s <= (sums && b == 256 ? 1 : 8) && (s == 1 || fills >= 4 * s); s *= 2) consider(false, b, s);
   p.split = split;
   L.slots = resident[pair || split == 2 ? 1 : split == 1 ? 0 : split == 4 ? 2 : 3];

@@ -342,7 +342,10 @@ tbStatus tb_matmul(const tb_matmul_desc* desc, const void* A, int64_t lda,
  * aligned; the *_workspace_bytes functions say how much that takes for the
  * operands that they are given (0 in the ordinary case, then workspace may be
  * NULL). Sums are in f32; the output is rounded once. Results repeat bit for
- * bit (no atomics). beta = 0 does not read the output. */
+ * bit (no atomics). beta = 0 does not read the output. An output may not
+ * overlap an operand, nor its groups' matrices each other. Kernels are
+ * launched with programmatic stream serialization: their set-up may run
+ * while the kernel before them in the stream ends, their work does not. */
 typedef struct tb_grouped_desc {
   int64_t groups;                  /* 0 … 1024; 1 for tb_matmul_blockscaled */
   int64_t rows;                    /* rows of A and C, over all groups */

@@ -37,6 +37,18 @@
 // cluster, which add their partial sums through distributed shared memory in
 // a fixed order — no workspace, no atomics, results repeat bit for bit.
 //
+// What bounds it (B200, 148 SMs; times of single calls in a CUDA graph):
+// * Training sizes: the operands' way from L2 into the SMs, 43–46 bytes a cycle
+//   and SM for 32 KB per fill of a 256 × 256 pair tile (the MMAs of a fill
+//   need 512 cycles), and below that the power cap: 16384 rows over 8 experts
+//   of 4096 × 4096 bf16 in 380 µs (1450 TFLOP/s), 1220 in a sustained loop.
+// * 8-bit products: besides, the epilogue takes 64 KB of sums per block and
+//   CTA out of TMEM: 8192³ e4m3 in 490 µs (2240 TFLOP/s; 437 µs with the
+//   epilogue's arithmetic left out).
+// * Decoding steps: HBM, once the weights flow (6.2 TB/s), and some 4 µs of
+//   start and end around it: offsets, first tile, first fill, exchange.
+//   96 rows over 32 experts of 2048 × 1408 f16 (179 MB): 35.5 µs.
+//
 // Every wait is bounded, as in the dense GEMM.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -251,7 +263,9 @@ __device__ __forceinline__ float2 unpack2(const GParams& p, uint32_t w) {
   memcpy(&h, &w, 4);
   return __bfloat1622float2(h);
 }
-// 32 bytes in one store: a whole sector, so that a warp's rows need no merging in L2.
+// 32 bytes in one store: a whole sector, so that a warp's rows need no merging
+// in L2. (The output through shared memory, by TMA or in whole rows, gained 3 to
+// 13 % where little but the output is written and lost as much elsewhere.)
 __device__ __forceinline__ void st_32(void* q, const uint32_t* w) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(q), "r"(w[0]), "r"(w[1]),
                "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
@@ -460,259 +474,259 @@ __global__ void __launch_bounds__(kThreadsG, 1)
   // 224 + 128 × 56 registers = the launch's 384 × 168.
   constexpr bool kMoveRegs = Cf::kSums && BN == 256;
   if (warp < 4) {
-  if constexpr (kMoveRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-  if (warp != 3) start();
-  if (warp == 0) {
-    // ------------------------------------------------------------ producer
-    // An operand's fill is a few boxes: box j of fill f lies at coordinates
-    // (x + f·fx + j·jx, y + f·fy + j·jy) and goes to dst + j·step. What
-    // decides them is worked out once per tile; with the parameters read and
-    // tested inside the loop a fill took 475 cycles to issue.
-    const bool a_mn = p.a_mn, b_mn = !p.b_kmaj, grouped_k = p.k_grouped;
-    const int32_t a_fx = a_mn ? 0 : Cf::kKB, a_fy = a_mn ? Cf::kKB : 0;
-    const int32_t b_fx = b_mn ? 0 : Cf::kKB, b_fy = b_mn ? Cf::kKB : 0;
-    const int32_t b_boxes = b_mn ? Cf::kBnCta / Cf::kMnBox : 1;
-    const int32_t sr = 1 << p.small_log2;
-    const uint32_t full0 = smem_addr(&bars.full[0]), empty0 = smem_addr(&bars.empty[0]), fix0 = smem_addr(&bars.fix[0]);
-    const uint32_t full0_leader = G == 2 ? map_to_cta(full0, 0) : full0;
-    const uint32_t sa0 = smem_addr(sA), sb0 = smem_addr(sB);
-    int stage = 0;
-    uint32_t phase = 0;
-    uint32_t issued = 0;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    while (take(kSiteProducer)) {
-      const GTile g = bars.tile[slot];
-      done();
-      // K-major A of a tile with few rows: only the small boxes that hold them
-      const bool few = G == 1 && !a_mn && g.rows <= 3 * sr;
-      const CUtensorMap* const map_a = few ? &tmAs : &tmA;
-      const int32_t a_boxes = a_mn ? 128 / Cf::kMnBox : few ? (g.rows + sr - 1) >> p.small_log2 : 1;
-      const uint32_t a_step = a_mn ? Cf::kMnBoxBytes : (uint32_t)sr * 128u;
-      const int32_t a_jx = a_mn ? Cf::kMnBox : 0, a_jy = a_mn ? 0 : sr;
-      const uint32_t bytes = (few ? (uint32_t)a_boxes * a_step : Cf::kABytes) + Cf::kBBytes;
-      const int32_t am = g.row0 + (int32_t)rank * 128, bn = g.n0 + (int32_t)rank * Cf::kBnCta;
-      const int32_t k_first = g.k0 + g.f0 * Cf::kKB;
-      int32_t ax = a_mn ? am : k_first, ay = a_mn ? k_first : am;
-      int32_t bx = b_mn ? bn : k_first, by = b_mn ? k_first : bn;
-      const int32_t be = grouped_k ? 0 : g.e;
-      // the fill (if any) whose last rows the fixer takes out
-      const int32_t fix_at = grouped_k && (g.k_end - g.k0) % Cf::kMmaK != 0 && g.f1 * Cf::kKB > g.k_end - g.k0 - Cf::kMmaK
-                                 ? (g.k_end - g.k0) / Cf::kKB : -1;
-      for (int32_t f = g.f0; f < g.f1; ++f) {
-        if (issued >= (uint32_t)S && !warp_wait(empty0 + stage * 8, phase ^ 1u, abort_flag, kSiteProducer, lane)) {
-          ok = false;
-          break;
-        }
-        if (elect_one()) {
-          uint32_t bar;
-          if (f == fix_at) {  // this CTA's fixer takes the fill on from here
-            bar = fix0 + stage * 8;
-            mbar_expect_tx(bar, bytes);
-          } else {
-            bar = full0_leader + stage * 8;
-            if (leader) mbar_expect_tx(full0 + stage * 8, G * bytes);
-            else if (grouped_k) mbar_arrive_remote(bar);
-          }
-          uint32_t dst = sa0 + (uint32_t)stage * Cf::kABytes;
-          for (int32_t j = 0; j < a_boxes; ++j, dst += a_step) {
-            if constexpr (G == 2) tma_load_2d_pair(dst, map_a, bar, ax + j * a_jx, ay + j * a_jy);
-            else tma_load_2d(dst, map_a, bar, ax + j * a_jx, ay + j * a_jy);
-          }
-          dst = sb0 + (uint32_t)stage * Cf::kBBytes;
-          for (int32_t j = 0; j < b_boxes; ++j, dst += Cf::kMnBoxBytes) {
-            if constexpr (G == 2) tma_load_3d_pair(dst, &tmB, bar, bx + j * Cf::kMnBox, by, be);
-            else tma_load_3d(dst, &tmB, bar, bx + j * Cf::kMnBox, by, be);
-          }
-        }
-        __syncwarp();
-        ax += a_fx;
-        ay += a_fy;
-        bx += b_fx;
-        by += b_fy;
-        ++issued;
-        if (++stage == S) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-    }
-    if (lane == 0) bars.issued = issued;
-  } else if (warp == 1) {
-    // ---------------------------------------------------------- MMA issuer
-    if constexpr (G == 1) {
-      tmem_alloc_g<G>(smem_addr(&bars.tmem_holder), Cf::kTmemCols);
-      tmem_relinquish_g<G>();
-    }
-    if (leader) {
-      const uint32_t tmem_base = *const_cast<volatile uint32_t*>(&bars.tmem_holder);
-      const uint32_t idesc = idesc_f16_f32(Cf::kBM, BN, p.a_mn ? 1 : 0, p.b_kmaj ? 0 : 1) | (p.fmt << 7) |
-                             (p.fmt << 10);
-      // descriptor words: the start address (16-byte units) moves in the low one
-      const uint32_t a_step = (p.a_mn ? Cf::kMnStep : 32u) >> 4, b_step = (p.b_kmaj ? 32u : Cf::kMnStep) >> 4;
-      const uint64_t da = smem_desc_sw128(smem_addr(sA), p.a_mn ? Cf::kMnBoxBytes : 16u, 1024);
-      const uint64_t db = smem_desc_sw128(smem_addr(sB), p.b_kmaj ? 16u : Cf::kMnBoxBytes, 1024);
-      const uint32_t a_hi = (uint32_t)(da >> 32), b_hi = (uint32_t)(db >> 32);
-      const uint32_t full0 = smem_addr(&bars.full[0]), empty0 = smem_addr(&bars.empty[0]),
-                     tfull0 = smem_addr(&bars.tfull[0]), tempty0 = smem_addr(&bars.tempty[0]);
-      auto commit = [&](uint32_t bar) {
-        if constexpr (G == 2) umma_commit_pair(bar, 0x3);
-        else umma_commit(bar);
-      };
-      int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0;
-      bool issued_any = false;
-      while (take(kSiteMma)) {
-        // this tile's fills, and the MMA steps of the last one
-        const int32_t fills = field(&GTile::f1) - field(&GTile::f0);
-        const int32_t last_valid = min(Cf::kKB, field(&GTile::k_end) - field(&GTile::k0) - (field(&GTile::f1) - 1) * Cf::kKB);
-        const int last_steps = (last_valid + Cf::kMmaK - 1) / Cf::kMmaK;
+    if constexpr (kMoveRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp != 3) start();
+    if (warp == 0) {
+      // ------------------------------------------------------------ producer
+      // An operand's fill is a few boxes: box j of fill f lies at coordinates
+      // (x + f·fx + j·jx, y + f·fy + j·jy) and goes to dst + j·step. What
+      // decides them is worked out once per tile; with the parameters read and
+      // tested inside the loop a fill took 475 cycles to issue.
+      const bool a_mn = p.a_mn, b_mn = !p.b_kmaj, grouped_k = p.k_grouped;
+      const int32_t a_fx = a_mn ? 0 : Cf::kKB, a_fy = a_mn ? Cf::kKB : 0;
+      const int32_t b_fx = b_mn ? 0 : Cf::kKB, b_fy = b_mn ? Cf::kKB : 0;
+      const int32_t b_boxes = b_mn ? Cf::kBnCta / Cf::kMnBox : 1;
+      const int32_t sr = 1 << p.small_log2;
+      const uint32_t full0 = smem_addr(&bars.full[0]), empty0 = smem_addr(&bars.empty[0]), fix0 = smem_addr(&bars.fix[0]);
+      const uint32_t full0_leader = G == 2 ? map_to_cta(full0, 0) : full0;
+      const uint32_t sa0 = smem_addr(sA), sb0 = smem_addr(sB);
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t issued = 0;
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      while (take(kSiteProducer)) {
+        const GTile g = bars.tile[slot];
         done();
-        bool here = false;  // the fill at hand was seen to have landed
-        for (int32_t f = 0; f < fills; ++f) {
-          // first and last fill of an accumulation
-          const bool opens = Cf::kSums ? f % Cf::kSegFills == 0 : f == 0;
-          const bool closes = f + 1 == fills || (Cf::kSums && (f + 1) % Cf::kSegFills == 0);
-          if ((opens && !warp_poll(tempty0 + acc * 8, acc_phase ^ 1u, abort_flag, kSiteMma, lane)) ||
-              (!here && !warp_poll(full0 + stage * 8, phase, abort_flag, kSiteMma, lane))) {
+        // K-major A of a tile with few rows: only the small boxes that hold them
+        const bool few = G == 1 && !a_mn && g.rows <= 3 * sr;
+        const CUtensorMap* const map_a = few ? &tmAs : &tmA;
+        const int32_t a_boxes = a_mn ? 128 / Cf::kMnBox : few ? (g.rows + sr - 1) >> p.small_log2 : 1;
+        const uint32_t a_step = a_mn ? Cf::kMnBoxBytes : (uint32_t)sr * 128u;
+        const int32_t a_jx = a_mn ? Cf::kMnBox : 0, a_jy = a_mn ? 0 : sr;
+        const uint32_t bytes = (few ? (uint32_t)a_boxes * a_step : Cf::kABytes) + Cf::kBBytes;
+        const int32_t am = g.row0 + (int32_t)rank * 128, bn = g.n0 + (int32_t)rank * Cf::kBnCta;
+        const int32_t k_first = g.k0 + g.f0 * Cf::kKB;
+        int32_t ax = a_mn ? am : k_first, ay = a_mn ? k_first : am;
+        int32_t bx = b_mn ? bn : k_first, by = b_mn ? k_first : bn;
+        const int32_t be = grouped_k ? 0 : g.e;
+        // the fill (if any) whose last rows the fixer takes out
+        const int32_t fix_at = grouped_k && (g.k_end - g.k0) % Cf::kMmaK != 0 && g.f1 * Cf::kKB > g.k_end - g.k0 - Cf::kMmaK
+                                   ? (g.k_end - g.k0) / Cf::kKB : -1;
+        for (int32_t f = g.f0; f < g.f1; ++f) {
+          if (issued >= (uint32_t)S && !warp_wait(empty0 + stage * 8, phase ^ 1u, abort_flag, kSiteProducer, lane)) {
             ok = false;
             break;
           }
-          tc_fence_after();
-          const uint32_t a_lo = (uint32_t)da + (uint32_t)stage * (Cf::kABytes >> 4);
-          const uint32_t b_lo = (uint32_t)db + (uint32_t)stage * (Cf::kBBytes >> 4);
-          const uint32_t d = tmem_base + (uint32_t)(acc * BN);
-          const uint32_t empty = empty0 + stage * 8;
+          if (elect_one()) {
+            uint32_t bar;
+            if (f == fix_at) {  // this CTA's fixer takes the fill on from here
+              bar = fix0 + stage * 8;
+              mbar_expect_tx(bar, bytes);
+            } else {
+              bar = full0_leader + stage * 8;
+              if (leader) mbar_expect_tx(full0 + stage * 8, G * bytes);
+              else if (grouped_k) mbar_arrive_remote(bar);
+            }
+            uint32_t dst = sa0 + (uint32_t)stage * Cf::kABytes;
+            for (int32_t j = 0; j < a_boxes; ++j, dst += a_step) {
+              if constexpr (G == 2) tma_load_2d_pair(dst, map_a, bar, ax + j * a_jx, ay + j * a_jy);
+              else tma_load_2d(dst, map_a, bar, ax + j * a_jx, ay + j * a_jy);
+            }
+            dst = sb0 + (uint32_t)stage * Cf::kBBytes;
+            for (int32_t j = 0; j < b_boxes; ++j, dst += Cf::kMnBoxBytes) {
+              if constexpr (G == 2) tma_load_3d_pair(dst, &tmB, bar, bx + j * Cf::kMnBox, by, be);
+              else tma_load_3d(dst, &tmB, bar, bx + j * Cf::kMnBox, by, be);
+            }
+          }
+          __syncwarp();
+          ax += a_fx;
+          ay += a_fy;
+          bx += b_fx;
+          by += b_fy;
+          ++issued;
           if (++stage == S) {
             stage = 0;
             phase ^= 1u;
           }
-          // the next fill's barrier is read while this one's MMAs are issued
-          const bool peek = f + 1 < fills && mbar_test_wait(full0 + stage * 8, phase);
-          if (elect_one()) {
-            if (f + 1 < fills || last_steps == 4) {
-#pragma unroll
-              for (uint32_t kk = 0; kk < 4; ++kk)
-                umma_words<G, Cf::kBytes>(d, a_lo + a_step * kk, a_hi, b_lo + b_step * kk, b_hi, idesc,
-                                          (!opens || kk > 0) ? 1u : 0u);
-            } else {
-              for (uint32_t kk = 0; kk < (uint32_t)last_steps; ++kk)
-                umma_words<G, Cf::kBytes>(d, a_lo + a_step * kk, a_hi, b_lo + b_step * kk, b_hi, idesc,
-                                          (!opens || kk > 0) ? 1u : 0u);
-            }
-            commit(empty);
-            if (closes) commit(tfull0 + acc * 8);
-          }
-          here = __all_sync(0xffffffffu, peek);
-          issued_any = true;
-          if (closes && ++acc == 2) {
-            acc = 0;
-            acc_phase ^= 1u;
-          }
         }
       }
-      if (!ok && issued_any && lane == 0) {
-        // Given up with MMAs possibly in flight: wait for them before TMEM goes.
-        if constexpr (G == 2) umma_commit_pair(smem_addr(&bars.drain), 0x1);
-        else umma_commit(smem_addr(&bars.drain));
-        const long long t0 = clock64();
-        while (!mbar_try_wait(smem_addr(&bars.drain), 0)) {
-          if (clock64() - t0 > kWaitBudgetCycles) {
-            record_error(TB_ERR_DEVICE_TIMEOUT, kSiteDrain);
+      if (lane == 0) bars.issued = issued;
+    } else if (warp == 1) {
+      // ---------------------------------------------------------- MMA issuer
+      if constexpr (G == 1) {
+        tmem_alloc_g<G>(smem_addr(&bars.tmem_holder), Cf::kTmemCols);
+        tmem_relinquish_g<G>();
+      }
+      if (leader) {
+        const uint32_t tmem_base = *const_cast<volatile uint32_t*>(&bars.tmem_holder);
+        const uint32_t idesc = idesc_f16_f32(Cf::kBM, BN, p.a_mn ? 1 : 0, p.b_kmaj ? 0 : 1) | (p.fmt << 7) |
+                               (p.fmt << 10);
+        // descriptor words: the start address (16-byte units) moves in the low one
+        const uint32_t a_step = (p.a_mn ? Cf::kMnStep : 32u) >> 4, b_step = (p.b_kmaj ? 32u : Cf::kMnStep) >> 4;
+        const uint64_t da = smem_desc_sw128(smem_addr(sA), p.a_mn ? Cf::kMnBoxBytes : 16u, 1024);
+        const uint64_t db = smem_desc_sw128(smem_addr(sB), p.b_kmaj ? 16u : Cf::kMnBoxBytes, 1024);
+        const uint32_t a_hi = (uint32_t)(da >> 32), b_hi = (uint32_t)(db >> 32);
+        const uint32_t full0 = smem_addr(&bars.full[0]), empty0 = smem_addr(&bars.empty[0]),
+                       tfull0 = smem_addr(&bars.tfull[0]), tempty0 = smem_addr(&bars.tempty[0]);
+        auto commit = [&](uint32_t bar) {
+          if constexpr (G == 2) umma_commit_pair(bar, 0x3);
+          else umma_commit(bar);
+        };
+        int stage = 0, acc = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        bool issued_any = false;
+        while (take(kSiteMma)) {
+          // this tile's fills, and the MMA steps of the last one
+          const int32_t fills = field(&GTile::f1) - field(&GTile::f0);
+          const int32_t last_valid = min(Cf::kKB, field(&GTile::k_end) - field(&GTile::k0) - (field(&GTile::f1) - 1) * Cf::kKB);
+          const int last_steps = (last_valid + Cf::kMmaK - 1) / Cf::kMmaK;
+          done();
+          bool here = false;  // the fill at hand was seen to have landed
+          for (int32_t f = 0; f < fills; ++f) {
+            // first and last fill of an accumulation
+            const bool opens = Cf::kSums ? f % Cf::kSegFills == 0 : f == 0;
+            const bool closes = f + 1 == fills || (Cf::kSums && (f + 1) % Cf::kSegFills == 0);
+            if ((opens && !warp_poll(tempty0 + acc * 8, acc_phase ^ 1u, abort_flag, kSiteMma, lane)) ||
+                (!here && !warp_poll(full0 + stage * 8, phase, abort_flag, kSiteMma, lane))) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t a_lo = (uint32_t)da + (uint32_t)stage * (Cf::kABytes >> 4);
+            const uint32_t b_lo = (uint32_t)db + (uint32_t)stage * (Cf::kBBytes >> 4);
+            const uint32_t d = tmem_base + (uint32_t)(acc * BN);
+            const uint32_t empty = empty0 + stage * 8;
+            if (++stage == S) {
+              stage = 0;
+              phase ^= 1u;
+            }
+            // the next fill's barrier is read while this one's MMAs are issued
+            const bool peek = f + 1 < fills && mbar_test_wait(full0 + stage * 8, phase);
+            if (elect_one()) {
+              if (f + 1 < fills || last_steps == 4) {
+#pragma unroll
+                for (uint32_t kk = 0; kk < 4; ++kk)
+                  umma_words<G, Cf::kBytes>(d, a_lo + a_step * kk, a_hi, b_lo + b_step * kk, b_hi, idesc,
+                                            (!opens || kk > 0) ? 1u : 0u);
+              } else {
+                for (uint32_t kk = 0; kk < (uint32_t)last_steps; ++kk)
+                  umma_words<G, Cf::kBytes>(d, a_lo + a_step * kk, a_hi, b_lo + b_step * kk, b_hi, idesc,
+                                            (!opens || kk > 0) ? 1u : 0u);
+              }
+              commit(empty);
+              if (closes) commit(tfull0 + acc * 8);
+            }
+            here = __all_sync(0xffffffffu, peek);
+            issued_any = true;
+            if (closes && ++acc == 2) {
+              acc = 0;
+              acc_phase ^= 1u;
+            }
+          }
+        }
+        if (!ok && issued_any && lane == 0) {
+          // Given up with MMAs possibly in flight: wait for them before TMEM goes.
+          if constexpr (G == 2) umma_commit_pair(smem_addr(&bars.drain), 0x1);
+          else umma_commit(smem_addr(&bars.drain));
+          const long long t0 = clock64();
+          while (!mbar_try_wait(smem_addr(&bars.drain), 0)) {
+            if (clock64() - t0 > kWaitBudgetCycles) {
+              record_error(TB_ERR_DEVICE_TIMEOUT, kSiteDrain);
+              break;
+            }
+          }
+        }
+        __syncwarp();
+      }
+    } else if (warp == 2) {
+      // --------------------------------------------------------------- fixer
+      if (p.k_grouped) {
+        int stage = 0;
+        uint32_t fix_phase = 0;  // bit s: parity of stage s's next fix
+        while (take(kSiteFixer)) {
+          const GTile g = bars.tile[slot];
+          done();
+          const int32_t n = g.f1 - g.f0;
+          if (n <= 0) continue;
+          const int32_t last = (stage + n - 1) % S;  // only a tile's last fill can be short
+          const int32_t valid = min(Cf::kKB, g.k_end - (g.k0 + (g.f1 - 1) * Cf::kKB));
+          stage = (stage + n) % S;
+          if (valid % Cf::kMmaK == 0) continue;
+          if (!warp_wait(smem_addr(&bars.fix[last]), (fix_phase >> last) & 1u, abort_flag, kSiteFixer, lane)) {
+            ok = false;
             break;
           }
-        }
-      }
-      __syncwarp();
-    }
-  } else if (warp == 2) {
-    // --------------------------------------------------------------- fixer
-    if (p.k_grouped) {
-      int stage = 0;
-      uint32_t fix_phase = 0;  // bit s: parity of stage s's next fix
-      while (take(kSiteFixer)) {
-        const GTile g = bars.tile[slot];
-        done();
-        const int32_t n = g.f1 - g.f0;
-        if (n <= 0) continue;
-        const int32_t last = (stage + n - 1) % S;  // only a tile's last fill can be short
-        const int32_t valid = min(Cf::kKB, g.k_end - (g.k0 + (g.f1 - 1) * Cf::kKB));
-        stage = (stage + n) % S;
-        if (valid % Cf::kMmaK == 0) continue;
-        if (!warp_wait(smem_addr(&bars.fix[last]), (fix_phase >> last) & 1u, abort_flag, kSiteFixer, lane)) {
-          ok = false;
-          break;
-        }
-        fix_phase ^= 1u << last;
-        // K rows [valid, next multiple of the K step) of every box of both
-        // operands: 128 bytes per row (the swizzle stays inside a row)
-        const int32_t end = (valid + Cf::kMmaK - 1) / Cf::kMmaK * Cf::kMmaK;
-        const int32_t words = (end - valid) * 8;
-        auto zero = [&](uint8_t* stage_base, int nboxes) {
-          for (int b = 0; b < nboxes; ++b) {
-            uint4* q = reinterpret_cast<uint4*>(stage_base + (size_t)b * Cf::kMnBoxBytes + (size_t)valid * 128);
-            for (int i = lane; i < words; i += 32) q[i] = make_uint4(0, 0, 0, 0);
+          fix_phase ^= 1u << last;
+          // K rows [valid, next multiple of the K step) of every box of both
+          // operands: 128 bytes per row (the swizzle stays inside a row)
+          const int32_t end = (valid + Cf::kMmaK - 1) / Cf::kMmaK * Cf::kMmaK;
+          const int32_t words = (end - valid) * 8;
+          auto zero = [&](uint8_t* stage_base, int nboxes) {
+            for (int b = 0; b < nboxes; ++b) {
+              uint4* q = reinterpret_cast<uint4*>(stage_base + (size_t)b * Cf::kMnBoxBytes + (size_t)valid * 128);
+              for (int i = lane; i < words; i += 32) q[i] = make_uint4(0, 0, 0, 0);
+            }
+          };
+          zero(sA + (size_t)last * Cf::kABytes, 128 / Cf::kMnBox);
+          zero(sB + (size_t)last * Cf::kBBytes, Cf::kBnCta / Cf::kMnBox);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (G == 2) mbar_arrive_cluster(map_to_cta(smem_addr(&bars.full[last]), 0));
+            else mbar_arrive(smem_addr(&bars.full[last]));
           }
-        };
-        zero(sA + (size_t)last * Cf::kABytes, 128 / Cf::kMnBox);
-        zero(sB + (size_t)last * Cf::kBBytes, Cf::kBnCta / Cf::kMnBox);
-        fence_proxy_async_smem();
-        __syncwarp();
+        }
+      }
+    } else {
+      // ----------------------------------------------------------- scheduler
+      const void* const offsets = p.offsets;
+      const bool wide = p.offsets_64;
+      const int32_t groups = p.groups, all_rows = p.k_grouped ? p.K : p.M, tiles_n = p.tiles_n;
+      // What this launch reads may be written by the kernel before it in the
+      // stream, which each role waits for before its first access to memory
+      // (programmatic launch).
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      int32_t before = 0;
+      for (int32_t e0 = 0; e0 < groups; e0 += 32) {
+        const int32_t e = e0 + lane;
+        // every lane loads one offset; the last also the one behind its 32
+        int32_t lo = e <= groups ? read_offset(offsets, wide, all_rows, e) : all_rows;
+        const int32_t behind = lane == 31 && e < groups ? read_offset(offsets, wide, all_rows, e + 1) : 0;
+        const int32_t up = __shfl_down_sync(0xffffffffu, lo, 1);
+        const int32_t rows = e < groups ? max(0, (lane == 31 ? behind : up) - lo) : 0;
+        if (e < groups) {
+          tab.start[e] = lo;
+          tab.rows[e] = rows;
+        }
+        int32_t v = (rows + Cf::kBM - 1) / Cf::kBM * tiles_n;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+          const int32_t o = __shfl_up_sync(0xffffffffu, v, d);
+          if (lane >= d) v += o;
+        }
+        if (e < groups) tab.cum[e + 1] = before + v;
+        before += __shfl_sync(0xffffffffu, v, 31);
+      }
+      if (lane == 0) tab.cum[0] = 0;
+      __syncwarp();
+      const int32_t tiles = p.k_grouped ? groups * p.tiles_m * tiles_n : before;
+      int32_t cursor = 0;
+      for (int32_t t = first;; t += stride) {
+        GTile tile = {};
+        if (t < tiles) tile = tile_at<Cf::kBM, BN, Cf::kKB>(p, tab, t, part, cursor, lane);
+        if (t == first) start();
+        if (!warp_wait(smem_addr(&bars.tile_empty[slot]), slot_phase ^ 1u, abort_flag, kSiteScheduler, lane)) break;
         if (lane == 0) {
-          if constexpr (G == 2) mbar_arrive_cluster(map_to_cta(smem_addr(&bars.full[last]), 0));
-          else mbar_arrive(smem_addr(&bars.full[last]));
+          bars.tile[slot] = tile;
+          mbar_arrive(smem_addr(&bars.tile_full[slot]));
+        }
+        if (t >= tiles) break;  // that was the tile without columns
+        if (++slot == kTileSlots) {
+          slot = 0;
+          slot_phase ^= 1u;
         }
       }
     }
-  } else {
-    // ----------------------------------------------------------- scheduler
-    const void* const offsets = p.offsets;
-    const bool wide = p.offsets_64;
-    const int32_t groups = p.groups, all_rows = p.k_grouped ? p.K : p.M, tiles_n = p.tiles_n;
-    // What this launch reads may be written by the kernel before it in the
-    // stream, which each role waits for before its first access to memory
-    // (programmatic launch).
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    int32_t before = 0;
-    for (int32_t e0 = 0; e0 < groups; e0 += 32) {
-      const int32_t e = e0 + lane;
-      // every lane loads one offset; the last also the one behind its 32
-      int32_t lo = e <= groups ? read_offset(offsets, wide, all_rows, e) : all_rows;
-      const int32_t behind = lane == 31 && e < groups ? read_offset(offsets, wide, all_rows, e + 1) : 0;
-      const int32_t up = __shfl_down_sync(0xffffffffu, lo, 1);
-      const int32_t rows = e < groups ? max(0, (lane == 31 ? behind : up) - lo) : 0;
-      if (e < groups) {
-        tab.start[e] = lo;
-        tab.rows[e] = rows;
-      }
-      int32_t v = (rows + Cf::kBM - 1) / Cf::kBM * tiles_n;
-#pragma unroll
-      for (int d = 1; d < 32; d *= 2) {
-        const int32_t o = __shfl_up_sync(0xffffffffu, v, d);
-        if (lane >= d) v += o;
-      }
-      if (e < groups) tab.cum[e + 1] = before + v;
-      before += __shfl_sync(0xffffffffu, v, 31);
-    }
-    if (lane == 0) tab.cum[0] = 0;
-    __syncwarp();
-    const int32_t tiles = p.k_grouped ? groups * p.tiles_m * tiles_n : before;
-    int32_t cursor = 0;
-    for (int32_t t = first;; t += stride) {
-      GTile tile = {};
-      if (t < tiles) tile = tile_at<Cf::kBM, BN, Cf::kKB>(p, tab, t, part, cursor, lane);
-      if (t == first) start();
-      if (!warp_wait(smem_addr(&bars.tile_empty[slot]), slot_phase ^ 1u, abort_flag, kSiteScheduler, lane)) break;
-      if (lane == 0) {
-        bars.tile[slot] = tile;
-        mbar_arrive(smem_addr(&bars.tile_full[slot]));
-      }
-      if (t >= tiles) break;  // that was the tile without columns
-      if (++slot == kTileSlots) {
-        slot = 0;
-        slot_phase ^= 1u;
-      }
-    }
-  }
   } else {
     if constexpr (kMoveRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     start();
@@ -931,18 +945,18 @@ __global__ void __launch_bounds__(kThreadsG, 1)
             break;
         } else {
 #pragma unroll
-        for (int c = 0; c < Cf::kChunks; ++c) {
-          if (!warp_ok) break;
-          if (fills > 0) {
-            tmem_ld_32x32b_x32(tm() + (uint32_t)(acc * BN + c * 32), v[0]);
-          } else {
+          for (int c = 0; c < Cf::kChunks; ++c) {
+            if (!warp_ok) break;
+            if (fills > 0) {
+              tmem_ld_32x32b_x32(tm() + (uint32_t)(acc * BN + c * 32), v[0]);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[0][i] = 0.f;
+              for (int i = 0; i < 32; ++i) v[0][i] = 0.f;
+            }
+            const int ncol = min(32, cols - c * 32);
+            if (row_ok && ncol > 0) emit32(p, row + c * 32 * el, v[0], ncol);
+            __syncwarp();
           }
-          const int ncol = min(32, cols - c * 32);
-          if (row_ok && ncol > 0) emit32(p, row + c * 32 * el, v[0], ncol);
-          __syncwarp();
-        }
         }
         if (fills > 0) {
           release(acc);

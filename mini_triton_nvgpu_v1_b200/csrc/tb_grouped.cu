@@ -778,7 +778,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           mbar_expect_tx(ready0, (uint32_t)(mine * p.split) * (uint32_t)((cols + 31) / 32 * 128));
         if (q * 32 == r0) {
           // every CTA has read the rows before
-          if (!warp_poll(consumed0, red_phase ^ 1u, abort_flag, kSiteCluster, lane)) return false;
+          if (!warp_poll<true>(consumed0, red_phase ^ 1u, abort_flag, kSiteCluster, lane)) return false;
           const uint32_t owner = (uint32_t)lane & (uint32_t)(p.split - 1);
           const uint32_t to = map_to_cta(red0 + (uint32_t)(part * per + (lane >> p.split_log2)) * Cf::kRedStride, owner);
           const uint32_t bar = map_to_cta(ready0, owner);
@@ -796,7 +796,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
             }
           }
         }
-        if (!warp_poll(ready0, red_phase, abort_flag, kSiteCluster, lane)) return false;
+        if (!warp_poll<true>(ready0, red_phase, abort_flag, kSiteCluster, lane)) return false;
         for (int i = warp - 4; i < mine; i += 8) {
 #pragma unroll
           for (int h = 0; h < BN / 128; ++h) {  // four columns of each 128 to a lane
@@ -843,13 +843,15 @@ __global__ void __launch_bounds__(kThreadsG, 1)
         const float *sa = nullptr, *sb = nullptr;
         int64_t sb_col[4] = {0, 0, 0, 0};
         float xa = 1.f, xb = 1.f, xc[4] = {0.f, 0.f, 0.f, 0.f};
+        // (Plain loads: the kernel before this one may have written them while
+        // this one was already resident.)
         auto fetch = [&]() {
-          xa = __ldg(sa);
+          xa = *sa;
           sa += p.sa.sk;
-          if constexpr (KIND == kByte) xb = __ldg(sb);
+          if constexpr (KIND == kByte) xb = *sb;
           if constexpr (KIND == kByteCol) {
 #pragma unroll
-            for (int j = 0; j < Cf::kHalfCols / 32; ++j) xc[j] = __ldg(sb + sb_col[j]);
+            for (int j = 0; j < Cf::kHalfCols / 32; ++j) xc[j] = sb[sb_col[j]];
           }
           sb += p.sb.sk;
         };
@@ -986,7 +988,8 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     }
     // Nothing of another CTA is on its way to this one any more (a cluster
     // barrier at the end took 1200 cycles).
-    if (Cf::kShares && p.split > 1 && ok) warp_poll(smem_addr(&bars.consumed), red_phase ^ 1u, abort_flag, kSiteCluster, lane);
+    if (Cf::kShares && p.split > 1 && ok)
+      warp_poll<true>(smem_addr(&bars.consumed), red_phase ^ 1u, abort_flag, kSiteCluster, lane);
   }
 
   __syncthreads();

@@ -53,15 +53,21 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 
 // warp_wait without the blocking probe: the warp polls until the phase is
 // complete, for waits whose every cycle is on the critical path (a blocked
-// try_wait wakes up hundreds of cycles after the phase completes).
+// try_wait wakes up hundreds of cycles after the phase completes). CLUSTER:
+// the barrier is arrived on by, or hands over data from, other CTAs of the cluster.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool warp_poll(uint32_t bar, uint32_t parity, volatile int* abort_flag,
                                           uint32_t site, int lane) {
-  if (__all_sync(0xffffffffu, tb::sm100::mbar_test_wait(bar, parity))) return true;
+  auto probe = [&]() {
+    if constexpr (CLUSTER) return tb::sm100::mbar_test_wait_cluster(bar, parity);
+    else return tb::sm100::mbar_test_wait(bar, parity);
+  };
+  if (__all_sync(0xffffffffu, probe())) return true;
   const long long t0 = clock64();
   while (true) {
 #pragma unroll 1
     for (int i = 0; i < 32; ++i)
-      if (__all_sync(0xffffffffu, tb::sm100::mbar_test_wait(bar, parity))) return true;
+      if (__all_sync(0xffffffffu, probe())) return true;
     int stop = 0;
     if (lane == 0) {
       stop = *abort_flag;

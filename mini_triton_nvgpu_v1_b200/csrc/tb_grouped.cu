@@ -160,6 +160,7 @@ struct GParams {
   int32_t groups;
   int32_t M, N, K;        // rows grouped: A is M × K; K grouped: A is K × M, D is K × N (K = rows of both)
   int32_t tiles_m, tiles_n;  // K grouped: tiles of one group; rows grouped: tiles_n only
+  int32_t most_tiles;     // as many as offsets that do not fall can give
   const void* offsets;    // groups + 1 entries, or null: one group of all rows
   int32_t offsets_64;
   int32_t a_mn, b_kmaj;
@@ -681,7 +682,8 @@ __global__ void __launch_bounds__(kThreadsG, 1)
       // ----------------------------------------------------------- scheduler
       const void* const offsets = p.offsets;
       const bool wide = p.offsets_64;
-      const int32_t groups = p.groups, all_rows = p.k_grouped ? p.K : p.M, tiles_n = p.tiles_n;
+      const int32_t groups = p.groups, all_rows = p.k_grouped ? p.K : p.M, tiles_n = p.tiles_n,
+                    most_tiles = p.most_tiles;
       // What this launch reads may be written by the kernel before it in the
       // stream, which each role waits for before its first access to memory
       // (programmatic launch).
@@ -698,14 +700,18 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           tab.start[e] = lo;
           tab.rows[e] = rows;
         }
+        // Offsets that fall and rise again give the same rows to several
+        // groups; the sums stop at what others can reach, so they fit in 32
+        // bits and the work is bounded whatever the offsets are.
         int32_t v = (rows + Cf::kBM - 1) / Cf::kBM * tiles_n;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
           const int32_t o = __shfl_up_sync(0xffffffffu, v, d);
-          if (lane >= d) v += o;
+          if (lane >= d) v = min(v + o, most_tiles);
         }
-        if (e < groups) tab.cum[e + 1] = before + v;
-        before += __shfl_sync(0xffffffffu, v, 31);
+        v = min(before + v, most_tiles);
+        if (e < groups) tab.cum[e + 1] = v;
+        before = __shfl_sync(0xffffffffu, v, 31);
       }
       if (lane == 0) tab.cum[0] = 0;
       __syncwarp();
@@ -1318,6 +1324,7 @@ tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int
   p.tiles_n = (int32_t)cdiv(n, bn);
   L.tiles = p.k_grouped ? groups * p.tiles_m * p.tiles_n
                         : (p.M / (pair ? 256 : 128) + std::min<int64_t>(groups, p.M)) * p.tiles_n;
+  p.most_tiles = (int32_t)L.tiles;
   return pair        ? launch_tile<256, 2>(L, dev, stream)
          : bn == 256 ? launch_tile<256, 1>(L, dev, stream)
                      : launch_tile<128, 1>(L, dev, stream);

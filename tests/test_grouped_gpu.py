@@ -464,3 +464,32 @@ def test_calls_follow_the_work_before_them(cuda):
         assert torch.equal(c.double(), _reference(values[i % 6], W, torch.zeros_like(c), ends, 0))
         # e4m3: off by at most 2^-4 relative, and half its least step (2^-10) in units of the scale below that
         assert ((v - c).abs() <= 2.0 ** -4 * c.abs() + 2.0 ** -10 * c.abs().amax() / 448).all()
+
+
+def test_offsets_that_fall_and_rise_stay_inside(cuda):
+    """Rows in several groups: every group has the same weights, so that each gives the same rows."""
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(10)
+    A, B = _ints((300, 64), g, torch.float16), _ints((1, 64, 64), g, torch.float16)
+    C = torch.full((302, 64), 7.0, device="cuda")
+    off = torch.tensor([0, 300] * 20 + [0], dtype=torch.int32, device="cuda")   # 20 groups of all rows among 40
+    tb.grouped_matmul(A, B.repeat(40, 1, 1), C[1:301], off, beta=0)
+    assert torch.equal(C[1:301].double(), A.double() @ B[0].double())
+    assert (C[0] == 7).all() and (C[301] == 7).all()
+    tb.device_status()
+
+
+@pytest.mark.parametrize("beta", [0.5, 2, -1, None])
+def test_beta_is_zero_or_one(cuda, beta):
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    A, B = torch.ones(4, 64, device="cuda").half(), torch.ones(1, 64, 64, device="cuda").half()
+    off, C = torch.tensor([0, 4], dtype=torch.int32, device="cuda"), torch.ones(4, 64, device="cuda")
+    for _ in range(2):   # 1.0 and True are 1
+        tb.grouped_matmul(A, B, C, off, beta=1.0)
+        tb.grouped_matmul(A, B, C, off, beta=True)
+        with pytest.raises(tb.TBError, match="beta"):
+            tb.grouped_matmul(A, B, C, off, beta=beta)
+    assert (C == 257).all()

@@ -93,8 +93,12 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
     PyErr_SetString(PyExc_TypeError, "call(op, tensors..., x, y)");
     return nullptr;
   }
+  if (!PyLong_Check(args[n - 2]) || !PyLong_Check(args[n - 1])) return PyLong_FromLong(-1);
   const int64_t x = PyLong_AsLongLong(args[n - 2]), y = PyLong_AsLongLong(args[n - 1]);
-  if (PyErr_Occurred()) return nullptr;
+  if (PyErr_Occurred()) {  // beyond 64 bits
+    PyErr_Clear();
+    return PyLong_FromLong(-1);
+  }
   Signature s;
   const at::Tensor* t[kMaxTensors];
   if (!sign(args + 1, op, x, y, &s, t)) return PyLong_FromLong(-1);

@@ -97,13 +97,18 @@ def _batch(t, name: str) -> int:
     e, r, c = t.shape
     if e <= 1 or t.numel() == 0:
         return max(1, r * c)
+    _apart(t, name)
+    return t.stride(0)
+
+
+def _apart(t, name: str) -> None:
+    """Refuses a t with two entries in one place."""
     spans = sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1)
     reach = 1
     for st, sz in spans:
         if st < reach:
-            raise _bad(f"the matrices of {name} overlap", TB_ERR_UNSUPPORTED)
+            raise _bad(f"entries of {name} overlap", TB_ERR_UNSUPPORTED)
         reach = st * (sz - 1) + reach
-    return t.stride(0)
 
 
 def _check_offsets(offsets, groups: int) -> int:
@@ -206,7 +211,7 @@ def grouped_matmul(A, B, Cm, offsets, *, beta: int = 1, workspace=None, stream=N
     _call(dev, stream, _lib.tb_grouped_matmul, d, A.data_ptr(), lda, B.data_ptr(), ldb, stride_b, Cm.data_ptr(), ldc,
           offsets.data_ptr(), ws, nbytes)
     if even:
-        _remember(_ROWS, A, B, Cm, offsets, beta, 0, d, (lda, ldb, stride_b, ldc), None, None)
+        _remember(_ROWS, A, B, Cm, offsets, int(beta), 0, d, (lda, ldb, stride_b, ldc), None, None)
     return Cm
 
 
@@ -241,7 +246,7 @@ def grouped_matmul_wgrad(A, D, G, offsets, *, beta: int = 1, workspace=None, str
     _call(dev, stream, _lib.tb_grouped_matmul_wgrad, d, A.data_ptr(), lda, D.data_ptr(), ldd, G.data_ptr(), ldg,
           stride_g, offsets.data_ptr(), ws, nbytes)
     if not (lda * 2 % 16 or ldd * 2 % 16):
-        _remember(_WGRAD, A, D, G, offsets, beta, 0, d, (lda, ldd, ldg, stride_g), None, None)
+        _remember(_WGRAD, A, D, G, offsets, int(beta), 0, d, (lda, ldd, ldg, stride_g), None, None)
     return G
 
 
@@ -285,15 +290,15 @@ def quantize_fp8(X, Q=None, S=None, *, block=(1, 128), stream=None):
     batched = X.dim() == 3
     d = _capi.tb_quantize_desc()
     d.batch, d.rows, d.cols = (X.shape[0] if batched else 1), rows, cols
-    d.block_rows, d.block_cols, d.x_dtype = br, bc, _OUT[X.dtype]
-    if batched:
-        _batch(Q, "Q")
-        _batch(S, "S")
+    d.block_rows, d.block_cols, d.x_dtype = int(br), int(bc), _OUT[X.dtype]
+    if X.numel():
+        _apart(Q, "Q")
+        _apart(S, "S")
     ints = (_rows(X, "X"), X.stride(0) if batched else 0, _rows(Q, "Q"), Q.stride(0) if batched else 0,
             S.stride(0) if batched else 0, S.stride(-2), S.stride(-1))
     _call(dev, stream, _lib.tb_quantize_blocks, d, X.data_ptr(), *ints[:2], Q.data_ptr(), *ints[2:4], S.data_ptr(),
           *ints[4:])
-    _remember(_QUANTIZE, X, Q, S, br, bc, d, ints, None, None)
+    _remember(_QUANTIZE, X, Q, S, int(br), int(bc), d, ints, None, None)
     return Q, S
 
 
@@ -343,7 +348,7 @@ def matmul_fp8(A, SA, B, SB, Cm, *, beta: int = 1, workspace=None, stream=None):
     _call(dev, stream, _lib.tb_matmul_blockscaled, d, A.data_ptr(), lda, sa, B.data_ptr(), ldb, sb, Cm.data_ptr(), ldc,
           ws, nbytes)
     if not (lda % 16 or ldb % 16):
-        _remember(_BYTES, A, SA, B, SB, Cm, beta, 0, d, (lda, ldb, ldc), sa, sb)
+        _remember(_BYTES, A, SA, B, SB, Cm, int(beta), 0, d, (lda, ldb, ldc), sa, sb)
     return Cm
 
 
@@ -369,5 +374,5 @@ def grouped_matmul_fp8(A, SA, B, SB, Cm, offsets, *, beta: int = 1, workspace=No
     _call(dev, stream, _lib.tb_grouped_matmul_blockscaled, d, A.data_ptr(), lda, sa, B.data_ptr(), ldb, stride_b, sb,
           Cm.data_ptr(), ldc, offsets.data_ptr(), ws, nbytes)
     if even:
-        _remember(_ROWS_BYTES, A, SA, B, SB, Cm, offsets, beta, 0, d, (lda, ldb, stride_b, ldc), sa, sb)
+        _remember(_ROWS_BYTES, A, SA, B, SB, Cm, offsets, int(beta), 0, d, (lda, ldb, stride_b, ldc), sa, sb)
     return Cm

@@ -430,3 +430,12 @@ def test_expert_layer_together(cuda):
         p, q = _spread(qa[lo:hi], sa[lo:hi], 1, 128), _spread(q2[e], s2[e], 128, 128).t()
         assert ((y8[lo:hi].double() - p @ q).abs() <= 140 * 2.0 ** -23 * (p.abs() @ q.abs())).all()
     tb.device_status()
+
+
+def test_scales_that_overlap_are_refused(cuda):
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    X = torch.ones(4, 256, device="cuda")
+    Q = torch.empty(4, 256, dtype=torch.float8_e4m3fn, device="cuda")
+    with pytest.raises(tb.TBError, match="overlap"):
+        tb.quantize_fp8(X, Q, torch.empty(4, 1, device="cuda").expand(4, 2))

@@ -174,3 +174,24 @@ def test_layouts_of_views():
     assert grouped._either(x[:1, :1], "x") in ((False, 1), (True, 1))
     assert grouped._batch(torch.zeros(3, 4, 5), "x") == 20
     assert grouped._batch(torch.zeros(4, 3, 5).transpose(0, 1), "x") == 5
+
+
+def test_outputs_do_not_overlap():
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    from mini_triton_nvgpu_v1_b200 import grouped
+    for t in (torch.zeros(4, 1).expand(4, 3), torch.zeros(3).expand(4, 3), torch.zeros(5).as_strided((2, 3), (2, 1)),
+              torch.zeros(1, 4, 3).expand(2, 4, 3)):
+        with pytest.raises(tb.TBError, match="overlap"):
+            grouped._apart(t, "S")
+    for t in (torch.zeros(4, 3), torch.zeros(4, 3).t(), torch.zeros(6, 8)[::2, ::3], torch.zeros(1).expand(1, 1)):
+        grouped._apart(t, "S")
+
+
+def test_known_calls_take_whole_numbers_only():
+    """A beta or block that is no whole number is left to the checks, not answered by a TypeError."""
+    import torch
+    from mini_triton_nvgpu_v1_b200 import grouped
+    t = torch.zeros(2, 2)
+    for beta in (0.5, 1.0, None, 1 << 80, "1"):
+        assert grouped._call0(grouped._ROWS, t, t, t, t, beta, 0) == -1

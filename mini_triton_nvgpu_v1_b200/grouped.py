@@ -46,12 +46,15 @@ def _load_calls():
                           "`python -m mini_triton_nvgpu_v1_b200.build`") from e
     _tbtorch.library(*(C.cast(f, C.c_void_p).value for f in (
         _lib.tb_grouped_matmul, _lib.tb_grouped_matmul_wgrad, _lib.tb_quantize_blocks, _lib.tb_matmul_blockscaled,
-        _lib.tb_grouped_matmul_blockscaled)))
+        _lib.tb_grouped_matmul_blockscaled, _lib.tb_grouped_matmul_workspace_bytes,
+        _lib.tb_grouped_matmul_wgrad_workspace_bytes)))
     return _tbtorch
 
 
 # Calls like an earlier one, by the tensors' sizes, strides, types and device:
-# _call0(op, tensors..., x, y) is 0 when it ran them, -1 when it knows no such call.
+# _call0(op, tensors..., x, y) is 0 when it ran them, -1 when it knows no such
+# call or has to leave the copy of its operands in the caller's workspace to the
+# long way.
 _calls = _load_calls()
 _call0, _remember = _calls.call, _calls.remember
 _ROWS, _WGRAD, _QUANTIZE, _BYTES, _ROWS_BYTES = range(5)
@@ -162,7 +165,7 @@ def _call(dev: int, stream, fn, *args) -> None:
 
 
 def _setup_grouped(A, B, Cm, offsets, beta, eight_bit: bool):
-    """(device, desc, lda, ldb, stride_b, ldc, whether every row begins on 16 bytes if the bases do)."""
+    """(desc, lda, ldb, stride_b, ldc)."""
     if A.dim() != 2 or B.dim() != 3 or Cm.dim() != 2:
         raise _bad("grouped products take A [rows, k], B [groups, k, n] and C [rows, n]")
     rows, k = A.shape
@@ -183,10 +186,7 @@ def _setup_grouped(A, B, Cm, offsets, beta, eight_bit: bool):
     b_col, ldb = _either(B, "B")
     lda, ldc = _rows(A, "A"), _rows(Cm, "C")
     d = _desc(groups, rows, n, k, ab, _OUT[Cm.dtype], beta, False, b_col, long_)
-    stride_b = _batch(B, "B")
-    el = 1 if eight_bit else 2
-    even = not (lda * el % 16 or ldb * el % 16 or stride_b * el % 16)
-    return d, lda, ldb, stride_b, ldc, even
+    return d, lda, ldb, _batch(B, "B"), ldc
 
 
 def _need(d, A, lda, B, ldb, stride_b) -> int:
@@ -200,18 +200,17 @@ def grouped_matmul(A, B, Cm, offsets, *, beta: int = 1, workspace=None, stream=N
     [rows, n] f32, f16 or bf16, offsets groups + 1 int32 or int64 on the
     device. Rows outside every group keep what C held. Returns C."""
     if stream is None:
-        code = _call0(_ROWS, A, B, Cm, offsets, beta, 0)
+        code = _call0(_ROWS, A, B, Cm, offsets, beta, workspace is not None)
         if code >= 0:
             if code:
                 _check(code)
             return Cm
     dev = _same_device(A=A, B=B, C=Cm, offsets=offsets)
-    d, lda, ldb, stride_b, ldc, even = _setup_grouped(A, B, Cm, offsets, beta, False)
+    d, lda, ldb, stride_b, ldc = _setup_grouped(A, B, Cm, offsets, beta, False)
     ws, nbytes, _kept = _scratch(_need(d, A, lda, B, ldb, stride_b), workspace, Cm.device, stream)
     _call(dev, stream, _lib.tb_grouped_matmul, d, A.data_ptr(), lda, B.data_ptr(), ldb, stride_b, Cm.data_ptr(), ldc,
           offsets.data_ptr(), ws, nbytes)
-    if even:
-        _remember(_ROWS, A, B, Cm, offsets, int(beta), 0, d, (lda, ldb, stride_b, ldc), None, None)
+    _remember(_ROWS, A, B, Cm, offsets, int(beta), 0, d, (lda, ldb, stride_b, ldc), None, None)
     return Cm
 
 
@@ -221,7 +220,7 @@ def grouped_matmul_wgrad(A, D, G, offsets, *, beta: int = 1, workspace=None, str
     A [rows, k] and D [rows, n] f16 or bf16, G [groups, k, n] f32, f16 or
     bf16. A group without rows gets beta·G[e]. Returns G."""
     if stream is None:
-        code = _call0(_WGRAD, A, D, G, offsets, beta, 0)
+        code = _call0(_WGRAD, A, D, G, offsets, beta, workspace is not None)
         if code >= 0:
             if code:
                 _check(code)
@@ -245,8 +244,7 @@ def grouped_matmul_wgrad(A, D, G, offsets, *, beta: int = 1, workspace=None, str
     ws, nbytes, _kept = _scratch(need, workspace, G.device, stream)
     _call(dev, stream, _lib.tb_grouped_matmul_wgrad, d, A.data_ptr(), lda, D.data_ptr(), ldd, G.data_ptr(), ldg,
           stride_g, offsets.data_ptr(), ws, nbytes)
-    if not (lda * 2 % 16 or ldd * 2 % 16):
-        _remember(_WGRAD, A, D, G, offsets, int(beta), 0, d, (lda, ldd, ldg, stride_g), None, None)
+    _remember(_WGRAD, A, D, G, offsets, int(beta), 0, d, (lda, ldd, ldg, stride_g), None, None)
     return G
 
 
@@ -323,7 +321,7 @@ def matmul_fp8(A, SA, B, SB, Cm, *, beta: int = 1, workspace=None, stream=None):
     n or ceil(n / 128)]; C [m, n] f32, f16 or bf16. The sum over a block and
     over the blocks is in f32. Returns C."""
     if stream is None:
-        code = _call0(_BYTES, A, SA, B, SB, Cm, beta, 0)
+        code = _call0(_BYTES, A, SA, B, SB, Cm, beta, workspace is not None)
         if code >= 0:
             if code:
                 _check(code)
@@ -347,8 +345,7 @@ def matmul_fp8(A, SA, B, SB, Cm, *, beta: int = 1, workspace=None, stream=None):
     ws, nbytes, _kept = _scratch(_need(d, A, lda, B, ldb, 0), workspace, Cm.device, stream)
     _call(dev, stream, _lib.tb_matmul_blockscaled, d, A.data_ptr(), lda, sa, B.data_ptr(), ldb, sb, Cm.data_ptr(), ldc,
           ws, nbytes)
-    if not (lda % 16 or ldb % 16):
-        _remember(_BYTES, A, SA, B, SB, Cm, int(beta), 0, d, (lda, ldb, ldc), sa, sb)
+    _remember(_BYTES, A, SA, B, SB, Cm, int(beta), 0, d, (lda, ldb, ldc), sa, sb)
     return Cm
 
 
@@ -358,13 +355,13 @@ def grouped_matmul_fp8(A, SA, B, SB, Cm, offsets, *, beta: int = 1, workspace=No
     transposed view) with SB [groups, ceil(k / 128), n or ceil(n / 128)].
     Returns C."""
     if stream is None:
-        code = _call0(_ROWS_BYTES, A, SA, B, SB, Cm, offsets, beta, 0)
+        code = _call0(_ROWS_BYTES, A, SA, B, SB, Cm, offsets, beta, workspace is not None)
         if code >= 0:
             if code:
                 _check(code)
             return Cm
     dev = _same_device(A=A, SA=SA, B=B, SB=SB, C=Cm, offsets=offsets)
-    d, lda, ldb, stride_b, ldc, even = _setup_grouped(A, B, Cm, offsets, beta, True)
+    d, lda, ldb, stride_b, ldc = _setup_grouped(A, B, Cm, offsets, beta, True)
     rows, k = A.shape
     groups, _, n = B.shape
     if SA.dim() != 2 or SA.shape[0] != rows:
@@ -373,6 +370,5 @@ def grouped_matmul_fp8(A, SA, B, SB, Cm, offsets, *, beta: int = 1, workspace=No
     ws, nbytes, _kept = _scratch(_need(d, A, lda, B, ldb, stride_b), workspace, Cm.device, stream)
     _call(dev, stream, _lib.tb_grouped_matmul_blockscaled, d, A.data_ptr(), lda, sa, B.data_ptr(), ldb, stride_b, sb,
           Cm.data_ptr(), ldc, offsets.data_ptr(), ws, nbytes)
-    if even:
-        _remember(_ROWS_BYTES, A, SA, B, SB, Cm, offsets, int(beta), 0, d, (lda, ldb, stride_b, ldc), sa, sb)
+    _remember(_ROWS_BYTES, A, SA, B, SB, Cm, offsets, int(beta), 0, d, (lda, ldb, stride_b, ldc), sa, sb)
     return Cm

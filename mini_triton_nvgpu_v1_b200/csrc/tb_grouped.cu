@@ -113,6 +113,9 @@ struct GCfg {
   // One CTA's tile may be shared by a cluster, but not with 128 sums per
   // thread: the exchange does not fit beside them into the registers.
   static constexpr bool kShares = G == 1 && !(kSums && BN == 256);
+  // Outputs that no vector access reaches go through emit32_spread, for the
+  // same reason not from 128 sums (the spills made e4m3 8192³ 1.5 times as long).
+  static constexpr bool kSpreads = !(kSums && BN == 256);
   static constexpr uint32_t kRedStride = (BN + 4) * 4;  // bytes per row of the cluster's partial sums
   static constexpr uint32_t kRedBytes = 32 * kRedStride;  // 32 rows at a time
 };
@@ -271,6 +274,107 @@ __device__ __forceinline__ void st_32(void* q, const uint32_t* w) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(q), "r"(w[0]), "r"(w[1]),
                "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
+}
+
+// Row lane of n registers to register lane of n rows, in every n lanes: n − 1
+// exchanges of half the registers with the lane n / 2, … 1 away. Its own inverse.
+template <typename T, int N>
+__device__ __forceinline__ void transpose(T (&v)[N], int lane) {
+#pragma unroll
+  for (int d = N / 2; d > 0; d /= 2) {
+    const bool up = lane & d;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i & d) continue;
+      const T got = __shfl_xor_sync(0xffffffffu, up ? v[i] : v[i + d], d);
+      if (up) v[i] = got;
+      else v[i + d] = got;
+    }
+  }
+}
+
+// beta·C + v of `ncol` of 32 consecutive columns, whatever the alignment: v is
+// a lane's row, which begins at q; the first `rows` lanes' rows are stored. The
+// values are transposed in registers, so that an access of the warp covers
+// consecutive columns of one row (f32) or the 32-bit words of two (16 bits; a
+// row that begins inside a word has its first column alone). Each lane storing
+// its own row, an element at a time, touched 32 sectors with every access
+// (5481 × 2679 of 8-bit operands, k = 128: bf16 143 µs, now 28.5; f32 98, now 31).
+template <int KIND>
+__device__ __forceinline__ void emit32_spread(const GParams& p, char* q, float (&v)[32], int rows, int ncol, int lane) {
+  if (KIND == kHalfSum || (KIND != kHalf && p.c_dtype == TB_F32)) {
+    const int64_t step = p.ldc * 4;
+    transpose(v, lane);
+    if (lane >= ncol) return;
+    q += lane * (4 - step);
+    constexpr int kAhead = 4;  // rows whose loads run together
+#pragma unroll
+    for (int i0 = 0; i0 < 32; i0 += kAhead) {
+      if (i0 >= rows) break;
+      if (p.beta) {
+        float c[kAhead];
+        const char* at = q;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          c[i] = 0.f;
+          if (i0 + i < rows) c[i] = *reinterpret_cast<const float*>(at);
+          at += step;
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) v[i0 + i] += c[i];
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (i0 + i < rows) *reinterpret_cast<float*>(q) = v[i0 + i];
+        q += step;
+        asm volatile("" : "+l"(q));  // one address, not 32
+      }
+    }
+    return;
+  }
+  const int64_t step = p.ldc * 2;
+  const bool odd = reinterpret_cast<uintptr_t>(q) & 2, mine = lane < rows;
+  const int half = lane & 16, x = lane & 15;
+  char* const first = q + (half - lane) * step;  // of this half's 16 rows
+  // word x of row i of the 16: its columns and their address
+  auto each_word = [&](auto&& f) {
+    char* at = first;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int col = 2 * x + (int)((reinterpret_cast<uintptr_t>(at) >> 1) & 1);
+      if (half + i < rows && col < ncol) f(i, at + col * 2, col + 1 < ncol);
+      at += step;
+      asm volatile("" : "+l"(at));
+    }
+  };
+  if (p.beta) {
+    uint32_t c[16] = {};
+    each_word([&](int i, const char* at, bool both) {
+      if (both) c[i] = *reinterpret_cast<const uint32_t*>(at);
+      else c[i] = *reinterpret_cast<const unsigned short*>(at);
+    });
+    __syncwarp();
+    transpose(c, lane);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float2 u = unpack2(p, c[j]);
+      v[2 * j] += odd ? 0.f : u.x;
+      v[2 * j + 1] += odd ? u.x : u.y;
+      if (j < 15) v[2 * j + 2] += odd ? u.y : 0.f;
+    }
+    if (odd && mine) v[0] += load_out(p, q);
+  }
+  uint32_t w[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    w[j] = pack2(p, odd ? v[2 * j + 1] : v[2 * j], odd ? (j < 15 ? v[2 * j + 2] : 0.f) : v[2 * j + 1]);
+  if (odd && mine) store_out(p, q, v[0]);
+  __syncwarp();
+  transpose(w, lane);
+  each_word([&](int i, char* at, bool both) {
+    if (both) *reinterpret_cast<uint32_t*>(at) = w[i];
+    else *reinterpret_cast<unsigned short*>(at) = (unsigned short)w[i];
+  });
 }
 
 // beta·C + v of `ncol` of 32 consecutive columns at q.
@@ -952,18 +1056,28 @@ __global__ void __launch_bounds__(kThreadsG, 1)
                 })))
             break;
         } else {
+          auto chunks = [&](auto&& emit) {
 #pragma unroll
-          for (int c = 0; c < Cf::kChunks; ++c) {
-            if (!warp_ok) break;
-            if (fills > 0) {
-              tmem_ld_32x32b_x32(tm() + (uint32_t)(acc * BN + c * 32), v[0]);
-            } else {
+            for (int c = 0; c < Cf::kChunks; ++c) {
+              if (!warp_ok) break;
+              if (fills > 0) {
+                tmem_ld_32x32b_x32(tm() + (uint32_t)(acc * BN + c * 32), v[0]);
+              } else {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[0][i] = 0.f;
+                for (int i = 0; i < 32; ++i) v[0][i] = 0.f;
+              }
+              const int ncol = min(32, cols - c * 32);
+              if (ncol > 0) emit(row + c * 32 * el, ncol);
+              __syncwarp();
             }
-            const int ncol = min(32, cols - c * 32);
-            if (row_ok && ncol > 0) emit32(p, row + c * 32 * el, v[0], ncol);
-            __syncwarp();
+          };
+          if (!Cf::kSpreads || p.vec) {
+            chunks([&](char* at, int ncol) {
+              if (row_ok) emit32(p, at, v[0], ncol);
+            });
+          } else {
+            const int32_t rows = field(&GTile::rows) - (row_in_tile - lane);  // of this warp
+            chunks([&](char* at, int ncol) { emit32_spread<KIND>(p, at, v[0], rows, ncol, lane); });
           }
         }
         if (fills > 0) {
@@ -982,10 +1096,20 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           const bool row_ok = row_in_tile < field(&GTile::rows);
           const int32_t cols = field(&GTile::cols) - c_half;
           char* row = row_at();
+          if (!Cf::kSpreads || p.vec) {
 #pragma unroll
-          for (int c = 0; c < Cf::kChunks; ++c) {
-            const int ncol = min(32, cols - c * 32);
-            if (row_ok && ncol > 0) emit32(p, row + c * 32 * el, v[c], ncol);
+            for (int c = 0; c < Cf::kChunks; ++c) {
+              const int ncol = min(32, cols - c * 32);
+              if (row_ok && ncol > 0) emit32(p, row + c * 32 * el, v[c], ncol);
+            }
+          } else if constexpr (Cf::kSpreads) {
+            const int32_t rows = field(&GTile::rows) - (row_in_tile - lane);  // of this warp; may be none
+#pragma unroll
+            for (int c = 0; c < Cf::kChunks; ++c) {
+              const int ncol = min(32, cols - c * 32);
+              if (ncol > 0) emit32_spread<KIND>(p, row + c * 32 * el, v[c], rows, ncol, lane);
+              __syncwarp();
+            }
           }
           __syncwarp();
         }
@@ -1275,7 +1399,8 @@ tbStatus resident_clusters(int dev, int sms, int (&out)[4]) {
 // share of HBM, 45 the most that one SM was seen to draw while others idle,
 // and L2 feeds all SMs together 46 bytes a cycle each (42 where a CTA takes
 // 48 KB at a time). A pair's two cluster barriers take 600 cycles.
-// Storing a tile (16 bytes a cycle and SM) overlaps the next tile's fills.
+// Storing a tile overlaps the next tile's fills: 16 bytes a cycle and SM, or
+// (rows off 16-byte boundaries) 8 elements, 0.6 where a lane stores its own row.
 tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int dev, cudaStream_t stream) {
   GParams& p = L.p;
   int resident[4];  // clusters of 1, 2, 4 and 8 CTAs
@@ -1288,6 +1413,7 @@ tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int
   const int64_t fills = std::max<int64_t>(1, cdiv(p.k_grouped ? cdiv(p.K, std::max<int64_t>(1, groups)) : p.K, 128 / L.el));
   const int ce = p.c_dtype == TB_F32 ? 4 : 2;
   const bool even = p.k_grouped || !p.offsets;  // every group has m rows
+  const bool sums = L.el == 1 || p.c_dtype == TB_F32;
   double best = 0;
   int bn = 0, split = 1;
   bool pair = false;
@@ -1305,7 +1431,7 @@ tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int
     const double near = 128.0 * (is_pair ? 256 : b + tile_rows);  // into the SM, from L2
     const double fill = std::max(std::max(512.0, near / (is_pair || b == 128 ? 46.0 : 42.0)), bytes / std::min(45.0, 23.0 / used));
     const double main = (double)cdiv(fills, s) * fill + (s > 1 ? 300.0 + 300.0 * cdiv((int64_t)tile_rows, 32) : 0.0);
-    const double store = tile_rows * b * ce / 16.0 / (s > 1 ? s : 1);
+    const double store = tile_rows * b / (p.vec ? 16.0 / ce : sums && b == 256 ? 0.6 : 8.0) / (s > 1 ? s : 1);
     const double cycles = rounds * std::max(main, store) + std::min(main, store) + (is_pair ? 600.0 : 0.0);
     if (!bn || cycles < best) {
       best = cycles;
@@ -1315,7 +1441,6 @@ tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int
     }
   };
   if (m > 64) consider(true, 256, 1);
-  const bool sums = L.el == 1 || p.c_dtype == TB_F32;
   for (int b : {128, 256})
     for (int s = 1; s <= (sums && b == 256 ? 1 : 8) && (s == 1 || fills >= 4 * s); s *= 2) consider(false, b, s);
   p.split = split;

@@ -493,3 +493,86 @@ def test_beta_is_zero_or_one(cuda, beta):
         with pytest.raises(tb.TBError, match="beta"):
             tb.grouped_matmul(A, B, C, off, beta=beta)
     assert (C == 257).all()
+
+
+@pytest.mark.parametrize("out", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("eight_bit", [False, True])
+def test_outputs_off_vector_boundaries(cuda, eight_bit, out):
+    """Rows that begin anywhere, widths that end anywhere: the places beside the output keep what they held."""
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(16)
+    dt = getattr(torch, out)
+    off, ends = _offsets([3, 0, 130, 33])
+    rows, k = ends[-1], 128
+    A = _ints((rows, k), g, torch.float16, 2)
+    for n, skip, pad, beta in itertools.product([1, 2, 31, 33, 64, 95, 130, 383], [0, 1, 2, 3], [0, 1, 2], [0, 1]):
+        whole = _ints((rows + 1, skip + n + pad), g, dt, 7)
+        C, want = whole[:rows, skip:skip + n], whole.clone()
+        B = _ints((4, k, n), g, torch.float16, 2)
+        want[:rows, skip:skip + n] = _reference(A, B, C, ends, beta).to(dt)
+        if eight_bit:
+            one = torch.ones(rows, 1, device="cuda")
+            f8 = torch.float8_e4m3fn
+            SB = torch.ones(4, 1, n if n % 2 else (n + 127) // 128, device="cuda")
+            tb.grouped_matmul_fp8(A.to(f8), one, B.to(f8), SB, C, off, beta=beta)
+        else:
+            tb.grouped_matmul(A, B, C, off, beta=beta)
+        assert torch.equal(whole, want), (n, skip, pad, beta)
+    tb.device_status()
+
+
+@pytest.mark.parametrize("out", ["float32", "bfloat16"])
+def test_weight_gradients_off_vector_boundaries(cuda, out):
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(17)
+    dt = getattr(torch, out)
+    off, ends = _offsets([3, 0, 130, 33])
+    A = _ints((ends[-1], 300), g, torch.float16, 2)
+    for n, pad, beta in itertools.product([33, 257, 511], [0, 1], [0, 1]):
+        D = _ints((ends[-1], n), g, torch.float16, 2)
+        whole = _ints((4, 300, n + pad), g, dt, 7)
+        G, want = whole[:, :, pad:], whole.clone()
+        ref = torch.stack([A[lo:hi].double().t() @ D[lo:hi].double() for lo, hi in zip(ends, ends[1:])])
+        want[:, :, pad:] = (ref + beta * G.double()).to(dt)
+        tb.grouped_matmul_wgrad(A, D, G, off, beta=beta)
+        assert torch.equal(whole, want), (n, pad, beta)
+    tb.device_status()
+
+
+def test_repacked_calls_again(cuda):
+    """Operands off 16-byte boundaries, the second time like the first: another stream, a graph, a workspace of one's own."""
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(18)
+    off, ends = _offsets([9, 0, 140, 3])
+    A, B = _ints((ends[-1], 77), g, torch.float16), _ints((4, 77, 51), g, torch.float16)
+    C = torch.zeros(ends[-1], 51, device="cuda")
+    want = _reference(A, B, C, ends, 0).float()
+    for _ in range(3):
+        tb.grouped_matmul(A, B, C, off, beta=0)
+    assert torch.equal(C, want)
+    with pytest.raises(tb.TBError, match="workspace"):
+        tb.grouped_matmul(A, B, C, off, beta=0, workspace=torch.empty(256, dtype=torch.uint8, device="cuda"))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        C2 = torch.zeros_like(C)
+        for _ in range(3):
+            tb.grouped_matmul(A, B, C2, off, beta=1)
+    side.synchronize()
+    assert torch.equal(C2, 3 * want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tb.grouped_matmul(A, B, C, off, beta=1)
+        tb.grouped_matmul_wgrad(A, C2.half(), torch.zeros(4, 77, 51, device="cuda"), off, beta=0)
+    A.copy_(_ints(tuple(A.shape), g, torch.float16))
+    want = C.double() + _reference(A, B, C, ends, 0)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(C.double(), want)
+    tb.device_status()

@@ -61,6 +61,7 @@
 #include <cmath>
 #include <cstring>
 #include <string>
+#include <type_traits>
 
 #include "tb_plan.h"
 #include "tb_sm100.cuh"
@@ -113,7 +114,7 @@ struct GCfg {
   // One CTA's tile may be shared by a cluster, but not with 128 sums per
   // thread: the exchange does not fit beside them into the registers.
   static constexpr bool kShares = G == 1 && !(kSums && BN == 256);
-  // Outputs that no vector access reaches go through emit32_spread, for the
+  // Outputs that no vector access reaches go through emit32_spread, and for the
   // same reason not from 128 sums (the spills made e4m3 8192³ 1.5 times as long).
   static constexpr bool kSpreads = !(kSums && BN == 256);
   static constexpr uint32_t kRedStride = (BN + 4) * 4;  // bytes per row of the cluster's partial sums
@@ -168,7 +169,7 @@ struct GParams {
   int32_t offsets_64;
   int32_t a_mn, b_kmaj;
   uint32_t fmt;           // MMA operand format (idesc bits 7 and 10)
-  int32_t beta, c_dtype, vec;  // vec: bytes of a vector access to C (32, 16 or 0)
+  int32_t beta, c_dtype, vec;  // vec: what C's rows are multiples of (128, 32, 16 bytes, or 0)
   void* C;
   int64_t ldc, group_c;
   GScale sa, sb;
@@ -394,7 +395,7 @@ __device__ __forceinline__ void emit32(const GParams& p, char* q, float (&v)[32]
         v[4 * i] += c.x; v[4 * i + 1] += c.y; v[4 * i + 2] += c.z; v[4 * i + 3] += c.w;
       }
     }
-    if (p.vec == 32) {
+    if (p.vec >= 32) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint32_t w[8];
@@ -425,7 +426,7 @@ __device__ __forceinline__ void emit32(const GParams& p, char* q, float (&v)[32]
   uint32_t w[16];
 #pragma unroll
   for (int j = 0; j < 16; ++j) w[j] = pack2(p, v[2 * j], v[2 * j + 1]);
-  if (p.vec == 32) {
+  if (p.vec >= 32) {
     st_32(q, w);
     st_32(q + 32, w + 8);
   } else {
@@ -433,6 +434,71 @@ __device__ __forceinline__ void emit32(const GParams& p, char* q, float (&v)[32]
     for (int i = 0; i < 4; ++i)
       reinterpret_cast<uint4*>(q)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
   }
+}
+
+// beta·C + v of a warp's 32 rows × 32 columns where the rows of C begin on 128
+// bytes: v is a lane's row, at q. Transposed in registers in units of 32 bytes,
+// so that a store covers 128 (f32) or 64 consecutive bytes of a row. (Weight
+// gradients, f32: 41 × 768 × 1024 from 26 rows 41.2 µs with each lane storing
+// its own row, now 30.8; 8 × 1024 × 1024 from 2048 rows 19.6, now 16.5. Where
+// rows begin off 128 bytes it is the other way round, 41 × 760 × 1048: 39 and
+// 52; warps with fewer rows would pay for the exchange and store no faster.)
+template <int KIND>
+__device__ __forceinline__ void emit32_rows(const GParams& p, char* q, float (&v)[32], int lane) {
+  auto run = [&](auto lanes) {
+    constexpr int L = decltype(lanes)::value;  // lanes of a row: 4 (f32) or 2
+    const int64_t step = p.ldc * L;
+    const int x = lane & (L - 1);
+    char* const first = q + x * (32 - step);
+    uint32_t w[L][8];
+    auto turn = [&]() {  // word x of row i of the L to word i of row x
+#pragma unroll
+      for (int d = L / 2; d > 0; d /= 2) {
+        const bool up = lane & d;
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+          if (i & d) continue;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? w[i][k] : w[i + d][k], d);
+            if (up) w[i][k] = got;
+            else w[i + d][k] = got;
+          }
+        }
+      }
+    };
+    if (p.beta) {
+#pragma unroll
+      for (int i = 0; i < L; ++i) {
+#pragma unroll
+        for (int h = 0; h < 8; h += 4) {
+          const uint4 u = *reinterpret_cast<const uint4*>(first + i * step + 4 * h);
+          w[i][h] = u.x; w[i][h + 1] = u.y; w[i][h + 2] = u.z; w[i][h + 3] = u.w;
+        }
+      }
+      turn();
+#pragma unroll
+      for (int j = 0; j < 8 * L; ++j) {
+        if constexpr (L == 4) {
+          v[j] += __uint_as_float(w[j / 8][j % 8]);
+        } else {
+          const float2 f = unpack2(p, w[j / 8][j % 8]);
+          v[2 * j] += f.x;
+          v[2 * j + 1] += f.y;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8 * L; ++j) {
+      if constexpr (L == 4) w[j / 8][j % 8] = __float_as_uint(v[j]);
+      else w[j / 8][j % 8] = pack2(p, v[2 * j], v[2 * j + 1]);
+    }
+    turn();
+#pragma unroll
+    for (int i = 0; i < L; ++i) st_32(first + i * step, w[i]);
+  };
+  if (KIND == kHalfSum || (KIND != kHalf && p.c_dtype == TB_F32)) run(std::integral_constant<int, 4>());
+  else run(std::integral_constant<int, 2>());
 }
 
 // beta·C + v of `ncol` (at most 4) consecutive columns at q.
@@ -1072,8 +1138,10 @@ __global__ void __launch_bounds__(kThreadsG, 1)
             }
           };
           if (!Cf::kSpreads || p.vec) {
+            const bool whole = p.vec == 128 && row_in_tile - lane + 32 <= field(&GTile::rows);
             chunks([&](char* at, int ncol) {
-              if (row_ok) emit32(p, at, v[0], ncol);
+              if (whole && ncol == 32) emit32_rows<KIND>(p, at, v[0], lane);
+              else if (row_ok) emit32(p, at, v[0], ncol);
             });
           } else {
             const int32_t rows = field(&GTile::rows) - (row_in_tile - lane);  // of this warp
@@ -1097,10 +1165,17 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           const int32_t cols = field(&GTile::cols) - c_half;
           char* row = row_at();
           if (!Cf::kSpreads || p.vec) {
+            bool whole = false;
+            if constexpr (Cf::kSpreads) whole = p.vec == 128 && row_in_tile - lane + 32 <= field(&GTile::rows);
 #pragma unroll
             for (int c = 0; c < Cf::kChunks; ++c) {
               const int ncol = min(32, cols - c * 32);
-              if (row_ok && ncol > 0) emit32(p, row + c * 32 * el, v[c], ncol);
+              bool stored = false;
+              if constexpr (Cf::kSpreads) {
+                stored = whole && ncol == 32;
+                if (stored) emit32_rows<KIND>(p, row + c * 32 * el, v[c], lane);
+              }
+              if (!stored && row_ok && ncol > 0) emit32(p, row + c * 32 * el, v[c], ncol);
             }
           } else if constexpr (Cf::kSpreads) {
             const int32_t rows = field(&GTile::rows) - (row_in_tile - lane);  // of this warp; may be none
@@ -1458,7 +1533,7 @@ tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int
 int c_bytes(int32_t dt) { return dt == TB_F32 ? 4 : 2; }
 
 int vector_bytes(const void* C, int64_t ldc, int64_t group, int el) {
-  for (int b : {32, 16})
+  for (int b : {128, 32, 16})
     if (al(C, b) && ldc * el % b == 0 && group * el % b == 0) return b;
   return 0;
 }

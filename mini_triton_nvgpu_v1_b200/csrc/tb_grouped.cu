@@ -950,11 +950,14 @@ __global__ void __launch_bounds__(kThreadsG, 1)
       for (int r0 = 0; r0 < rows; r0 += 32) {
         const int here = min(32, rows - r0);
         const int mine = (here - part + p.split - 1) >> p.split_log2;  // rows part, part + split, … below `here`
+        // Every CTA has read the rows before. All eight warps wait for it, not
+        // only the senders: a CTA without a row of its own has nothing else to
+        // wait for, and a warp that went on would arrive a second time and stand
+        // in for one that still reads.
+        if (!warp_poll<true>(consumed0, red_phase ^ 1u, abort_flag, kSiteCluster, lane)) return false;
         if (warp == 4 && lane == 0)
           mbar_expect_tx(ready0, (uint32_t)(mine * p.split) * (uint32_t)((cols + 31) / 32 * 128));
         if (q * 32 == r0) {
-          // every CTA has read the rows before
-          if (!warp_poll<true>(consumed0, red_phase ^ 1u, abort_flag, kSiteCluster, lane)) return false;
           const uint32_t owner = (uint32_t)lane & (uint32_t)(p.split - 1);
           const uint32_t to = map_to_cta(red0 + (uint32_t)(part * per + (lane >> p.split_log2)) * Cf::kRedStride, owner);
           const uint32_t bar = map_to_cta(ready0, owner);

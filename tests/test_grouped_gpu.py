@@ -576,3 +576,69 @@ def test_repacked_calls_again(cuda):
     torch.cuda.synchronize()
     assert torch.equal(C.double(), want)
     tb.device_status()
+
+
+# (groups, n, k, output, 8 bits): several tiles to a cluster of 2, 4 or 8 CTAs that share each tile's K range
+SHARED = [(32, 1408, 2048, "f16", False), (10, 4096, 1024, "bf16", False), (24, 2048, 4096, "f32", False),
+          (5, 2048, 4096, "f32", False), (5, 2048, 8192, "bf16", True)]
+
+
+@pytest.mark.parametrize("groups,n,k,out,eight_bit", SHARED)
+@pytest.mark.parametrize("rows", [1, 3, 7, 33, 39])
+def test_shared_tiles_of_fewer_rows_than_ctas(cuda, groups, n, k, out, eight_bit, rows):
+    """Tiles, and last blocks of 32 rows, with fewer rows than the cluster has CTAs, one after another: a CTA without
+    a row may not run ahead of the others."""
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(19)
+    off, ends = _offsets([max(1, rows - e % 3) for e in range(groups)])
+    A, B = _ints((ends[-1], k), g, torch.float16, 2), _ints((groups, n, k), g, torch.float16, 2).transpose(1, 2)
+    C = _ints((ends[-1], n), g, _types(out), 7)
+    want = [_reference(A, B, C, ends, beta).to(C.dtype) for beta in (0, 1)]
+    if eight_bit:
+        f8 = torch.float8_e4m3fn
+        A, B = A.to(f8), B.to(f8)
+        SA, SB = torch.ones(ends[-1], k // 128, device="cuda"), torch.ones(groups, k // 128, n // 128, device="cuda")
+    for i in range(40):
+        got = C.clone()
+        if eight_bit:
+            tb.grouped_matmul_fp8(A, SA, B, SB, got, off, beta=i % 2)
+        else:
+            tb.grouped_matmul(A, B, got, off, beta=i % 2)
+        assert torch.equal(got, want[i % 2]), i
+    tb.device_status()
+
+
+@pytest.mark.parametrize("groups,k,n,rows", [(64, 1, 384, 1024), (64, 33, 384, 1024), (100, 3, 384, 1024),
+                                             (40, 3, 256, 4096)])
+def test_shared_weight_gradients_of_fewer_rows_than_ctas(cuda, groups, k, n, rows):
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(20)
+    off, ends = _offsets([rows + e % 5 for e in range(groups)])
+    A, D = _ints((ends[-1], (k + 7) // 8 * 8), g, torch.bfloat16, 2)[:, :k], _ints((ends[-1], n), g, torch.bfloat16, 2)
+    G = _ints((groups, k, n), g, torch.float32, 7)
+    ref = torch.stack([A[lo:hi].double().t() @ D[lo:hi].double() for lo, hi in zip(ends, ends[1:])])
+    for i in range(40):
+        got = G.clone()
+        tb.grouped_matmul_wgrad(A, D, got, off, beta=i % 2)
+        assert torch.equal(got.double(), ref + i % 2 * G.double()), i
+    tb.device_status()
+
+
+@pytest.mark.parametrize("m", [33, 35, 39])
+def test_shared_8_bit_tiles_of_one_matrix(cuda, m):
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(21)
+    A, B = _ints((m, 4096), g, torch.float16, 2), _ints((4096, 4096), g, torch.float16, 2)
+    want = (A.double() @ B.double()).float()
+    f8, one = torch.float8_e4m3fn, torch.ones(m, 32, device="cuda")
+    A, B = A.to(f8), B.t().contiguous().to(f8).t()
+    for _ in range(40):
+        C = tb.matmul_fp8(A, one, B, torch.ones(32, 32, device="cuda"), torch.zeros(m, 4096, device="cuda"), beta=0)
+        assert torch.equal(C, want)
+    tb.device_status()

@@ -751,6 +751,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           const int32_t fills = field(&GTile::f1) - field(&GTile::f0);
           const int32_t last_valid = min(Cf::kKB, field(&GTile::k_end) - field(&GTile::k0) - (field(&GTile::f1) - 1) * Cf::kKB);
           const int last_steps = (last_valid + Cf::kMmaK - 1) / Cf::kMmaK;
+          const int32_t fixed_at = p.k_grouped && last_valid % Cf::kMmaK != 0 ? fills - 1 : -1;
           done();
           bool here = false;  // the fill at hand was seen to have landed
           for (int32_t f = 0; f < fills; ++f) {
@@ -762,6 +763,8 @@ __global__ void __launch_bounds__(kThreadsG, 1)
               ok = false;
               break;
             }
+            // The other CTA's fixer wrote to its shared memory before it arrived here.
+            if (G == 2 && !Cf::kBytes && f == fixed_at) mbar_test_wait_cluster(full0 + stage * 8, phase);
             tc_fence_after();
             const uint32_t a_lo = (uint32_t)da + (uint32_t)stage * (Cf::kABytes >> 4);
             const uint32_t b_lo = (uint32_t)db + (uint32_t)stage * (Cf::kBBytes >> 4);
@@ -942,6 +945,19 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     // behind a cluster-scope release and read by the others took 4100 cycles
     // from the last fill to the stores.) False: a wait gave up.
     uint32_t red_phase = 0;
+    // Rows read are handed back to the senders of the next ones by an arrival
+    // that is released at cluster scope, so that what was read here is not
+    // overwritten before. The release takes half a microsecond: a tile's last
+    // rows are handed back behind the start of the next tile's sums, or (no next
+    // tile) not at all. (8-bit, K = N = 4096: 16 rows 7.9 µs as with a release of
+    // CTA scope, which orders nothing for the other CTAs; 33 rows 9.4 → 9.9, 128
+    // rows, of three hand-backs inside the tile, 14.2 → 15.7.)
+    bool owed = false;
+    auto hand_back = [&]() {
+      __syncwarp();
+      if (lane < p.split) mbar_arrive_cluster(map_to_cta(smem_addr(&bars.consumed), (uint32_t)lane));
+      owed = false;
+    };
     auto share = [&](auto&& sums) -> bool {
       const int rows = field(&GTile::rows), cols = field(&GTile::cols);
       char* tile = tile_at_c();
@@ -991,8 +1007,8 @@ __global__ void __launch_bounds__(kThreadsG, 1)
             emit4(p, tile + ((int64_t)(r0 + part + (i << p.split_log2)) * p.ldc + c0) * el, s, cols - c0);
           }
         }
-        __syncwarp();
-        if (lane < p.split) mbar_arrive_remote(map_to_cta(consumed0, (uint32_t)lane));
+        if (r0 + 32 < rows) hand_back();
+        else owed = true;
         red_phase ^= 1u;
       }
       return true;
@@ -1002,6 +1018,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     if (Cf::kShares && cluster > 1) cluster_wait();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     while (take(kSiteEpilogue)) {
+      if (Cf::kShares && owed) hand_back();
       // Only the count of accumulations and the scales' places stay in
       // registers during the sums; the rest is read again for the stores.
       const int32_t fills = field(&GTile::f1) - field(&GTile::f0);
@@ -1194,10 +1211,8 @@ __global__ void __launch_bounds__(kThreadsG, 1)
       }
       done();
     }
-    // Nothing of another CTA is on its way to this one any more (a cluster
-    // barrier at the end took 1200 cycles).
-    if (Cf::kShares && p.split > 1 && ok)
-      warp_poll<true>(smem_addr(&bars.consumed), red_phase ^ 1u, abort_flag, kSiteCluster, lane);
+    // The last rows are not handed back, so nothing of another CTA is on its way
+    // to this one any more (a cluster barrier at the end took 1200 cycles).
   }
 
   __syncthreads();

@@ -118,7 +118,6 @@ struct GCfg {
   // same reason not from 128 sums (the spills made e4m3 8192³ 1.5 times as long).
   static constexpr bool kSpreads = !(kSums && BN == 256);
   static constexpr uint32_t kRedStride = (BN + 4) * 4;  // bytes per row of the cluster's partial sums
-  static constexpr uint32_t kRedBytes = 32 * kRedStride;  // 32 rows at a time
 };
 
 // Tiles of every group, built by each CTA from the offsets.
@@ -175,6 +174,7 @@ struct GParams {
   GScale sa, sb;
   int32_t stages;         // ring depth
   int32_t split, split_log2;  // CTAs per cluster that share a tile's K range (G = 1)
+  int32_t block;          // rows whose partial sums they exchange at a time: 32, 64 or 128
   int32_t small_log2;     // log2 of the rows of tmAs's boxes: a K-major A tile of few rows comes in these (G = 1)
 };
 
@@ -558,7 +558,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
   uint8_t* sA = smem;
   uint8_t* sB = smem + (size_t)S * Cf::kABytes;
   uint8_t* red = smem + (size_t)S * Cf::kStageBytes;
-  uint8_t* tail = red + (p.split > 1 ? Cf::kRedBytes : 0u);
+  uint8_t* tail = red + (Cf::kShares && p.split > 1 ? (uint32_t)p.block * Cf::kRedStride : 0u);
   GBars& bars = *reinterpret_cast<GBars*>(tail);
   GroupTable& tab = *reinterpret_cast<GroupTable*>(tail + ((sizeof(GBars) + 15) & ~size_t(15)));
   volatile int* abort_flag = &bars.abort_flag;
@@ -937,7 +937,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
       return static_cast<char*>(p.C) + (group + (int64_t)field(&GTile::row0) * p.ldc + field(&GTile::n0)) * el;
     };
     auto row_at = [&]() { return tile_at_c() + ((int64_t)row_in_tile * p.ldc + c_half) * el; };
-    // The cluster's CTAs hold partial sums of one tile. 32 rows at a time,
+    // The cluster's CTAs hold partial sums of one tile. `block` rows at a time,
     // each sends row r of its own (sums(c): this warp's chunk c) to CTA
     // r mod split, which adds them in CTA order and stores the row. The rows
     // come as st.async, counted on the receiver's barrier: no fence, and the
@@ -947,11 +947,12 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     uint32_t red_phase = 0;
     // Rows read are handed back to the senders of the next ones by an arrival
     // that is released at cluster scope, so that what was read here is not
-    // overwritten before. The release takes half a microsecond: a tile's last
-    // rows are handed back behind the start of the next tile's sums, or (no next
-    // tile) not at all. (8-bit, K = N = 4096: 16 rows 7.9 µs as with a release of
-    // CTA scope, which orders nothing for the other CTAs; 33 rows 9.4 → 9.9, 128
-    // rows, of three hand-backs inside the tile, 14.2 → 15.7.)
+    // overwritten before. The release waits for this warp's stores, half a
+    // microsecond and more: so a block has as many rows as the tiles have, and a
+    // tile's last block is handed back behind the start of the next tile's sums,
+    // or (no next tile) not at all. (8-bit, K = N = 4096, blocks of 32 rows and of
+    // the tile's: 33 rows 9.9 and 8.6 µs, 128 rows 15.7 and 12.8; a release of
+    // CTA scope, which orders nothing for the other CTAs: 9.4 and 14.2.)
     bool owed = false;
     auto hand_back = [&]() {
       __syncwarp();
@@ -961,10 +962,10 @@ __global__ void __launch_bounds__(kThreadsG, 1)
     auto share = [&](auto&& sums) -> bool {
       const int rows = field(&GTile::rows), cols = field(&GTile::cols);
       char* tile = tile_at_c();
-      const int per = 32 >> p.split_log2;  // rows of each CTA in 32
+      const int per = p.block >> p.split_log2;  // rows of each CTA in a block
       const uint32_t red0 = smem_addr(red), ready0 = smem_addr(&bars.ready), consumed0 = smem_addr(&bars.consumed);
-      for (int r0 = 0; r0 < rows; r0 += 32) {
-        const int here = min(32, rows - r0);
+      for (int r0 = 0; r0 < rows; r0 += p.block) {
+        const int here = min(p.block, rows - r0);
         const int mine = (here - part + p.split - 1) >> p.split_log2;  // rows part, part + split, … below `here`
         // Every CTA has read the rows before. All eight warps wait for it, not
         // only the senders: a CTA without a row of its own has nothing else to
@@ -973,15 +974,16 @@ __global__ void __launch_bounds__(kThreadsG, 1)
         if (!warp_poll<true>(consumed0, red_phase ^ 1u, abort_flag, kSiteCluster, lane)) return false;
         if (warp == 4 && lane == 0)
           mbar_expect_tx(ready0, (uint32_t)(mine * p.split) * (uint32_t)((cols + 31) / 32 * 128));
-        if (q * 32 == r0) {
-          const uint32_t owner = (uint32_t)lane & (uint32_t)(p.split - 1);
-          const uint32_t to = map_to_cta(red0 + (uint32_t)(part * per + (lane >> p.split_log2)) * Cf::kRedStride, owner);
+        const int row = q * 32 - r0 + lane;  // of the block
+        if (row >= lane && row - lane < here) {
+          const uint32_t owner = (uint32_t)row & (uint32_t)(p.split - 1);
+          const uint32_t to = map_to_cta(red0 + (uint32_t)(part * per + (row >> p.split_log2)) * Cf::kRedStride, owner);
           const uint32_t bar = map_to_cta(ready0, owner);
 #pragma unroll
           for (int c = 0; c < Cf::kChunks; ++c) {
             if (c_half + c * 32 < cols) {
               const float(&s)[32] = sums(c);
-              if (lane < here) {
+              if (row < here) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                   st_async_f4(to + (uint32_t)(c_half + c * 32 + 4 * i) * 4, bar, s[4 * i], s[4 * i + 1], s[4 * i + 2],
@@ -1007,7 +1009,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
             emit4(p, tile + ((int64_t)(r0 + part + (i << p.split_log2)) * p.ldc + c0) * el, s, cols - c0);
           }
         }
-        if (r0 + 32 < rows) hand_back();
+        if (r0 + p.block < rows) hand_back();
         else owed = true;
         red_phase ^= 1u;
       }
@@ -1396,6 +1398,7 @@ struct Launch {
   int el, bf16;
   int64_t tiles;  // an upper bound of the tiles
   int64_t rows;   // mean rows of a group that has any
+  int64_t tile_rows;  // and of a tile
   int64_t slots;  // clusters at once
   GParams p;
 };
@@ -1413,7 +1416,9 @@ tbStatus launch(Launch& L, int dev, cudaStream_t stream) {
     st = encode(&tb_, 3, L.b, L.el, L.bf16, p.b_kmaj ? Cf::kKB : Cf::kMnBox, p.b_kmaj ? Cf::kBnCta : Cf::kKB, "B");
   if (st != TB_OK) return st;
   p.split_log2 = p.split == 8 ? 3 : p.split == 4 ? 2 : p.split == 2 ? 1 : 0;
-  const size_t fixed = 1024 + kTailBytes + (p.split > 1 ? Cf::kRedBytes : 0);
+  // A block holds the rows that a tile has on average, if the ring keeps three stages beside it.
+  p.block = BN == 128 && L.tile_rows > 64 ? 128 : L.tile_rows > 32 ? 64 : 32;
+  const size_t fixed = 1024 + kTailBytes + (p.split > 1 ? (size_t)p.block * Cf::kRedStride : 0);
   p.stages = (int)std::min<size_t>(kMaxStages, (kSmemLimitG - fixed) / Cf::kStageBytes);
   const size_t smem = fixed + (size_t)p.stages * Cf::kStageBytes;
   auto kern = tb_grouped_sm100_kernel<KIND, BN, G>;
@@ -1500,6 +1505,7 @@ tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int
   tbStatus st = resident_clusters(dev, sms, resident);
   if (st != TB_OK) return st;
   L.rows = rows;
+  L.tile_rows = std::min<int64_t>(p.k_grouped ? p.M : rows, 128);
   const int64_t n = p.N;
   const int64_t m = p.k_grouped ? p.M : rows;
   const int64_t busy = p.k_grouped ? groups : std::min<int64_t>(groups, p.M);

@@ -76,26 +76,32 @@ constexpr int kMaxGroups = 1024;
 constexpr int kMaxStages = 10;
 constexpr size_t kSmemLimitG = 232448;  // 227 KB opt-in per CTA
 
-// kHalf      16-bit operands (f16 / bf16), the whole K range summed in TMEM
-// kHalfSum   16-bit operands, segments of kSumFills fills summed in f32 registers
+// kHalf      16-bit operands (f16 / bf16) and outputs, the whole K range (at most kOneSum) summed in TMEM
+// kHalfSum   16-bit operands, segments of GParams::seg fills summed in f32 registers
 // kByte      8-bit operands (e4m3), a scale of B per 128 columns
 // kByteCol   8-bit operands, a scale of B per column
 enum Kind : int { kHalf = 0, kHalfSum = 1, kByte = 2, kByteCol = 3 };
 // The MMA truncates when it adds to its accumulator: the error of a sum grows
-// with the number of additions and leans one way. An f32 output takes it out
-// of TMEM every 8 fills (512 elements of K, 32 additions) and adds the
-// segments in registers, rounded to nearest. Relative error of f16 products
-// against 64 bits at K = 1032 and 4096: 3.5e-7 and 6.5e-7 (f32 arithmetic by
-// itself: 5.7e-7 and 1.1e-6; one sum in TMEM: 1.3e-6 at 1032). Segments of 4
-// fills gave 3.5e-7 at both and took 4 % longer.
-constexpr int kSumFills = 8;
+// with the number of additions (one for 16 elements of K) and leans one way, and
+// K may be a number of rows without a bound. So a segment of K is taken out of
+// TMEM and the segments are added in registers, rounded to nearest: every 8
+// fills (512 elements of K) for f32 outputs, every 16 for 16-bit outputs, whose
+// own rounding is hundreds of times as large. Relative error of f16 products
+// against 64 bits, f32 outputs: 3.4e-7 at K = 256, 6.5e-7 from K = 512 on, where
+// f32 arithmetic has 4.0e-7 at 512, 5.7e-7 at 1032 and 1.1e-6 at 4096. (Segments
+// of 4 fills: 3.5e-7 from 256 on; 16384 rows over 8 experts of 4096 × 4096 took
+// 534 µs in place of 470, their weight gradient 308 in place of 246.) bf16
+// outputs of K = 4096 and 16384 that are not the nearest value: 0.064 % and
+// 0.063 %; in one sum 0.12 % and 0.47 %, by f32 arithmetic 0.03 %. It costs 2 %
+// (16384 rows, 8 × 4096 × 4096 bf16), and 10 % where rows are off 16 bytes.
+constexpr int kSegF32 = 8, kSegHalf = 16;
+constexpr int64_t kOneSum = 64 * kSegHalf;  // elements of K
 
 // KIND's ring fill is 128 bytes of K: 64 or 128 elements, four MMA K steps.
 template <int KIND, int BN, int G>
 struct GCfg {
   static constexpr bool kBytes = KIND == kByte || KIND == kByteCol;
   static constexpr bool kSums = KIND != kHalf;          // sums held in registers
-  static constexpr int kSegFills = kBytes ? 1 : kSumFills;  // fills per accumulation in TMEM (kSums)
   static constexpr int kEl = kBytes ? 1 : 2;
   static constexpr int kKB = 128 / kEl;                 // K elements per fill
   static constexpr int kMmaK = 32 / kEl;                // K elements per MMA
@@ -114,8 +120,10 @@ struct GCfg {
   // One CTA's tile may be shared by a cluster, but not with 128 sums per
   // thread: the exchange does not fit beside them into the registers.
   static constexpr bool kShares = G == 1 && !(kSums && BN == 256);
-  // Outputs that no vector access reaches go through emit32_spread, and for the
-  // same reason not from 128 sums (the spills made e4m3 8192³ 1.5 times as long).
+  // Outputs that no vector access reaches go through emit32_spread, but for the
+  // same reason not straight from 128 sums: those of 16-bit operands go through
+  // local memory, those of 8-bit operands are stored by the element (either way's
+  // spills made e4m3 products 1.5 to 1.8 times as long).
   static constexpr bool kSpreads = !(kSums && BN == 256);
   static constexpr uint32_t kRedStride = (BN + 4) * 4;  // bytes per row of the cluster's partial sums
 };
@@ -173,6 +181,7 @@ struct GParams {
   int64_t ldc, group_c;
   GScale sa, sb;
   int32_t stages;         // ring depth
+  int32_t seg;            // fills per accumulation in TMEM, a power of two (kinds with sums)
   int32_t split, split_log2;  // CTAs per cluster that share a tile's K range (G = 1)
   int32_t block;          // rows whose partial sums they exchange at a time: 32, 64 or 128
   int32_t small_log2;     // log2 of the rows of tmAs's boxes: a K-major A tile of few rows comes in these (G = 1)
@@ -303,7 +312,7 @@ __device__ __forceinline__ void transpose(T (&v)[N], int lane) {
 // (5481 × 2679 of 8-bit operands, k = 128: bf16 143 µs, now 28.5; f32 98, now 31).
 template <int KIND>
 __device__ __forceinline__ void emit32_spread(const GParams& p, char* q, float (&v)[32], int rows, int ncol, int lane) {
-  if (KIND == kHalfSum || (KIND != kHalf && p.c_dtype == TB_F32)) {
+  if (KIND != kHalf && p.c_dtype == TB_F32) {
     const int64_t step = p.ldc * 4;
     transpose(v, lane);
     if (lane >= ncol) return;
@@ -497,7 +506,7 @@ __device__ __forceinline__ void emit32_rows(const GParams& p, char* q, float (&v
 #pragma unroll
     for (int i = 0; i < L; ++i) st_32(first + i * step, w[i]);
   };
-  if (KIND == kHalfSum || (KIND != kHalf && p.c_dtype == TB_F32)) run(std::integral_constant<int, 4>());
+  if (KIND != kHalf && p.c_dtype == TB_F32) run(std::integral_constant<int, 4>());
   else run(std::integral_constant<int, 2>());
 }
 
@@ -743,6 +752,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           if constexpr (G == 2) umma_commit_pair(bar, 0x3);
           else umma_commit(bar);
         };
+        const int32_t seg_mask = Cf::kBytes ? 0 : p.seg - 1;
         int stage = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool issued_any = false;
@@ -756,8 +766,8 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           bool here = false;  // the fill at hand was seen to have landed
           for (int32_t f = 0; f < fills; ++f) {
             // first and last fill of an accumulation
-            const bool opens = Cf::kSums ? f % Cf::kSegFills == 0 : f == 0;
-            const bool closes = f + 1 == fills || (Cf::kSums && (f + 1) % Cf::kSegFills == 0);
+            const bool opens = Cf::kSums ? (f & seg_mask) == 0 : f == 0;
+            const bool closes = f + 1 == fills || (Cf::kSums && ((f + 1) & seg_mask) == 0);
             if ((opens && !warp_poll(tempty0 + acc * 8, acc_phase ^ 1u, abort_flag, kSiteMma, lane)) ||
                 (!here && !warp_poll(full0 + stage * 8, phase, abort_flag, kSiteMma, lane))) {
               ok = false;
@@ -1068,7 +1078,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           }
           if (fills > 0) fetch();
         }
-        for (int32_t left = fills; left > 0; left -= Cf::kSegFills) {
+        for (int32_t left = fills; left > 0; left -= Cf::kBytes ? 1 : p.seg) {
           const float x = xa * xb;
           float* cs = bars.col_scale[warp - 4];
           if constexpr (KIND == kByteCol) {
@@ -1117,6 +1127,30 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           }
         }
         if (!ok) break;
+        if (KIND == kHalfSum && !Cf::kSpreads && !p.vec) {
+          // 128 sums: through local memory, so that they are not in registers
+          // beside the exchange, and the loop above needs no room for it.
+          if (warp_ok) {
+            float all[Cf::kChunks][32];
+#pragma unroll
+            for (int c = 0; c < Cf::kChunks; ++c)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) unpack_f32x2(sum[c][i], all[c][2 * i], all[c][2 * i + 1]);
+            const int32_t rows = field(&GTile::rows) - (row_in_tile - lane);  // of this warp
+            const int32_t cols = field(&GTile::cols) - c_half;
+            char* row = row_at();
+#pragma unroll 1
+            for (int c = 0; c * 32 < cols && c < Cf::kChunks; ++c) {
+              float one[32];
+#pragma unroll
+              for (int i = 0; i < 32; ++i) one[i] = all[c][i];
+              emit32_spread<KIND>(p, row + c * 32 * el, one, rows, min(32, cols - c * 32), lane);
+              __syncwarp();
+            }
+          }
+          done();
+          continue;
+        }
 #pragma unroll
         for (int c = 0; c < Cf::kChunks; ++c)
 #pragma unroll
@@ -1451,13 +1485,17 @@ tbStatus launch(Launch& L, int dev, cudaStream_t stream) {
   return TB_OK;
 }
 
-// The kind of a tile's kernel, by the operands' and the output's types.
+// Whether a call's sums are held in registers: all but 16-bit outputs of so few
+// elements of K that one accumulation holds them.
+bool sums_in_registers(const Launch& L) { return L.el == 1 || L.p.c_dtype == TB_F32 || L.p.K > kOneSum; }
+
+// The kind of a tile's kernel, by the operands' and the output's types and K.
 template <int BN, int G>
 tbStatus launch_tile(Launch& L, int dev, cudaStream_t stream) {
   if (L.el == 1)
     return L.p.sb.shift ? launch<kByte, BN, G>(L, dev, stream) : launch<kByteCol, BN, G>(L, dev, stream);
-  return L.p.c_dtype == TB_F32 ? launch<kHalfSum, BN, G>(L, dev, stream)
-                               : launch<kHalf, BN, G>(L, dev, stream);
+  L.p.seg = L.p.c_dtype == TB_F32 ? kSegF32 : kSegHalf;
+  return sums_in_registers(L) ? launch<kHalfSum, BN, G>(L, dev, stream) : launch<kHalf, BN, G>(L, dev, stream);
 }
 
 tbStatus resident_clusters(int dev, int sms, int (&out)[4]) {
@@ -1498,7 +1536,8 @@ tbStatus resident_clusters(int dev, int sms, int (&out)[4]) {
 // and L2 feeds all SMs together 46 bytes a cycle each (42 where a CTA takes
 // 48 KB at a time). A pair's two cluster barriers take 600 cycles.
 // Storing a tile overlaps the next tile's fills: 16 bytes a cycle and SM, or
-// (rows off 16-byte boundaries) 8 elements, 0.6 where a lane stores its own row.
+// (rows off 16-byte boundaries) 8 elements, 4 by way of local memory, 0.6 where
+// a lane stores its own row.
 tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int dev, cudaStream_t stream) {
   GParams& p = L.p;
   int resident[4];  // clusters of 1, 2, 4 and 8 CTAs
@@ -1512,7 +1551,7 @@ tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int
   const int64_t fills = std::max<int64_t>(1, cdiv(p.k_grouped ? cdiv(p.K, std::max<int64_t>(1, groups)) : p.K, 128 / L.el));
   const int ce = p.c_dtype == TB_F32 ? 4 : 2;
   const bool even = p.k_grouped || !p.offsets;  // every group has m rows
-  const bool sums = L.el == 1 || p.c_dtype == TB_F32;
+  const bool sums = sums_in_registers(L);
   double best = 0;
   int bn = 0, split = 1;
   bool pair = false;
@@ -1530,7 +1569,7 @@ tbStatus choose_and_launch(Launch& L, int64_t groups, int64_t rows, int sms, int
     const double near = 128.0 * (is_pair ? 256 : b + tile_rows);  // into the SM, from L2
     const double fill = std::max(std::max(512.0, near / (is_pair || b == 128 ? 46.0 : 42.0)), bytes / std::min(45.0, 23.0 / used));
     const double main = (double)cdiv(fills, s) * fill + (s > 1 ? 300.0 + 300.0 * cdiv((int64_t)tile_rows, 32) : 0.0);
-    const double store = tile_rows * b / (p.vec ? 16.0 / ce : sums && b == 256 ? 0.6 : 8.0) / (s > 1 ? s : 1);
+    const double store = tile_rows * b / (p.vec ? 16.0 / ce : !sums || b == 128 ? 8.0 : L.el == 1 ? 0.6 : 4.0) / (s > 1 ? s : 1);
     const double cycles = rounds * std::max(main, store) + std::min(main, store) + (is_pair ? 600.0 : 0.0);
     if (!bn || cycles < best) {
       best = cycles;

@@ -642,3 +642,47 @@ def test_shared_8_bit_tiles_of_one_matrix(cuda, m):
         C = tb.matmul_fp8(A, one, B, torch.ones(32, 32, device="cuda"), torch.zeros(m, 4096, device="cuda"), beta=0)
         assert torch.equal(C, want)
     tb.device_status()
+
+
+# Sums of one sign: truncated additions would all lean the same way.
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_long_weight_gradients_round_once(cuda, dtype):
+    """Four million rows. A segment of 512 of them is off by at most 2^-23 per element, the f32 sums of the segments
+    by 2^-24 each (a CTA of a cluster has an eighth of them at least, the eight are added at the end), then half a step
+    of the output."""
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(22)
+    rows, k, n, dt = 1 << 22, 64, 72, _types(dtype)
+    A = torch.rand(rows, k, generator=g, device="cuda").to(dt)
+    D = (torch.rand(rows, n, generator=g, device="cuda") / 128).to(dt)
+    off = torch.tensor([0, 5, rows], dtype=torch.int32, device="cuda")
+    G = tb.grouped_matmul_wgrad(A, D, torch.zeros(2, k, n, device="cuda", dtype=dt), off, beta=0)
+    tb.device_status()
+    for e, (lo, hi) in enumerate(((0, 5), (5, rows))):
+        ref = torch.zeros(k, n, device="cuda", dtype=torch.float64)
+        for at in range(lo, hi, 1 << 20):
+            ref += A[at:min(hi, at + (1 << 20))].double().t() @ D[at:min(hi, at + (1 << 20))].double()
+        sums = (512 * 2.0 ** -23 + (rows // 512 + 8) * 2.0 ** -24) * ref
+        tol = sums + torch.finfo(dt).eps / 2 * (ref + sums)
+        assert ((G[e].double() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("sizes,n", [([3, 2], 256), ([300, 257], 2568)])   # shared tiles, pair tiles
+def test_long_k_rounds_once(cuda, dtype, sizes, n):
+    """As the gradients above, k = 65536 (16384 for the larger): segments of 512 elements."""
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(23)
+    k, dt = 65536 if n < 1000 else 16384, _types(dtype)
+    off, ends = _offsets(sizes)
+    A = torch.rand(ends[-1], k, generator=g, device="cuda").to(dt)
+    B = (torch.rand(2, k, n, generator=g, device="cuda") / 16).to(dt)
+    C = tb.grouped_matmul(A, B, torch.zeros(ends[-1], n, device="cuda", dtype=dt), off, beta=0)
+    tb.device_status()
+    ref = _reference(A, B, torch.zeros_like(C), ends, 0)
+    sums = (512 * 2.0 ** -23 + (k // 512 + 8) * 2.0 ** -24) * ref
+    assert ((C.double() - ref).abs() <= sums + torch.finfo(dt).eps / 2 * (ref + sums)).all()

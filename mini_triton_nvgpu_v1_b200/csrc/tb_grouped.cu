@@ -180,6 +180,7 @@ struct GParams {
   void* C;
   int64_t ldc, group_c;
   GScale sa, sb;
+  int64_t budget;         // cycles until a wait gives up
   int32_t stages;         // ring depth
   int32_t seg;            // fills per accumulation in TMEM, a power of two (kinds with sums)
   int32_t split, split_log2;  // CTAs per cluster that share a tile's K range (G = 1)
@@ -646,7 +647,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
   };
   bool ok = true;  // false: a wait gave up
   auto take = [&](uint32_t site) {
-    ok = ok && warp_poll(smem_addr(&bars.tile_full[slot]), slot_phase, abort_flag, site, lane);
+    ok = ok && warp_poll(smem_addr(&bars.tile_full[slot]), slot_phase, abort_flag, site, lane, p.budget);
     return ok && field(&GTile::cols) > 0;
   };
 
@@ -693,7 +694,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
         const int32_t fix_at = grouped_k && (g.k_end - g.k0) % Cf::kMmaK != 0 && g.f1 * Cf::kKB > g.k_end - g.k0 - Cf::kMmaK
                                    ? (g.k_end - g.k0) / Cf::kKB : -1;
         for (int32_t f = g.f0; f < g.f1; ++f) {
-          if (issued >= (uint32_t)S && !warp_wait(empty0 + stage * 8, phase ^ 1u, abort_flag, kSiteProducer, lane)) {
+          if (issued >= (uint32_t)S && !warp_wait(empty0 + stage * 8, phase ^ 1u, abort_flag, kSiteProducer, lane, p.budget)) {
             ok = false;
             break;
           }
@@ -733,10 +734,13 @@ __global__ void __launch_bounds__(kThreadsG, 1)
       if (lane == 0) bars.issued = issued;
     } else if (warp == 1) {
       // ---------------------------------------------------------- MMA issuer
+      // (Issuer and fixer touch no memory, but a wait of theirs is not to count
+      // the time of the kernel before.)
       if constexpr (G == 1) {
         tmem_alloc_g<G>(smem_addr(&bars.tmem_holder), Cf::kTmemCols);
         tmem_relinquish_g<G>();
       }
+      asm volatile("griddepcontrol.wait;" ::: "memory");
       if (leader) {
         const uint32_t tmem_base = *const_cast<volatile uint32_t*>(&bars.tmem_holder);
         const uint32_t idesc = idesc_f16_f32(Cf::kBM, BN, p.a_mn ? 1 : 0, p.b_kmaj ? 0 : 1) | (p.fmt << 7) |
@@ -768,8 +772,8 @@ __global__ void __launch_bounds__(kThreadsG, 1)
             // first and last fill of an accumulation
             const bool opens = Cf::kSums ? (f & seg_mask) == 0 : f == 0;
             const bool closes = f + 1 == fills || (Cf::kSums && ((f + 1) & seg_mask) == 0);
-            if ((opens && !warp_poll(tempty0 + acc * 8, acc_phase ^ 1u, abort_flag, kSiteMma, lane)) ||
-                (!here && !warp_poll(full0 + stage * 8, phase, abort_flag, kSiteMma, lane))) {
+            if ((opens && !warp_poll(tempty0 + acc * 8, acc_phase ^ 1u, abort_flag, kSiteMma, lane, p.budget)) ||
+                (!here && !warp_poll(full0 + stage * 8, phase, abort_flag, kSiteMma, lane, p.budget))) {
               ok = false;
               break;
             }
@@ -824,6 +828,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
       }
     } else if (warp == 2) {
       // --------------------------------------------------------------- fixer
+      asm volatile("griddepcontrol.wait;" ::: "memory");
       if (p.k_grouped) {
         int stage = 0;
         uint32_t fix_phase = 0;  // bit s: parity of stage s's next fix
@@ -836,7 +841,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           const int32_t valid = min(Cf::kKB, g.k_end - (g.k0 + (g.f1 - 1) * Cf::kKB));
           stage = (stage + n) % S;
           if (valid % Cf::kMmaK == 0) continue;
-          if (!warp_wait(smem_addr(&bars.fix[last]), (fix_phase >> last) & 1u, abort_flag, kSiteFixer, lane)) {
+          if (!warp_wait(smem_addr(&bars.fix[last]), (fix_phase >> last) & 1u, abort_flag, kSiteFixer, lane, p.budget)) {
             ok = false;
             break;
           }
@@ -904,7 +909,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
         GTile tile = {};
         if (t < tiles) tile = tile_at<Cf::kBM, BN, Cf::kKB>(p, tab, t, part, cursor, lane);
         if (t == first) start();
-        if (!warp_wait(smem_addr(&bars.tile_empty[slot]), slot_phase ^ 1u, abort_flag, kSiteScheduler, lane)) break;
+        if (!warp_wait(smem_addr(&bars.tile_empty[slot]), slot_phase ^ 1u, abort_flag, kSiteScheduler, lane, p.budget)) break;
         if (lane == 0) {
           bars.tile[slot] = tile;
           mbar_arrive(smem_addr(&bars.tile_full[slot]));
@@ -981,7 +986,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
         // only the senders: a CTA without a row of its own has nothing else to
         // wait for, and a warp that went on would arrive a second time and stand
         // in for one that still reads.
-        if (!warp_poll<true>(consumed0, red_phase ^ 1u, abort_flag, kSiteCluster, lane)) return false;
+        if (!warp_poll<true>(consumed0, red_phase ^ 1u, abort_flag, kSiteCluster, lane, p.budget)) return false;
         if (warp == 4 && lane == 0)
           mbar_expect_tx(ready0, (uint32_t)(mine * p.split) * (uint32_t)((cols + 31) / 32 * 128));
         const int row = q * 32 - r0 + lane;  // of the block
@@ -1003,7 +1008,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
             }
           }
         }
-        if (!warp_poll<true>(ready0, red_phase, abort_flag, kSiteCluster, lane)) return false;
+        if (!warp_poll<true>(ready0, red_phase, abort_flag, kSiteCluster, lane, p.budget)) return false;
         for (int i = warp - 4; i < mine; i += 8) {
 #pragma unroll
           for (int h = 0; h < BN / 128; ++h) {  // four columns of each 128 to a lane
@@ -1090,7 +1095,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           if constexpr (Cf::kBytes) {
             if (left > 1) fetch();
           }
-          if (!warp_poll(smem_addr(&bars.tfull[acc]), acc_phase, abort_flag, kSiteEpilogue, lane)) {
+          if (!warp_poll(smem_addr(&bars.tfull[acc]), acc_phase, abort_flag, kSiteEpilogue, lane, p.budget)) {
             ok = false;
             break;
           }
@@ -1160,7 +1165,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
         const int32_t cols = field(&GTile::cols) - c_half;
         char* row = row_at();
         if (fills > 0) {
-          if (!warp_poll(smem_addr(&bars.tfull[acc]), acc_phase, abort_flag, kSiteEpilogue, lane)) {
+          if (!warp_poll(smem_addr(&bars.tfull[acc]), acc_phase, abort_flag, kSiteEpilogue, lane, p.budget)) {
             ok = false;
             break;
           }
@@ -1449,6 +1454,9 @@ tbStatus launch(Launch& L, int dev, cudaStream_t stream) {
   if (st == TB_OK)
     st = encode(&tb_, 3, L.b, L.el, L.bf16, p.b_kmaj ? Cf::kKB : Cf::kMnBox, p.b_kmaj ? Cf::kBnCta : Cf::kKB, "B");
   if (st != TB_OK) return st;
+  // Some waits last as long as the tiles that the scheduler may be ahead by: a
+  // second, and 4096 cycles (three to eight times what it takes) for each of their fills.
+  p.budget = kWaitBudgetCycles + (int64_t)kTileSlots * 4096 * cdiv(p.K, Cf::kKB);
   p.split_log2 = p.split == 8 ? 3 : p.split == 4 ? 2 : p.split == 2 ? 1 : 0;
   // A block holds the rows that a tile has on average, if the ring keeps three stages beside it.
   p.block = BN == 128 && L.tile_rows > 64 ? 128 : L.tile_rows > 32 ? 64 : 32;

@@ -23,14 +23,14 @@ __device__ __forceinline__ void record_error(uint32_t code, uint32_t site) {
 }
 
 // Bounded wait: false when the abort flag is up or the budget ran out.
-__device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity,
-                                             volatile int* abort_flag, uint32_t site) {
+__device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t site,
+                                             long long budget = kWaitBudgetCycles) {
   if (tb::sm100::mbar_try_wait(bar, parity)) return true;
   const long long t0 = clock64();
   while (true) {
     if (tb::sm100::mbar_try_wait(bar, parity)) return true;
     if (*abort_flag) return false;
-    if (clock64() - t0 > kWaitBudgetCycles) {
+    if (clock64() - t0 > budget) {
       record_error(TB_ERR_DEVICE_TIMEOUT, site);
       *abort_flag = 1;
       return false;
@@ -39,15 +39,15 @@ __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity,
 }
 
 // Lane 0 waits (bounded), the result is broadcast so the warp stays converged.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
-                                          uint32_t site, int lane) {
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t site,
+                                          int lane, long long budget = kWaitBudgetCycles) {
   // Every lane probes first with the non-blocking test_wait: in the common
   // case (phase already complete) that is one probe, while a blocking
   // try_wait costs hundreds of cycles even on a completed phase (measured:
   // 142 → 118 cycles per MMA for a 128×128 tile, 154 → 132 for 128×256).
   if (tb::sm100::mbar_test_wait(bar, parity)) return true;
   int ok = 0;
-  if (lane == 0) ok = wait_bounded(bar, parity, abort_flag, site);
+  if (lane == 0) ok = wait_bounded(bar, parity, abort_flag, site, budget);
   return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
@@ -56,8 +56,8 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 // try_wait wakes up hundreds of cycles after the phase completes). CLUSTER:
 // the barrier is arrived on by, or hands over data from, other CTAs of the cluster.
 template <bool CLUSTER = false>
-__device__ __forceinline__ bool warp_poll(uint32_t bar, uint32_t parity, volatile int* abort_flag,
-                                          uint32_t site, int lane) {
+__device__ __forceinline__ bool warp_poll(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t site,
+                                          int lane, long long budget = kWaitBudgetCycles) {
   auto probe = [&]() {
     if constexpr (CLUSTER) return tb::sm100::mbar_test_wait_cluster(bar, parity);
     else return tb::sm100::mbar_test_wait(bar, parity);
@@ -71,7 +71,7 @@ __device__ __forceinline__ bool warp_poll(uint32_t bar, uint32_t parity, volatil
     int stop = 0;
     if (lane == 0) {
       stop = *abort_flag;
-      if (!stop && clock64() - t0 > kWaitBudgetCycles) {
+      if (!stop && clock64() - t0 > budget) {
         record_error(TB_ERR_DEVICE_TIMEOUT, site);
         *abort_flag = stop = 1;
       }

@@ -686,3 +686,37 @@ def test_long_k_rounds_once(cuda, dtype, sizes, n):
     ref = _reference(A, B, torch.zeros_like(C), ends, 0)
     sums = (512 * 2.0 ** -23 + (k // 512 + 8) * 2.0 ** -24) * ref
     assert ((C.double() - ref).abs() <= sums + torch.finfo(dt).eps / 2 * (ref + sums)).all()
+
+
+def test_tiles_longer_than_a_second(cuda):
+    """One group has 330 million of the rows of 1000 groups, a tile of more than a second: the waits for it, and those
+    of the next call, which is on the SMs that the others left, go on. Whole numbers whose sums stay below 2^24."""
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(24)
+    sizes = [330_000_005] + [e % 3 for e in range(999)]
+    off, ends = _offsets(sizes)
+    rows = ends[-1]
+    A, D = (torch.empty(rows, 8, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    first = torch.zeros(8, 8, device="cuda", dtype=torch.float64)
+    for at in range(0, rows, 1 << 24):
+        end = min(rows, at + (1 << 24))
+        for t in (A, D):
+            t[at:end] = torch.randint(-2, 3, (end - at, 8), generator=g, device="cuda", dtype=torch.int8)
+        in_first = min(end, ends[1])
+        first += A[at:in_first].double().t() @ D[at:in_first].double()
+    ref = torch.stack([first] + [A[lo:hi].double().t() @ D[lo:hi].double() for lo, hi in zip(ends[1:], ends[2:])])
+    few, few_ends = _offsets([5, 0, 130, 40])
+    A2, B2 = _ints((175, 64), g, torch.bfloat16), _ints((4, 64, 128), g, torch.bfloat16)
+    C2 = torch.zeros(175, 128, device="cuda")
+    G = torch.zeros(1000, 8, 8, device="cuda")
+    times = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+    times[0].record()
+    tb.grouped_matmul_wgrad(A, D, G, off, beta=0)
+    tb.grouped_matmul(A2, B2, C2, few, beta=0)
+    times[1].record()
+    tb.device_status()
+    assert times[0].elapsed_time(times[1]) > 1000
+    assert torch.equal(G.double(), ref)
+    assert torch.equal(C2.double(), _reference(A2, B2, torch.zeros_like(C2), few_ends, 0))

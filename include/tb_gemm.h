@@ -442,6 +442,10 @@ tbStatus tb_device_status(void* stream, uint32_t* raw_status);
  * stays usable. No counterpart in the reference. */
 tbStatus tb_selftest_bounded_wait(void* stream, uint64_t budget_cycles);
 
+/* The same for the kernels of grouped rows and 8-bit operands, which have
+ * waits and a status word of their own; tb_device_status() reads both. */
+tbStatus tb_selftest_grouped_wait(void* stream, uint64_t budget_cycles);
+
 /* Message of the calling thread's most recent failure ("" if none). */
 const char* tb_last_error(void);
 

@@ -1285,6 +1285,20 @@ __global__ void __launch_bounds__(kThreadsG, 1)
   }
 }
 
+// Self-test of these kernels' waits: one warp polls a barrier that nothing
+// arrives on until the budget is spent, and a second wait of the same CTA then
+// sees the abort flag.
+__global__ void tb_grouped_selftest_kernel(long long budget) {
+  __shared__ __align__(8) uint64_t bars[2];
+  __shared__ int abort_flag;
+  if (threadIdx.x < 2) mbar_init(smem_addr(&bars[threadIdx.x]), 1);
+  if (threadIdx.x == 0) abort_flag = 0;
+  fence_mbar_init();
+  __syncthreads();
+  if (!warp_poll(smem_addr(&bars[0]), 0, &abort_flag, kSiteSelfTest, threadIdx.x, budget))
+    warp_wait(smem_addr(&bars[1]), 0, &abort_flag, kSiteDrain, threadIdx.x, budget);
+}
+
 // Copies rows of `row_bytes` to rows of ld_dst bytes (a multiple of 16), the
 // rest of each row zero: operands whose rows TMA cannot address. HBM bound: a
 // lane reads the one or two aligned 16-byte words that hold its 16 bytes (they
@@ -1744,6 +1758,16 @@ tbStatus tb_grouped_status(uint32_t* raw) {
   }
   *raw = v;
   return TB_OK;
+}
+
+extern "C" tbStatus tb_selftest_grouped_wait(void* stream, uint64_t budget_cycles) {
+  tb_clear_error();
+  if (budget_cycles == 0 || budget_cycles > (uint64_t)kWaitBudgetCycles)
+    return tb_fail(TB_ERR_INVALID_ARGUMENT, "budget_cycles must be in (0, 2e9]");
+  tb_grouped_selftest_kernel<<<1, 32, 0, reinterpret_cast<cudaStream_t>(stream)>>>((long long)budget_cycles);
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? TB_OK
+                          : tb_fail(TB_ERR_CUDA, std::string("tb_grouped_selftest launch: ") + cudaGetErrorString(e));
 }
 
 extern "C" tbStatus tb_grouped_desc_init(tb_grouped_desc* d) {

@@ -720,3 +720,25 @@ def test_tiles_longer_than_a_second(cuda):
     assert times[0].elapsed_time(times[1]) > 1000
     assert torch.equal(G.double(), ref)
     assert torch.equal(C2.double(), _reference(A2, B2, torch.zeros_like(C2), few_ends, 0))
+
+
+def test_expired_wait_is_reported(cuda):
+    """A wait of these kernels that runs out: the status says so once, both status words are cleared, and the context
+    stays usable."""
+    import ctypes
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    from mini_triton_nvgpu_v1_b200 import _capi
+    lib, raw = _capi.load(), ctypes.c_uint32()
+    assert tb.device_status() == 0
+    for both in (False, True):
+        assert lib.tb_selftest_grouped_wait(None, 2_000_000) == 0       # ~1 ms of SM clocks
+        if both:
+            assert lib.tb_selftest_bounded_wait(None, 2_000_000) == 0
+        assert lib.tb_device_status(None, ctypes.byref(raw)) == _capi.TB_ERR_DEVICE_TIMEOUT
+        assert raw.value >> 16 == _capi.TB_ERR_DEVICE_TIMEOUT << 8 | 5   # the first wait that gave up
+        assert tb.device_status() == 0
+    off, ends = _offsets([3, 5])
+    A, B = torch.ones(8, 64, device="cuda").half(), torch.ones(2, 64, 64, device="cuda").half()
+    assert (tb.grouped_matmul(A, B, torch.zeros(8, 64, device="cuda"), off) == 64).all()
+    assert tb.device_status() == 0

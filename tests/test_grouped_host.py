@@ -195,3 +195,8 @@ def test_known_calls_take_whole_numbers_only():
     t = torch.zeros(2, 2)
     for beta in (0.5, 1.0, None, 1 << 80, "1"):
         assert grouped._call0(grouped._ROWS, t, t, t, t, beta, 0) == -1
+
+
+def test_selftest_budget_is_validated(lib):
+    assert lib.tb_selftest_grouped_wait(None, 0) == INVALID
+    assert lib.tb_selftest_grouped_wait(None, 3_000_000_000) == INVALID

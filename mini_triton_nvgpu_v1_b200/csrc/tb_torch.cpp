@@ -32,6 +32,7 @@ namespace {
 
 enum Op : int { kRows = 0, kWgrad = 1, kQuantize = 2, kBytes = 3, kRowsBytes = 4, kOps = 5 };
 constexpr int kTensors[kOps] = {4, 4, 3, 5, 6};
+constexpr unsigned kOutputs[kOps] = {1u << 2, 1u << 2, 1u << 1 | 1u << 2, 1u << 4, 1u << 4};  // bit i: tensor i is written
 
 // The C ABI, handed over by the binding that loaded the library.
 struct {
@@ -116,7 +117,9 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (c10::cuda::current_device() != k.device) return PyLong_FromLong(-1);
     void* stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)k.device).stream();
     void* p[kMaxTensors];
-    for (int j = 0; j < kTensors[op]; ++j) p[j] = const_cast<void*>(t[j]->const_data_ptr());
+    // A written tensor that shares its storage until then (copy on write) gets its own here.
+    for (int j = 0; j < kTensors[op]; ++j)
+      p[j] = kOutputs[op] >> j & 1 ? t[j]->mutable_data_ptr() : const_cast<void*>(t[j]->const_data_ptr());
     size_t need = 0;
     if (op == kWgrad) need = g_abi.need_wgrad(&k.d, p[0], k.a[0], p[1], k.a[1]);
     else if (op != kQuantize)

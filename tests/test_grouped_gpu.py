@@ -742,3 +742,33 @@ def test_expired_wait_is_reported(cuda):
     A, B = torch.ones(8, 64, device="cuda").half(), torch.ones(2, 64, 64, device="cuda").half()
     assert (tb.grouped_matmul(A, B, torch.zeros(8, 64, device="cuda"), off) == 64).all()
     assert tb.device_status() == 0
+
+
+def test_outputs_that_share_storage_until_written(cuda):
+    """A lazy clone as the output of a call like an earlier one: its source keeps what it held."""
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(25)
+    off, ends = _offsets([9, 0, 30])
+    A, B = _ints((39, 64), g, torch.bfloat16), _ints((3, 64, 128), g, torch.bfloat16)
+    D = _ints((39, 128), g, torch.bfloat16)
+    one, f8 = torch.ones(39, 1, device="cuda"), torch.float8_e4m3fn
+    SB, W = torch.ones(3, 1, 1, device="cuda"), _ints((64, 128), g, torch.bfloat16)
+    X = torch.randn(39, 128, generator=g, device="cuda")
+    calls = {
+        "rows": (lambda o: tb.grouped_matmul(A, B, *o, off), [torch.zeros(39, 128, device="cuda")]),
+        "wgrad": (lambda o: tb.grouped_matmul_wgrad(A, D, *o, off), [torch.zeros(3, 64, 128, device="cuda")]),
+        "quantize": (lambda o: tb.quantize_fp8(X, *o), [torch.zeros(39, 128, device="cuda").to(f8), torch.zeros(39, 1, device="cuda")]),
+        "fp8": (lambda o: tb.matmul_fp8(A.to(f8), one, W.to(f8), SB[0], *o), [torch.zeros(39, 128, device="cuda")]),
+        "rows fp8": (lambda o: tb.grouped_matmul_fp8(A.to(f8), one, B.to(f8), SB, *o, off), [torch.zeros(39, 128, device="cuda")]),
+    }
+    for name, (call, source) in calls.items():
+        plain = [s.clone() for s in source]
+        call(plain)
+        for _ in range(2):
+            lazy = [torch._lazy_clone(s) for s in source]
+            call(lazy)
+            assert not any(s.float().any() for s in source), name
+            assert all(torch.equal(x.float(), y.float()) for x, y in zip(lazy, plain)), name
+    tb.device_status()

@@ -18,8 +18,10 @@ device memory and streams.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import json
 from dataclasses import dataclass, field, asdict
+from pathlib import Path
 from typing import Optional
 
 from . import _capi
@@ -45,8 +47,11 @@ class _LazyLib:
 
 _lib = _LazyLib()
 
-__all__ = ["KernelConfig", "MatmulPlan", "DynamicMatmulPlan", "TBError", "matmul", "plan_for", "version", "lib",
-           "grouped_matmul", "grouped_matmul_wgrad", "quantize_fp8", "matmul_fp8", "grouped_matmul_fp8"]
+__all__ = ["KernelConfig", "MatmulPlan", "DynamicMatmulPlan", "TBError", "matmul", "plan_for", "version", "lib"]
+_GROUPED = ("grouped_matmul", "grouped_matmul_wgrad", "quantize_fp8", "matmul_fp8", "grouped_matmul_fp8")
+# of a star import only where they can be had: it works without torch too
+if importlib.util.find_spec("torch") is not None and (Path(__file__).parent / "_tbtorch.so").exists():
+    __all__ += _GROUPED
 
 _REDUCTION = {None: TB_REDUCTION_UNSET, "": TB_REDUCTION_UNSET,
               "split_k_serial": TB_REDUCTION_SPLIT_K_SERIAL,
@@ -407,9 +412,6 @@ def device_status(stream=None) -> int:
     code = _lib.tb_device_status(C.c_void_p(s.cuda_stream or None), C.byref(raw))
     _check(code)
     return raw.value
-
-
-_GROUPED = ("grouped_matmul", "grouped_matmul_wgrad", "quantize_fp8", "matmul_fp8", "grouped_matmul_fp8")
 
 
 def __getattr__(name):

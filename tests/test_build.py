@@ -2,6 +2,8 @@
 from __future__ import annotations
 
 import importlib.util
+import subprocess
+import sys
 
 import pytest
 
@@ -52,3 +54,14 @@ def test_another_torch_or_python_is_built_for_anew(commands):
 def test_a_failed_command_is_named():
     with pytest.raises(RuntimeError, match="false failed"):
         build._run(["false"], False)
+
+
+@pytest.mark.parametrize("torch", [True, False])
+def test_star_import(torch):
+    """All names with torch; without it the ones that do not need it."""
+    code = ("import sys\n" + ("" if torch else "sys.modules['torch'] = None\n") +
+            "from mini_triton_nvgpu_v1_b200 import *\n"
+            "assert matmul and plan_for and KernelConfig and version()\n"
+            f"assert ('grouped_matmul' in globals()) is {torch}\n")
+    r = subprocess.run([sys.executable, "-c", code], cwd=build.ROOT, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr

@@ -413,8 +413,11 @@ tbStatus tb_grouped_matmul_blockscaled(const tb_grouped_desc* desc, const void* 
                                        size_t workspace_bytes, void* stream);
 
 /* ---- 8-bit operands ----
- * m = max(max |block|, 448 · 2^-63), S = m / 448, Q = e4m3(448 · X / m), the
- * quotient rounded to nearest, ties to even. X: batch matrices of rows × cols
+ * m = max(max |block|, 448 · 2^-63), S = m / 448, Q = e4m3(448 · X / m). Of
+ * f16 and bf16 X the exact quotient is rounded to nearest, ties to even. Of f32
+ * X 0.4375 · X and its quotient by m / 1024 are rounded to f32 on the way: a
+ * quotient that lies within 2^-22 of its size from the border of two e4m3 values
+ * may go to either. X: batch matrices of rows × cols
  * (f32, f16 or bf16), row stride ldx; Q: e4m3, row stride ldq; S: f32,
  * ceil(rows / block_rows) × ceil(cols / block_cols) with strides s_row and
  * s_col. Matrices of the batch lie stride_x, stride_q and stride_s elements

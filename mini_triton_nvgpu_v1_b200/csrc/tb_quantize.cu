@@ -21,7 +21,9 @@
 // product with a rounded 1 / m would send them either way. One residual step
 // (Markstein, 1990: q' = q + r·(a − b·q), r = 1 / b) gives the division's
 // result for two more multiply-adds per element. 448 and m enter as 0.4375
-// and m / 1024: 0.4375 X is exact for 16-bit X and never overflows.
+// and m / 1024: 0.4375 X is exact for 16-bit X and never overflows. Of f32 X it
+// is rounded, and the quotient is rounded to f32 before it is to e4m3 (2^-24 and
+// 2^-23): one that lies that near to a border may go to either side.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

@@ -255,7 +255,9 @@ def _blocks(n: int) -> int:
 def quantize_fp8(X, Q=None, S=None, *, block=(1, 128), stream=None):
     """Q ← e4m3(448 · X / m), S ← m / 448 with m = max(max|block|, 448 · 2^-63)
     for every block (1, 128), (128, 1) or (128, 128) of X [rows, cols] or
-    [batch, rows, cols] (f32, f16 or bf16). Q: float8_e4m3fn of X's shape; S:
+    [batch, rows, cols] (f32, f16 or bf16). The exact quotient of f16 and bf16
+    values is rounded to nearest, ties to even; of f32 values one within 2^-22
+    of the border of two e4m3 values may go to either. Q: float8_e4m3fn of X's shape; S:
     f32 [(batch,) ceil(rows / block[0]), ceil(cols / block[1])]. A Q that is
     not given is made with rows that begin on 16-byte boundaries, as the
     8-bit products read them without a copy; what is not given belongs to

@@ -439,3 +439,24 @@ def test_scales_that_overlap_are_refused(cuda):
     Q = torch.empty(4, 256, dtype=torch.float8_e4m3fn, device="cuda")
     with pytest.raises(tb.TBError, match="overlap"):
         tb.quantize_fp8(X, Q, torch.empty(4, 1, device="cuda").expand(4, 2))
+
+
+@pytest.mark.parametrize("block", [(1, 128), (128, 1), (128, 128)])
+def test_quantize_f32_off_the_nearest_only_at_borders(cuda, block):
+    """0.4375·X is off by 2^-24 and the quotient by 2^-23 at most: where Q is not the nearest e4m3 value, it is the one
+    on the other side of a border that lies within 2^-22 of the exact quotient."""
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    x = torch.randn(2048, 4096, generator=_gen(40), device="cuda")
+    # quotients near a border: multiples of 1/16 of powers of two, a few f32 steps off
+    x[:, ::2] = torch.ldexp(torch.randint(16, 32, (2048, 2048), generator=_gen(41), device="cuda").float() / 16,
+                            torch.randint(-4, 5, (2048, 2048), generator=_gen(42), device="cuda"))
+    x[:, ::2] *= 1 + 2.0 ** -23 * torch.randint(-3, 4, (2048, 2048), generator=_gen(43), device="cuda").float()
+    x[::128, ::128] = 448.0 * (1 + 2.0 ** -20)
+    Q, S = tb.quantize_fp8(x, block=block)
+    q, s = _quantized64(x, *block)
+    assert torch.equal(S, s.float())
+    over = s.repeat_interleave(block[0], 0).repeat_interleave(block[1], 1)
+    v, off = x.double() / over, Q.double() != q
+    border = (Q.double() + q) / 2
+    assert ((v - border).abs()[off] <= 2.0 ** -22 * v.abs()[off]).all()

@@ -772,3 +772,47 @@ def test_outputs_that_share_storage_until_written(cuda):
             assert not any(s.float().any() for s in source), name
             assert all(torch.equal(x.float(), y.float()) for x, y in zip(lazy, plain)), name
     tb.device_status()
+
+
+@pytest.mark.parametrize("out", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("sizes,widths", [([3, 0, 130, 33], [1, 33, 130, 383]), ([300, 700, 1, 513], [2567, 2306])])
+def test_outputs_of_segments_off_vector_boundaries(cuda, out, sizes, widths):
+    """As test_outputs_off_vector_boundaries, K long enough for sums of segments; one-CTA tiles and pairs."""
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(26)
+    dt, k = getattr(torch, out), 1100
+    off, ends = _offsets(sizes, 1)
+    rows = ends[-1] + 2
+    A = torch.zeros(rows, 1104, device="cuda", dtype=torch.float16)[:, :k]
+    A.copy_(_ints((rows, k), g, torch.float16, 1))
+    for n, skip, pad, beta in itertools.product(widths, [0, 1, 3, 8], [0, 1, 2], [0, 1]):
+        whole = _ints((rows + 1, skip + n + pad), g, dt, 7)
+        C, want = whole[:rows, skip:skip + n], whole.clone()
+        B = _ints((4, (n + 7) // 8 * 8, 1104), g, torch.float16, 1)[:, :n, :k].transpose(1, 2)
+        want[:rows, skip:skip + n] = _reference(A, B, C, ends, beta).to(dt)
+        tb.grouped_matmul(A, B, C, off, beta=beta)
+        assert torch.equal(whole, want), (n, skip, pad, beta)
+    tb.device_status()
+
+
+@pytest.mark.parametrize("out", ["float32", "float16"])
+def test_weight_gradients_of_segments_off_vector_boundaries(cuda, out):
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(27)
+    dt = getattr(torch, out)
+    for (k, sizes), n, pad, beta in itertools.product([(72, [3, 0, 1300, 33]), (1000, [1100, 7, 0, 1500])], [33, 257, 2049],
+                                                      [0, 1], [0, 1]):
+        off, ends = _offsets(sizes)
+        A = _ints((ends[-1], k), g, torch.float16, 1)
+        D = _ints((ends[-1], (n + 7) // 8 * 8), g, torch.float16, 1)[:, :n]
+        whole = _ints((4, k, n + pad), g, dt, 7)
+        G, want = whole[:, :, pad:], whole.clone()
+        ref = torch.stack([A[lo:hi].double().t() @ D[lo:hi].double() for lo, hi in zip(ends, ends[1:])])
+        want[:, :, pad:] = (ref + beta * G.double()).to(dt)
+        tb.grouped_matmul_wgrad(A, D, G, off, beta=beta)
+        assert torch.equal(whole, want), (k, n, pad, beta)
+    tb.device_status()

@@ -341,8 +341,10 @@ tbStatus tb_matmul(const tb_matmul_desc* desc, const void* A, int64_t lda,
  * dimension or group stride) are first copied into `workspace`, 256-byte
  * aligned; the *_workspace_bytes functions say how much that takes for the
  * operands that they are given (0 in the ordinary case, then workspace may be
- * NULL). Sums are in f32; the output is rounded once. Results repeat bit for
- * bit (no atomics). beta = 0 does not read the output. An output may not
+ * NULL). Sums are in f32: of 512 (f32 outputs) or 1024 elements of k (16-bit
+ * outputs; 8-bit operands: 128) in the tensor cores' accumulator, which truncates
+ * as it adds, of such segments rounded to nearest; the output is rounded once.
+ * Results repeat bit for bit (no atomics). beta = 0 does not read the output. An output may not
  * overlap an operand, nor its groups' matrices each other. Kernels are
  * launched with programmatic stream serialization: their set-up may run
  * while the kernel before them in the stream ends, their work does not. */

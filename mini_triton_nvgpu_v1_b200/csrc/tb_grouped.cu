@@ -37,17 +37,19 @@
 // cluster, which add their partial sums through distributed shared memory in
 // a fixed order — no workspace, no atomics, results repeat bit for bit.
 //
-// What bounds it (B200, 148 SMs; times of single calls in a CUDA graph):
+// What bounds it (B200, 148 SMs; "burst": a few calls after a pause, at 1965 MHz;
+// in a loop the power cap lowers the clock):
 // * Training sizes: the operands' way from L2 into the SMs, 43–46 bytes a cycle
 //   and SM for 32 KB per fill of a 256 × 256 pair tile (the MMAs of a fill
 //   need 512 cycles), and below that the power cap: 16384 rows over 8 experts
-//   of 4096 × 4096 bf16 in 380 µs (1450 TFLOP/s), 1220 in a sustained loop.
+//   of 4096 × 4096 bf16 in 387 µs in a burst (1420 TFLOP/s), 455 in a loop.
 // * 8-bit products: besides, the epilogue takes 64 KB of sums per block and
-//   CTA out of TMEM: 8192³ e4m3 in 490 µs (2240 TFLOP/s; 437 µs with the
-//   epilogue's arithmetic left out).
+//   CTA out of TMEM, 1140 cycles a block: 8192³ e4m3 in 494 µs in a burst (2230
+//   TFLOP/s; 437 µs with the epilogue's arithmetic left out), 580 in a loop.
+//   With a scale per column (weight gradients) 952 and 954.
 // * Decoding steps: HBM, once the weights flow (6.2 TB/s), and some 4 µs of
 //   start and end around it: offsets, first tile, first fill, exchange.
-//   96 rows over 32 experts of 2048 × 1408 f16 (179 MB): 35.5 µs.
+//   96 rows over 32 experts of 2048 × 1408 f16 (179 MB): 38 µs in a CUDA graph.
 //
 // Every wait is bounded, as in the dense GEMM.
 #include <cuda.h>
@@ -1550,9 +1552,12 @@ tbStatus resident_clusters(int dev, int sms, int (&out)[4]) {
 
 // Tile and K split, by estimated cycles. `rows`: mean rows of a group that has any.
 //
-// One ring fill takes 512 cycles of MMAs whatever the tile's width: a
-// tcgen05.mma of 128 (or a pair's 256) rows was measured at 118–132 cycles for
-// 64, 128 and 256 columns alike, so a narrower tile only lowers the rate. A
+// One ring fill takes 512 cycles of MMAs whatever the tile's width: the loop
+// took 118–132 cycles per tcgen05.mma of 128 (or a pair's 256) rows, barriers
+// included, for 64, 128 and 256 columns alike (the instruction by itself was not
+// measured), so a narrower tile only lowers the rate of this loop. The pass of
+// the epilogue over each 8-bit accumulation (1140 cycles at 256 columns) has no
+// term here. A
 // fill takes longer where its bytes do: 23 bytes a cycle and SM are an SM's
 // share of HBM, 45 the most that one SM was seen to draw while others idle,
 // and L2 feeds all SMs together 46 bytes a cycle each (42 where a CTA takes

@@ -18,7 +18,10 @@ The gradients of ``C = grouped_matmul(A, B)`` for a gradient D of C are
 ``grouped_matmul(D, B.transpose(1, 2), dA, offsets)`` and
 ``grouped_matmul_wgrad(A, D, dB, offsets)``; those of ``matmul_fp8`` are
 ``matmul_fp8`` of D quantised along n with B.t(), and of A^T with D, both
-quantised in blocks of 128 rows (``block=(128, 1)``).
+quantised in blocks of 128 rows (``block=(128, 1)``). The gradient of the rows
+of ``grouped_matmul_fp8`` is the same call on ``B.transpose(1, 2)`` and
+``SB.transpose(1, 2)``; that of its weights takes 16-bit rows
+(``grouped_matmul_wgrad``).
 """
 from __future__ import annotations
 

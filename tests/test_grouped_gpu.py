@@ -816,3 +816,71 @@ def test_weight_gradients_of_segments_off_vector_boundaries(cuda, out):
         tb.grouped_matmul_wgrad(A, D, G, off, beta=beta)
         assert torch.equal(whole, want), (k, n, pad, beta)
     tb.device_status()
+
+
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("sizes,n,k", [([100, 1, 2], 2048, 1024), ([8, 8, 8], 2048, 1024), ([130, 70], 2048, 1024),
+                                       ([1000] + [0] * 7, 1001, 1024), ([120, 3, 2, 3], 2048, 4096), ([120, 70, 2], 2048, 8192),
+                                       ([100] + [1] * 23, 2048, 4096), ([1] * 12 + [128] + [2] * 11, 2048, 4096)])
+def test_shared_tiles_of_uneven_groups(cuda, sizes, n, k, out):
+    """Tiles of more rows than are exchanged at a time, before and behind tiles of fewer."""
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(28)
+    off, ends = _offsets(sizes)
+    A, B = _ints((ends[-1], k), g, torch.bfloat16, 2), _ints((len(sizes), n, k), g, torch.bfloat16, 2).transpose(1, 2)
+    C = _ints((ends[-1], n), g, _types(out), 7)
+    want = [_reference(A, B, C, ends, beta).to(C.dtype) for beta in (0, 1)]
+    for i in range(40):
+        got = C.clone()
+        tb.grouped_matmul(A, B, got, off, beta=i % 2)
+        assert torch.equal(got, want[i % 2]), i
+    tb.device_status()
+
+
+@pytest.mark.parametrize("groups,k,n,rows", [(8, 100, 1408, 2500), (100, 70, 384, 4000), (12, 128, 128, 3000)])
+@pytest.mark.parametrize("out", ["f32", "f16"])
+def test_shared_weight_gradients_of_many_rows(cuda, groups, k, n, rows, out):
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(29)
+    off, ends = _offsets([rows + 7 * e % 11 for e in range(groups)])
+    A, D = _ints((ends[-1], (k + 7) // 8 * 8), g, torch.float16, 2)[:, :k], _ints((ends[-1], n), g, torch.float16, 2)
+    G = _ints((groups, k, n), g, _types(out), 7)
+    ref = torch.stack([A[lo:hi].double().t() @ D[lo:hi].double() for lo, hi in zip(ends, ends[1:])])
+    want = [ref.to(G.dtype), (ref + G.double()).to(G.dtype)]
+    for i in range(40):
+        got = G.clone()
+        tb.grouped_matmul_wgrad(A, D, got, off, beta=i % 2)
+        assert torch.equal(got, want[i % 2]), i
+    tb.device_status()
+
+
+def test_two_graphs_at_once(cuda):
+    """Two captured graphs of calls that repack their operands and share tiles, replayed on two streams at once."""
+    import torch
+    import mini_triton_nvgpu_v1_b200 as tb
+    g = torch.Generator(device="cuda")
+    g.manual_seed(30)
+    off, ends = _offsets([9, 0, 40, 3])
+    sets = []
+    for k in (1025, 2047):
+        A, B = _ints((ends[-1], k), g, torch.float16, 2), _ints((4, k, 520), g, torch.float16, 2)
+        C = torch.zeros(ends[-1], 520, device="cuda")
+        tb.grouped_matmul(A, B, C, off, beta=0)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(3):
+                tb.grouped_matmul(A, B, C, off, beta=0)
+        sets.append((A, B, C, graph, torch.cuda.Stream()))
+    for _ in range(20):
+        for A, B, C, graph, s in sets:
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for A, B, C, _, _ in sets:
+        assert torch.equal(C.double(), _reference(A, B, torch.zeros_like(C), ends, 0))
+    tb.device_status()

@@ -846,7 +846,7 @@ __global__ void __launch_bounds__(kThreadsG, 1)
           const int32_t valid = min(Cf::kKB, g.k_end - (g.k0 + (g.f1 - 1) * Cf::kKB));
           stage = (stage + n) % S;
           if (valid % Cf::kMmaK == 0) continue;
-          if (!warp_wait(smem_addr(&bars.fix[last]), (fix_phase >> last) & 1u, abort_flag, kSiteFixer, lane, p.budget)) {
+          if (!warp_poll(smem_addr(&bars.fix[last]), (fix_phase >> last) & 1u, abort_flag, kSiteFixer, lane, p.budget)) {
             ok = false;
             break;
           }

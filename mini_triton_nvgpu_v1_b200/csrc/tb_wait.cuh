@@ -45,7 +45,9 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   // case (phase already complete) that is one probe, while a blocking
   // try_wait costs hundreds of cycles even on a completed phase (measured:
   // 142 → 118 cycles per MMA for a 128×128 tile, 154 → 132 for 128×256).
-  if (tb::sm100::mbar_test_wait(bar, parity)) return true;
+  // The warp goes by one answer: lanes that saw different ones would part here
+  // and wait for each other at two instructions.
+  if (__all_sync(0xffffffffu, tb::sm100::mbar_test_wait(bar, parity))) return true;
   int ok = 0;
   if (lane == 0) ok = wait_bounded(bar, parity, abort_flag, site, budget);
   return __shfl_sync(0xffffffffu, ok, 0) != 0;

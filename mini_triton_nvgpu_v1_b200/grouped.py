@@ -12,7 +12,7 @@ adds to it; ``beta=0`` overwrites) on the current stream of its device, and
 return it. Offsets stay on the device: no call waits for the GPU, and a captured
 CUDA graph follows their contents. Operands are strided views; rows that
 do not begin on 16-byte boundaries are copied first (into ``workspace``, or a
-buffer from torch's allocator).
+buffer from torch's allocator). An output may not overlap an operand.
 
 The gradients of ``C = grouped_matmul(A, B)`` for a gradient D of C are
 ``grouped_matmul(D, B.transpose(1, 2), dA, offsets)`` and
